@@ -1,0 +1,129 @@
+// Device helpers of the 8-bit operators: types, loads of eight values, sums over
+// the threads of a row.
+#pragma once
+
+#include "q8_shim.h"
+
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+namespace q8 {
+
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef int i32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x2 __attribute__((ext_vector_type(2)));
+typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+// the same at any address: the memory pipeline takes vector accesses at byte
+// alignment, so rows may start anywhere
+typedef u32x4 u32x4_at2 __attribute__((aligned(2)));
+typedef f32x4 f32x4_at4 __attribute__((aligned(4)));
+typedef u32x2 u32x2_at1 __attribute__((aligned(1)));
+typedef u32x4 u32x4_at1 __attribute__((aligned(1)));
+
+template <int DT> struct Type;
+template <> struct Type<Q8_F32> {
+    typedef float T;
+    static __device__ __forceinline__ float get(const T* p) { return *p; }
+    static __device__ __forceinline__ void put(T* p, float x) { *p = x; }
+    static __device__ __forceinline__ float round(float x) { return x; }
+    static __device__ __forceinline__ void load8(const T* p, float (&v)[8]) {
+        const f32x4 a = *reinterpret_cast<const f32x4_at4*>(p), b = *reinterpret_cast<const f32x4_at4*>(p + 4);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) { v[e] = a[e]; v[4 + e] = b[e]; }
+    }
+    static __device__ __forceinline__ void store8(T* p, const float (&v)[8]) {
+        *reinterpret_cast<f32x4_at4*>(p) = f32x4{v[0], v[1], v[2], v[3]};
+        *reinterpret_cast<f32x4_at4*>(p + 4) = f32x4{v[4], v[5], v[6], v[7]};
+    }
+};
+template <> struct Type<Q8_F16> {
+    typedef _Float16 T;
+    static __device__ __forceinline__ float get(const T* p) { return (float)*p; }
+    static __device__ __forceinline__ void put(T* p, float x) { *p = (T)x; }
+    static __device__ __forceinline__ float round(float x) { return (float)(T)x; }
+    static __device__ __forceinline__ void load8(const T* p, float (&v)[8]) {
+        const u32x4 w = *reinterpret_cast<const u32x4_at2*>(p);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const f16x2 h = __builtin_bit_cast(f16x2, (uint32_t)w[e]);
+            v[2 * e] = (float)h[0];
+            v[2 * e + 1] = (float)h[1];
+        }
+    }
+    static __device__ __forceinline__ uint32_t pair(float x, float y) {
+        const f16x2 h = {(_Float16)x, (_Float16)y};
+        return __builtin_bit_cast(uint32_t, h);
+    }
+    static __device__ __forceinline__ void store8(T* p, const float (&v)[8]) {
+        *reinterpret_cast<u32x4_at2*>(p) = u32x4{pair(v[0], v[1]), pair(v[2], v[3]), pair(v[4], v[5]), pair(v[6], v[7])};
+    }
+};
+template <> struct Type<Q8_BF16> {
+    typedef __bf16 T;
+    static __device__ __forceinline__ float get(const T* p) { return (float)*p; }
+    static __device__ __forceinline__ void put(T* p, float x) { *p = (T)x; }
+    static __device__ __forceinline__ float round(float x) { return (float)(T)x; }
+    static __device__ __forceinline__ void load8(const T* p, float (&v)[8]) {
+        const u32x4 w = *reinterpret_cast<const u32x4_at2*>(p);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            v[2 * e] = __builtin_bit_cast(float, (uint32_t)(w[e] << 16));
+            v[2 * e + 1] = __builtin_bit_cast(float, (uint32_t)(w[e] & 0xffff0000u));
+        }
+    }
+    static __device__ __forceinline__ uint32_t pair(float x, float y) {
+        const f32x2 v = {x, y};
+        return __builtin_bit_cast(uint32_t, __builtin_convertvector(v, bf16x2));
+    }
+    static __device__ __forceinline__ void store8(T* p, const float (&v)[8]) {
+        *reinterpret_cast<u32x4_at2*>(p) = u32x4{pair(v[0], v[1]), pair(v[2], v[3]), pair(v[4], v[5]), pair(v[6], v[7])};
+    }
+};
+
+// Eight values of a row from column c; those past `cols` are 0 (c < cols).
+template <int DT>
+__device__ __forceinline__ void load_part(const typename Type<DT>::T* row, uint32_t c, uint32_t cols, float (&v)[8]) {
+    if (cols - c >= 8) {
+        Type<DT>::load8(row + c, v);
+    } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = c + e < cols ? Type<DT>::get(row + c + e) : 0.0f;
+    }
+}
+template <int DT>
+__device__ __forceinline__ void store_part(typename Type<DT>::T* row, uint32_t c, uint32_t cols, const float (&v)[8]) {
+    if (cols - c >= 8) {
+        Type<DT>::store8(row + c, v);
+    } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+            if (c + e < cols) Type<DT>::put(row + c + e, v[e]);
+    }
+}
+
+// |x| as an integer that orders like it, infinities and then NaN last.
+__device__ __forceinline__ uint32_t magnitude(float x) { return __builtin_bit_cast(uint32_t, x) & 0x7fffffffu; }
+
+template <int CTRL> __device__ __forceinline__ uint32_t dpp(uint32_t x) {
+    return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, CTRL, 0xf, 0xf, true);
+}
+
+// Sum of f and maximum of u over a wave, in every lane, in a fixed order.
+__device__ __forceinline__ void wave_sum_max(float& f, uint32_t& u) {
+    auto step = [&](uint32_t fo, uint32_t uo) __attribute__((always_inline)) {
+        f += __builtin_bit_cast(float, fo);
+        u = u > uo ? u : uo;
+    };
+    auto bits = [&]() __attribute__((always_inline)) { return __builtin_bit_cast(uint32_t, f); };
+    step(dpp<0xb1>(bits()), dpp<0xb1>(u));     // lane ^ 1
+    step(dpp<0x4e>(bits()), dpp<0x4e>(u));     // lane ^ 2
+    step(dpp<0x141>(bits()), dpp<0x141>(u));   // the other four of eight
+    step(dpp<0x140>(bits()), dpp<0x140>(u));   // the other eight of sixteen
+    step((uint32_t)__shfl_xor((int)bits(), 16), (uint32_t)__shfl_xor((int)u, 16));
+    step((uint32_t)__shfl_xor((int)bits(), 32), (uint32_t)__shfl_xor((int)u, 32));
+}
+
+}  // namespace q8

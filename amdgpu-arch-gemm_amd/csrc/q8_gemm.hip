@@ -1,0 +1,410 @@
+// Products of the 8-bit operators on the matrix cores (gfx950).
+//
+// product_kernel: D = A B^T for rows that hold the summed index, in 8-bit
+// integers (int32 sums) or 16-bit floats (FP32 sums).  All three have operands of 16
+// bytes a lane and rows of 128 bytes a K tile, so one kernel serves them:
+//   HBM --buffer_load ... lds, 16 bytes a lane--> LDS, two buffers --> MFMA
+// few_kernel: few tokens; the weights go from memory to the matrix cores once.
+#include "q8_device.hpp"
+#include "q8_internal.hpp"
+#include "q8_plan.hpp"
+
+namespace q8 {
+namespace {
+
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+
+constexpr int BUFFER_RSRC_WORD3 = 0x00020000;
+constexpr int CPOL_SC1 = 0x10;
+constexpr int XCDS = 8;
+constexpr uint32_t NOWHERE = 0x80000000u;    // an offset past every descriptor's end: loads give 0
+constexpr int KB = kTileBytes;
+
+template <int E> struct Atom;
+template <> struct Atom<E_I8> {
+    typedef i32x4 Acc;
+    static __device__ __forceinline__ Acc mfma(u32x4 a, u32x4 b, Acc c) {
+        return __builtin_amdgcn_mfma_i32_16x16x64_i8(__builtin_bit_cast(i32x4, a), __builtin_bit_cast(i32x4, b), c, 0, 0, 0);
+    }
+};
+template <> struct Atom<E_F16> {
+    typedef f32x4 Acc;
+    static __device__ __forceinline__ Acc mfma(u32x4 a, u32x4 b, Acc c) {
+        return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+    }
+};
+template <> struct Atom<E_BF16> {
+    typedef f32x4 Acc;
+    static __device__ __forceinline__ Acc mfma(u32x4 a, u32x4 b, Acc c) {
+        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+    }
+};
+
+// Workgroups go round the XCDs one by one: consecutive tiles to one XCD instead, so that
+// its L2 serves their shared rows.
+__device__ __forceinline__ uint32_t xcd_order(uint32_t id, uint32_t total) {
+    const uint32_t x = id % XCDS, q = total / XCDS, r = total % XCDS;
+    return x * q + (x < r ? x : r) + id / XCDS;
+}
+// Tiles in groups of eight rows of them, column by column within a group.
+__device__ __forceinline__ void tile_of(uint32_t z, uint32_t nx, uint32_t ny, uint32_t& tx, uint32_t& ty) {
+    constexpr uint32_t GROUP = 8;
+    const uint32_t group = z / (GROUP * ny), first = group * GROUP;
+    const uint32_t width = min(nx - first, GROUP), in = z - group * GROUP * ny;
+    tx = first + in % width;
+    ty = in / width;
+}
+
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t rows_rsrc(const void* base, uint64_t ld, uint32_t row0, uint32_t rows,
+                                                            uint32_t kb) {
+    // a last piece of less than 16 bytes is read whole: it starts at a multiple of 16,
+    // so the bytes past the matrix lie in the same page
+    const uint64_t left = (uint64_t)(rows - 1 - row0) * ld + ((kb + 15u) & ~15u);
+    return __builtin_amdgcn_make_buffer_rsrc((void*)((const char*)base + (uint64_t)row0 * ld), (short)0,
+                                             (int)(left < 0x7fffffffu ? left : 0x7fffffffu), BUFFER_RSRC_WORD3);
+}
+
+// 1024 bytes, 16 a lane, to LDS from `lds` on: the assembly form, since the
+// compiler would wait for it before every read of LDS.  The barrier of the next K tile waits.
+// (m0 needs no clobber: it is reserved, and set right before each use.)
+__device__ __forceinline__ void load_lds(__amdgpu_buffer_rsrc_t rsrc, uint32_t lds, uint32_t voff, uint32_t soff) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds"
+                 :: "s"(lds), "v"(voff), "s"(rsrc), "s"(soff));
+}
+
+__device__ __forceinline__ float out_value(int v) { return (float)v; }
+__device__ __forceinline__ float out_value(float v) { return v; }
+
+// Eight outputs of a row, or those that the matrix still has.
+template <int DT>
+__device__ __forceinline__ void put_out(const Product& p, uint64_t row, uint32_t col, float (&v)[8]) {
+    typedef typename Type<DT>::T T;
+    T* y = (T*)p.y + row * p.ldy;
+    if (p.accumulate) {
+        float old[8];
+        load_part<DT>(y, col, p.n, old);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] += old[e];
+    }
+    store_part<DT>(y, col, p.n, v);
+}
+template <int DT> __device__ __forceinline__ float bias_of(const Product& p, uint32_t col) {
+    return Type<DT>::get((const typename Type<DT>::T*)p.bias + col);
+}
+__device__ __forceinline__ float bias_at(const Product& p, uint32_t col) {
+    return p.out == Q8_F32 ? bias_of<Q8_F32>(p, col) : p.out == Q8_F16 ? bias_of<Q8_F16>(p, col) : bias_of<Q8_BF16>(p, col);
+}
+
+// WM x WN waves of TM x TN tiles of 16 x 16.
+template <int E, int WM, int WN, int TM, int TN, int OCC>
+__global__ void __launch_bounds__(WM * WN * 64, OCC) product_kernel(const Product p) {
+    typedef Atom<E> A;
+    typedef typename A::Acc Acc;
+    constexpr int WAVES = WM * WN, BM = WM * TM * 16, BN = WN * TN * 16;
+    constexpr int LA = BM / 8 / WAVES, LB = BN / 8 / WAVES;     // loads of 8 rows a wave and K tile
+    constexpr int STAGE = (BM + BN) * KB;
+    constexpr int OUTP = TN * 16 + 4;                           // floats of a staged row of D
+    constexpr int OUT = WAVES * 16 * OUTP * 4;
+    constexpr int LDS = 2 * STAGE > OUT ? 2 * STAGE : OUT;
+    __shared__ __attribute__((aligned(128))) unsigned char lds[LDS];
+
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int wm = wave % WM, wn = wave / WM;
+    uint32_t tx, ty;
+    const uint32_t total = p.nwgx * p.nwgy;
+    tile_of(xcd_order(blockIdx.x, total), p.nwgx, p.nwgy, tx, ty);
+    const uint32_t row0 = tx * BM, col0 = ty * BN;
+    const uint32_t tiles_k = (p.kb + KB - 1) / KB;
+    const uint32_t k_first = blockIdx.y * p.tiles_per_split;
+    const uint32_t k_last = min(k_first + p.tiles_per_split, tiles_k);
+
+    const __amdgpu_buffer_rsrc_t ra = rows_rsrc(p.a, p.lda, row0, p.m, p.kb), rb = rows_rsrc(p.b, p.ldb, col0, p.n, p.kb);
+    const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) unsigned char*)lds;
+
+    // Row r of a tile keeps its piece c of 16 bytes at piece c ^ (r & 7): the
+    // eight lanes that read one piece of eight rows at a time meet all banks.  A load's
+    // lanes fill LDS in order, so it is the address in memory that is permuted.
+    const uint32_t lr = (uint32_t)lane >> 3, lc = ((uint32_t)lane & 7u) ^ lr;
+    uint32_t va[LA], vb[LB];
+#pragma unroll
+    for (int i = 0; i < LA; ++i) va[i] = (uint32_t)((i * WAVES + wave) * 8 + lr) * (uint32_t)p.lda + lc * 16u;
+#pragma unroll
+    for (int i = 0; i < LB; ++i) vb[i] = (uint32_t)((i * WAVES + wave) * 8 + lr) * (uint32_t)p.ldb + lc * 16u;
+
+    auto issue = [&](uint32_t kt, uint32_t buf) __attribute__((always_inline)) {
+        const uint32_t soff = kt * KB, at = lds0 + buf * STAGE;
+        const bool have = soff + lc * 16u < p.kb;   // pieces past the rows' end are zeros
+#pragma unroll
+        for (int i = 0; i < LA; ++i) load_lds(ra, at + (uint32_t)(i * WAVES + wave) * 1024u, have ? va[i] : NOWHERE, soff);
+#pragma unroll
+        for (int i = 0; i < LB; ++i)
+            load_lds(rb, at + BM * KB + (uint32_t)(i * WAVES + wave) * 1024u, have ? vb[i] : NOWHERE, soff);
+    };
+
+    Acc acc[TM][TN];
+#pragma unroll
+    for (int i = 0; i < TM; ++i)
+#pragma unroll
+        for (int j = 0; j < TN; ++j) acc[i][j] = Acc{0, 0, 0, 0};
+
+    const int fr = lane & 15, fg = lane >> 4;
+    const uint32_t fa = (uint32_t)(wm * TM * 16 + fr) * KB, fb = (uint32_t)(BM + wn * TN * 16 + fr) * KB;
+    const uint32_t fc = ((uint32_t)fg ^ ((uint32_t)fr & 7u)) * 16u;
+
+    auto compute = [&](uint32_t buf) __attribute__((always_inline)) {
+        const unsigned char* at = lds + buf * STAGE;
+#pragma unroll
+        for (int s = 0; s < 2; ++s) {
+            u32x4 a[TM], b[TN];
+            const uint32_t c = fc ^ (uint32_t)(s * 64);
+#pragma unroll
+            for (int j = 0; j < TN; ++j) b[j] = *reinterpret_cast<const u32x4*>(at + fb + j * 16 * KB + c);
+#pragma unroll
+            for (int i = 0; i < TM; ++i) a[i] = *reinterpret_cast<const u32x4*>(at + fa + i * 16 * KB + c);
+#pragma unroll
+            for (int i = 0; i < TM; ++i)
+#pragma unroll
+                for (int j = 0; j < TN; ++j) acc[i][j] = A::mfma(b[j], a[i], acc[i][j]);
+        }
+    };
+
+    if (k_first < k_last) {
+        issue(k_first, 0);
+        uint32_t buf = 0;
+        for (uint32_t kt = k_first; kt < k_last; ++kt, buf ^= 1) {
+            // this tile has landed, and every wave has read the last one
+            asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+            if (kt + 1 < k_last) issue(kt + 1, buf ^ 1);
+            if (E == E_I8 && (p.kb & 15u) && kt + 1 == tiles_k) {
+                // the last piece ends inside: A's bytes past the sum are cleared, and
+                // what B has there is multiplied by zero
+                if (tid < BM) {
+                    const uint32_t c = (p.kb % KB) / 16u, have = p.kb & 15u;
+                    uint32_t* piece = reinterpret_cast<uint32_t*>(lds + buf * STAGE + tid * KB + ((c ^ (tid & 7u)) * 16u));
+#pragma unroll
+                    for (uint32_t e = 0; e < 4; ++e) {
+                        const uint32_t bytes = have > 4u * e ? min(have - 4u * e, 4u) : 0u;
+                        if (bytes < 4u) piece[e] &= (1u << (8u * bytes)) - 1u;
+                    }
+                }
+                __syncthreads();
+            }
+            compute(buf);
+        }
+    }
+
+    // The K ranges meet: partial sums go past the XCD's L2, the last work-group of a tile
+    // to arrive adds them in range order.
+    if (p.splits > 1) {
+        constexpr uint32_t PART = BM * BN * 4;
+        const uint32_t tile = tx + ty * p.nwgx;
+        char* ws = (char*)p.partial + (uint64_t)tile * p.splits * PART;
+        auto part = [&](uint32_t s) __attribute__((always_inline)) {
+            return __builtin_amdgcn_make_buffer_rsrc(ws + (uint64_t)s * PART, (short)0, (int)PART, BUFFER_RSRC_WORD3);
+        };
+        const __amdgpu_buffer_rsrc_t mine = part(blockIdx.y);
+#pragma unroll
+        for (int i = 0; i < TM; ++i)
+#pragma unroll
+            for (int j = 0; j < TN; ++j)
+                __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, acc[i][j]), mine,
+                                                       ((i * TN + j) * WAVES * 64 + tid) * 16, 0, CPOL_SC1);
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        __shared__ uint32_t arrived;
+        __syncthreads();
+        if (tid == 0) arrived = __hip_atomic_fetch_add(p.tickets + tile, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        __syncthreads();
+        if (arrived + 1 != p.splits) return;
+        for (uint32_t s = 0; s < p.splits; ++s) {
+            const __amdgpu_buffer_rsrc_t r = part(s);
+#pragma unroll
+            for (int i = 0; i < TM; ++i)
+#pragma unroll
+                for (int j = 0; j < TN; ++j) {
+                    const Acc v = __builtin_bit_cast(
+                        Acc, __builtin_amdgcn_raw_buffer_load_b128(r, ((i * TN + j) * WAVES * 64 + tid) * 16, 0, CPOL_SC1));
+                    acc[i][j] = s ? acc[i][j] + v : v;
+                }
+        }
+        if (tid == 0) __hip_atomic_store(p.tickets + tile, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    }
+
+    // D: a lane holds four consecutive columns of a row; each wave turns 16 rows at a
+    // time in its own part of LDS into whole pieces of rows.
+    const uint32_t wrow = row0 + (uint32_t)(wm * TM * 16), wcol = col0 + (uint32_t)(wn * TN * 16);
+    float factor = 1.0f;
+    if (E == E_F16 && p.alpha) factor = p.alpha[1];
+    __syncthreads();
+    float* stage = reinterpret_cast<float*>(lds) + wave * 16 * OUTP;
+#pragma unroll
+    for (int i = 0; i < TM; ++i) {
+        const float sx = E == E_I8 ? p.sx[min(wrow + (uint32_t)(i * 16 + fr), p.m - 1)] : factor;
+#pragma unroll
+        for (int j = 0; j < TN; ++j) {
+            f32x4 v;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                v[e] = out_value(acc[i][j][e]) * sx;
+                if constexpr (E == E_I8) {
+                    const uint32_t c = min(wcol + (uint32_t)(j * 16 + fg * 4 + e), p.n - 1);
+                    v[e] = v[e] * p.sw[c] + (p.bias ? bias_at(p, c) : 0.0f);
+                }
+            }
+            *reinterpret_cast<f32x4*>(stage + fr * OUTP + j * 16 + fg * 4) = v;
+        }
+        __builtin_amdgcn_wave_barrier();
+        constexpr int LPR = TN * 2, RPI = 64 / LPR;             // lanes to a row of eights, rows at once
+#pragma unroll
+        for (int q = 0; q < 16 / RPI; ++q) {
+            const int r = q * RPI + lane / LPR, c = lane % LPR * 8;
+            float v[8];
+#pragma unroll
+            for (int e = 0; e < 8; e += 4) {
+                const f32x4 w = *reinterpret_cast<const f32x4*>(stage + r * OUTP + c + e);
+#pragma unroll
+                for (int k = 0; k < 4; ++k) v[e + k] = w[k];
+            }
+            const uint32_t row = wrow + (uint32_t)(i * 16 + r), col = wcol + (uint32_t)c;
+            if (row < p.m && col < p.n) {
+                if (p.out == Q8_F32) put_out<Q8_F32>(p, row, col, v);
+                else if (E != E_BF16 && p.out == Q8_F16) put_out<Q8_F16>(p, row, col, v);
+                else if (E != E_F16) put_out<Q8_BF16>(p, row, col, v);
+            }
+        }
+        __builtin_amdgcn_wave_barrier();
+    }
+}
+
+// Few tokens (m <= 64).  A work-group owns 16 * NT channels and all of K, in
+// steps of 64 bytes that its waves take in runs of RUN; each lane's weights go from
+// memory straight into an operand.  The waves' sums meet in LDS.
+template <int MT, int NT, int WAVES>
+__global__ void __launch_bounds__(WAVES * 64) few_kernel(const Product p) {
+    constexpr int RUN = 4;
+    typedef Atom<E_I8> A;
+    __shared__ __attribute__((aligned(16))) i32x4 red[WAVES][MT * NT][64];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+    const int fr = lane & 15, fg = lane >> 4;
+    const uint32_t col0 = blockIdx.x * (16 * NT);
+    const uint32_t whole = p.kb / 64;             // steps without an end inside
+    const char* w[NT];
+    const char* x[MT];
+    bool wok[NT], xok[MT];
+#pragma unroll
+    for (int j = 0; j < NT; ++j) {
+        const uint32_t c = col0 + (uint32_t)(j * 16 + fr);
+        wok[j] = c < p.n;
+        w[j] = (const char*)p.b + (uint64_t)(wok[j] ? c : 0u) * p.ldb + fg * 16;
+    }
+#pragma unroll
+    for (int i = 0; i < MT; ++i) {
+        const uint32_t r = (uint32_t)(i * 16 + fr);
+        xok[i] = r < p.m;
+        x[i] = (const char*)p.a + (uint64_t)(xok[i] ? r : 0u) * p.lda + fg * 16;
+    }
+    i32x4 acc[MT][NT];
+#pragma unroll
+    for (int i = 0; i < MT; ++i)
+#pragma unroll
+        for (int j = 0; j < NT; ++j) acc[i][j] = i32x4{0, 0, 0, 0};
+    const u32x4 zero = {0, 0, 0, 0};
+    for (uint32_t s0 = (uint32_t)wave * RUN; s0 < whole; s0 += WAVES * RUN) {
+        u32x4 wv[RUN][NT], xv[RUN][MT];
+#pragma unroll
+        for (int s = 0; s < RUN; ++s) {
+            const uint64_t at = (uint64_t)(s0 + s) * 64;
+            const bool on = s0 + s < whole;
+#pragma unroll
+            for (int j = 0; j < NT; ++j) wv[s][j] = on && wok[j] ? (u32x4)*reinterpret_cast<const u32x4_at1*>(w[j] + at) : zero;
+#pragma unroll
+            for (int i = 0; i < MT; ++i) xv[s][i] = on && xok[i] ? (u32x4)*reinterpret_cast<const u32x4_at1*>(x[i] + at) : zero;
+        }
+#pragma unroll
+        for (int s = 0; s < RUN; ++s)
+#pragma unroll
+            for (int i = 0; i < MT; ++i)
+#pragma unroll
+                for (int j = 0; j < NT; ++j) acc[i][j] = A::mfma(wv[s][j], xv[s][i], acc[i][j]);
+    }
+    if (p.kb % 64 && wave == WAVES - 1) {   // the rest, byte by byte
+        const uint32_t k0 = whole * 64 + fg * 16;
+        u32x4 wv[NT], xv[MT];
+        auto bytes = [&](const char* s, bool ok) __attribute__((always_inline)) {
+            u32x4 v = zero;
+#pragma unroll
+            for (int e = 0; e < 16; ++e)
+                if (ok && k0 + e < p.kb) v[e / 4] |= (uint32_t)(uint8_t)s[(uint64_t)whole * 64 + e] << (8 * (e % 4));
+            return v;
+        };
+#pragma unroll
+        for (int j = 0; j < NT; ++j) wv[j] = bytes(w[j], wok[j]);
+#pragma unroll
+        for (int i = 0; i < MT; ++i) xv[i] = bytes(x[i], xok[i]);
+#pragma unroll
+        for (int i = 0; i < MT; ++i)
+#pragma unroll
+            for (int j = 0; j < NT; ++j) acc[i][j] = A::mfma(wv[j], xv[i], acc[i][j]);
+    }
+#pragma unroll
+    for (int i = 0; i < MT; ++i)
+#pragma unroll
+        for (int j = 0; j < NT; ++j) red[wave][i * NT + j][lane] = acc[i][j];
+    __syncthreads();
+    for (int t = wave; t < MT * NT; t += WAVES) {
+        i32x4 v = red[0][t][lane];
+#pragma unroll
+        for (int k = 1; k < WAVES; ++k) v += red[k][t][lane];
+        const uint32_t row = (uint32_t)(t / NT * 16 + fr), col = col0 + (uint32_t)(t % NT * 16 + fg * 4);
+        if (row >= p.m) continue;
+        const float sx = p.sx[row];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const uint32_t c = col + e;
+            if (c >= p.n) break;
+            const float y = (float)v[e] * sx * p.sw[c] + (p.bias ? bias_at(p, c) : 0.0f);
+            const uint64_t at = row * p.ldy + c;
+            if (p.out == Q8_F32) ((float*)p.y)[at] = y;
+            else if (p.out == Q8_F16) ((_Float16*)p.y)[at] = (_Float16)y;
+            else ((__bf16*)p.y)[at] = (__bf16)y;
+        }
+    }
+}
+
+hipError_t launch(const void* f, dim3 grid, uint32_t threads, const Product& p, hipStream_t stream) {
+    void* args[] = {const_cast<Product*>(&p)};
+    return hipLaunchKernel(f, grid, dim3(threads), args, 0, stream);
+}
+
+template <int E> hipError_t product_any(const Route& r, Product p, hipStream_t s) {
+    const Tile& t = kTiles[r.kind];
+    p.nwgx = (uint32_t)ceil_div(p.m, t.m);
+    p.nwgy = (uint32_t)ceil_div(p.n, t.n);
+    p.splits = r.splits;
+    p.tiles_per_split = (uint32_t)ceil_div(ceil_div(p.kb, KB), r.splits);
+    const dim3 grid(p.nwgx * p.nwgy, r.splits);
+    if (r.kind == 0) return launch((const void*)&product_kernel<E, 2, 4, 8, 4, 2>, grid, 512, p, s);
+    return launch((const void*)&product_kernel<E, 2, 2, 4, 4, 2>, grid, 256, p, s);
+}
+
+template <int MT> hipError_t few_any(const Product& p, hipStream_t s) {
+    constexpr int WAVES = 16;
+    return launch((const void*)&few_kernel<MT, 1, WAVES>, dim3((uint32_t)ceil_div(p.n, 16)), WAVES * 64, p, s);
+}
+
+}  // namespace
+
+hipError_t launch_product(Element e, const Route& r, const Product& p, hipStream_t s) {
+    return e == E_I8 ? product_any<E_I8>(r, p, s) : e == E_F16 ? product_any<E_F16>(r, p, s) : product_any<E_BF16>(r, p, s);
+}
+
+hipError_t launch_few(const Product& p, hipStream_t s) {
+    return p.m <= 16 ? few_any<1>(p, s) : p.m <= 32 ? few_any<2>(p, s) : few_any<4>(p, s);
+}
+
+hipError_t prepare_products() {
+    hipFuncAttributes a;
+    return hipFuncGetAttributes(&a, (const void*)&product_kernel<E_I8, 2, 2, 4, 4, 2>);
+}
+
+}  // namespace q8

@@ -1,0 +1,120 @@
+// Interface between the 8-bit operators' host code (q8_shim.cpp) and their
+// kernels (q8_rows.hip, q8_pack.hip, q8_gemm.hip).  Nothing here is part of
+// the C-ABI.
+#pragma once
+
+#include "q8_shim.h"
+
+#include <hip/hip_runtime_api.h>
+
+#include <cstddef>
+#include <cstdint>
+
+#define Q8_INTERNAL __attribute__((visibility("hidden")))
+
+namespace q8 {
+
+inline uint32_t type_bytes(int dtype) { return dtype == Q8_F32 ? 4u : 2u; }
+inline uint64_t ceil_div(uint64_t a, uint64_t b) { return (a + b - 1) / b; }
+
+// Rows of `cols` values at `ld` elements.
+struct Quantize {
+    const void* x;
+    int8_t* q;
+    float* scale;
+    uint32_t ldx, ldq, rows, cols;
+    // the norm's (residual, hidden, rstd may be null)
+    const void* residual;
+    const void* gain;
+    void* hidden;
+    float* rstd;
+    uint32_t ldr, ldh;
+    float eps;
+};
+Q8_INTERNAL hipError_t launch_quantize(int dtype, bool norm, const Quantize& p, hipStream_t stream);
+
+struct Dequantize {
+    const int8_t* q;
+    const float* scale;
+    void* y;
+    uint32_t ldq, ldy, rows, cols;
+};
+Q8_INTERNAL hipError_t launch_dequantize(int dtype, const Dequantize& p, hipStream_t stream);
+
+struct NormBackward {
+    const void* dn;
+    const void* hidden;
+    const void* gain;
+    const float* rstd;
+    const void* dres;     // may be null
+    void* dx;
+    float* dgain;         // may be null
+    float* partial;       // parts x cols, where dgain is wanted
+    uint32_t lddn, ldh, lddr, lddx, rows, cols, parts;
+};
+// Row ranges that the gain's gradient is summed over first.
+Q8_INTERNAL uint32_t norm_backward_parts(uint32_t rows, uint32_t cols);
+Q8_INTERNAL hipError_t launch_norm_backward(int dtype, const NormBackward& p, hipStream_t stream);
+
+// What the matrix cores multiply.
+enum Element { E_I8 = 0, E_F16 = 1, E_BF16 = 2 };
+
+// One product D = A B^T: rows of A and of B hold the summed index, `kb` bytes of it.
+struct Product {
+    const void* a;
+    const void* b;
+    uint64_t lda, ldb;    // bytes
+    uint32_t m, n, kb;
+    const float* sx;      // E_I8: scales of A's and B's rows
+    const float* sw;
+    const void* bias;     // E_I8: of type `out`, may be null
+    const float* alpha;   // E_F16: a factor in device memory; null: 1
+    void* y;
+    uint64_t ldy;         // elements
+    int out;
+    int accumulate;
+    // set by the launcher
+    uint32_t nwgx, nwgy, splits, tiles_per_split, vec;
+    void* partial;
+    uint32_t* tickets;
+};
+
+// How a product runs: `kind` of q8_plan.hpp, and the K ranges.
+struct Route {
+    int kind;
+    uint32_t splits;
+};
+Q8_INTERNAL hipError_t launch_product(Element e, const Route& r, const Product& p, hipStream_t stream);
+Q8_INTERNAL hipError_t launch_few(const Product& p, hipStream_t stream);   // E_I8, m <= 64
+Q8_INTERNAL hipError_t prepare_products();   // loads the kernels on the current device
+
+// 8-bit rows to rows of whole 16 bytes: dst[r][0 .. cols) and zeros up to dst_ld.
+Q8_INTERNAL hipError_t launch_copy_rows(const int8_t* src, uint64_t src_ld, int8_t* dst, uint64_t dst_ld, uint32_t rows,
+                                        uint32_t cols, hipStream_t stream);
+// dst[j][t * cp + c] = scale_c q_cj (times pair[0] where pair is not null) in `e`
+// for c < rows, 0 up to cp; E_BF16 with terms == 3: q_cj alone, three times.
+struct PackWeights {
+    const int8_t* q;
+    const float* scale;   // null: 1
+    const float* pair;
+    void* dst;
+    uint64_t ldq, dst_ld; // dst_ld in elements
+    uint32_t rows, cols, cp, terms;
+};
+Q8_INTERNAL hipError_t launch_pack_weights(Element e, const PackWeights& p, hipStream_t stream);
+// dst[i][t * cp + c] = term t of src_ic (transposed: src_ci), scaled by scale_c
+// where scale is not null, 0 up to cp.  16-bit types: one term, copied.  F32: three
+// BF16 terms.
+struct PackGradient {
+    const void* src;
+    const float* scale;
+    void* dst;
+    uint64_t src_ld, dst_ld;  // elements
+    uint32_t rows, cols, cp;  // rows: of dst; cols: values of the summed index
+    int transposed;
+};
+Q8_INTERNAL hipError_t launch_pack_gradient(int dtype, const PackGradient& p, hipStream_t stream);
+// pair[0] = 2^-e, pair[1] = 2^e with the largest finite scale * 2^-e in [2^7, 2^8)
+Q8_INTERNAL hipError_t launch_scale_pair(const float* scale, uint32_t count, float* pair, hipStream_t stream);
+
+}  // namespace q8
