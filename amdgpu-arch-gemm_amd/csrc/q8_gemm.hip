@@ -24,20 +24,29 @@ constexpr int KB = kTileBytes;
 template <int E> struct Atom;
 template <> struct Atom<E_I8> {
     typedef i32x4 Acc;
-    static __device__ __forceinline__ Acc mfma(u32x4 a, u32x4 b, Acc c) {
-        return __builtin_amdgcn_mfma_i32_16x16x64_i8(__builtin_bit_cast(i32x4, a), __builtin_bit_cast(i32x4, b), c, 0, 0, 0);
+    static __device__ __forceinline__ void mfma(u32x4 a, u32x4 b, Acc& c) {
+        c = __builtin_amdgcn_mfma_i32_16x16x64_i8(__builtin_bit_cast(i32x4, a), __builtin_bit_cast(i32x4, b), c, 0, 0, 0);
+    }
+    static __device__ __forceinline__ void mfma_agpr(u32x4 a, u32x4 b, Acc& c) {
+        asm("v_mfma_i32_16x16x64_i8 %0, %1, %2, %0" : "+a"(c) : "v"(a), "v"(b));
     }
 };
 template <> struct Atom<E_F16> {
     typedef f32x4 Acc;
-    static __device__ __forceinline__ Acc mfma(u32x4 a, u32x4 b, Acc c) {
-        return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+    static __device__ __forceinline__ void mfma(u32x4 a, u32x4 b, Acc& c) {
+        c = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+    }
+    static __device__ __forceinline__ void mfma_agpr(u32x4 a, u32x4 b, Acc& c) {
+        asm("v_mfma_f32_16x16x32_f16 %0, %1, %2, %0" : "+a"(c) : "v"(a), "v"(b));
     }
 };
 template <> struct Atom<E_BF16> {
     typedef f32x4 Acc;
-    static __device__ __forceinline__ Acc mfma(u32x4 a, u32x4 b, Acc c) {
-        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+    static __device__ __forceinline__ void mfma(u32x4 a, u32x4 b, Acc& c) {
+        c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+    }
+    static __device__ __forceinline__ void mfma_agpr(u32x4 a, u32x4 b, Acc& c) {
+        asm("v_mfma_f32_16x16x32_bf16 %0, %1, %2, %0" : "+a"(c) : "v"(a), "v"(b));
     }
 };
 
@@ -65,30 +74,23 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t rows_rsrc(const void* base, ui
                                              (int)(left < 0x7fffffffu ? left : 0x7fffffffu), BUFFER_RSRC_WORD3);
 }
 
-// 1024 bytes, 16 a lane, to LDS from `lds` on: the assembly form, since the
-// compiler would wait for it before every read of LDS.  The barrier of the next K tile waits.
-// (m0 needs no clobber: it is reserved, and set right before each use.)
-__device__ __forceinline__ void load_lds(__amdgpu_buffer_rsrc_t rsrc, uint32_t lds, uint32_t voff, uint32_t soff) {
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds"
-                 :: "s"(lds), "v"(voff), "s"(rsrc), "s"(soff));
+// 1024 bytes, 16 a lane, to LDS from `lds` + at on; soff then moves on by `step`.  The
+// assembly form, since the compiler would wait for it before every read of LDS; the
+// barrier of the next K tile waits.  (m0 needs no clobber: it is reserved, and set
+// right before each use; the addition between the two is the wait state it needs.)
+__device__ __forceinline__ void load_lds(__amdgpu_buffer_rsrc_t rsrc, uint32_t lds, int at, uint32_t voff, uint32_t& soff,
+                                         uint32_t step) {
+    uint32_t from;
+    asm volatile("s_add_u32 m0, %2, %6\n\ts_mov_b32 %0, %1\n\ts_add_u32 %1, %1, %5\n\tbuffer_load_dwordx4 %3, %4, %0 offen lds"
+                 : "=&s"(from), "+s"(soff) : "s"(lds), "v"(voff), "s"(rsrc), "s"(step), "i"(at) : "scc");
 }
+
+template <bool V> struct Flag { static constexpr bool value = V; };
+template <int V> struct Int { static constexpr int value = V; };
 
 __device__ __forceinline__ float out_value(int v) { return (float)v; }
 __device__ __forceinline__ float out_value(float v) { return v; }
 
-// Eight outputs of a row, or those that the matrix still has.
-template <int DT>
-__device__ __forceinline__ void put_out(const Product& p, uint64_t row, uint32_t col, float (&v)[8]) {
-    typedef typename Type<DT>::T T;
-    T* y = (T*)p.y + row * p.ldy;
-    if (p.accumulate) {
-        float old[8];
-        load_part<DT>(y, col, p.n, old);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] += old[e];
-    }
-    store_part<DT>(y, col, p.n, v);
-}
 template <int DT> __device__ __forceinline__ float bias_of(const Product& p, uint32_t col) {
     return Type<DT>::get((const typename Type<DT>::T*)p.bias + col);
 }
@@ -96,13 +98,20 @@ __device__ __forceinline__ float bias_at(const Product& p, uint32_t col) {
     return p.out == Q8_F32 ? bias_of<Q8_F32>(p, col) : p.out == Q8_F16 ? bias_of<Q8_F16>(p, col) : bias_of<Q8_BF16>(p, col);
 }
 
-// WM x WN waves of TM x TN tiles of 16 x 16.
-template <int E, int WM, int WN, int TM, int TN, int OCC>
-__global__ void __launch_bounds__(WM * WN * 64, OCC) product_kernel(const Product p) {
+// 2 x 2 waves of T x T tiles of 16 x 16: 256 x 256 outputs with T = 8, one wave a SIMD,
+// or 128 x 128 with T = 4, two work-groups a CU.
+//
+// A K tile is two steps of 64 bytes.  While one step is multiplied, the next one's
+// operands are read from LDS between the matrix instructions; a tile's buffer is
+// free once its second step has been read, in the middle of the tile, and takes the
+// tile after next then.  So there is one barrier a tile, and a load has the time of a whole
+// tile to land.
+template <int E, int T, int OCC>
+__global__ void __launch_bounds__(256, OCC) product_kernel(const Product p) {
     typedef Atom<E> A;
     typedef typename A::Acc Acc;
-    constexpr int WAVES = WM * WN, BM = WM * TM * 16, BN = WN * TN * 16;
-    constexpr int LA = BM / 8 / WAVES, LB = BN / 8 / WAVES;     // loads of 8 rows a wave and K tile
+    constexpr int TM = T, TN = T, WAVES = 4, BM = 2 * T * 16, BN = BM;
+    constexpr int LOADS = BM / 8 / WAVES;                       // of 8 rows a wave, K tile and operand
     constexpr int STAGE = (BM + BN) * KB;
     constexpr int OUTP = TN * 16 + 4;                           // floats of a staged row of D
     constexpr int OUT = WAVES * 16 * OUTP * 4;
@@ -110,7 +119,7 @@ __global__ void __launch_bounds__(WM * WN * 64, OCC) product_kernel(const Produc
     __shared__ __attribute__((aligned(128))) unsigned char lds[LDS];
 
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int wm = wave % WM, wn = wave / WM;
+    const int wm = wave & 1, wn = wave >> 1;
     uint32_t tx, ty;
     const uint32_t total = p.nwgx * p.nwgy;
     tile_of(xcd_order(blockIdx.x, total), p.nwgx, p.nwgy, tx, ty);
@@ -126,20 +135,22 @@ __global__ void __launch_bounds__(WM * WN * 64, OCC) product_kernel(const Produc
     // eight lanes that read one piece of eight rows at a time meet all banks.  A load's
     // lanes fill LDS in order, so it is the address in memory that is permuted.
     const uint32_t lr = (uint32_t)lane >> 3, lc = ((uint32_t)lane & 7u) ^ lr;
-    uint32_t va[LA], vb[LB];
-#pragma unroll
-    for (int i = 0; i < LA; ++i) va[i] = (uint32_t)((i * WAVES + wave) * 8 + lr) * (uint32_t)p.lda + lc * 16u;
-#pragma unroll
-    for (int i = 0; i < LB; ++i) vb[i] = (uint32_t)((i * WAVES + wave) * 8 + lr) * (uint32_t)p.ldb + lc * 16u;
-
-    auto issue = [&](uint32_t kt, uint32_t buf) __attribute__((always_inline)) {
-        const uint32_t soff = kt * KB, at = lds0 + buf * STAGE;
-        const bool have = soff + lc * 16u < p.kb;   // pieces past the rows' end are zeros
-#pragma unroll
-        for (int i = 0; i < LA; ++i) load_lds(ra, at + (uint32_t)(i * WAVES + wave) * 1024u, have ? va[i] : NOWHERE, soff);
-#pragma unroll
-        for (int i = 0; i < LB; ++i)
-            load_lds(rb, at + BM * KB + (uint32_t)(i * WAVES + wave) * 1024u, have ? vb[i] : NOWHERE, soff);
+    const uint32_t lda = (uint32_t)p.lda, ldb = (uint32_t)p.ldb;
+    const uint32_t va = (uint32_t)(wave * 8 + lr) * lda + lc * 16u, vb = (uint32_t)(wave * 8 + lr) * ldb + lc * 16u;
+    const uint32_t stepa = WAVES * 8u * lda, stepb = WAVES * 8u * ldb;
+    uint32_t ua = 0, ub = 0, sa = 0, sb = 0, at = 0;    // of the tile that is being loaded
+    auto aim = [&](uint32_t kt, uint32_t buf) __attribute__((always_inline)) {
+        // pieces past the rows' end, and tiles past the range, are zeros
+        sa = sb = kt * KB;
+        const bool have = kt < k_last && sa + lc * 16u < p.kb;
+        ua = have ? va : NOWHERE;
+        ub = have ? vb : NOWHERE;
+        at = lds0 + buf * STAGE + (uint32_t)wave * 1024u;
+    };
+    auto load = [&](int i) __attribute__((always_inline)) {     // 0 .. 2 * LOADS - 1, A and B in turn
+        const int r = i / 2 * (WAVES * 1024);
+        if (i & 1) load_lds(rb, at, BM * KB + r, ub, sb, stepb);
+        else load_lds(ra, at, r, ua, sa, stepa);
     };
 
     Acc acc[TM][TN];
@@ -149,48 +160,59 @@ __global__ void __launch_bounds__(WM * WN * 64, OCC) product_kernel(const Produc
         for (int j = 0; j < TN; ++j) acc[i][j] = Acc{0, 0, 0, 0};
 
     const int fr = lane & 15, fg = lane >> 4;
-    const uint32_t fa = (uint32_t)(wm * TM * 16 + fr) * KB, fb = (uint32_t)(BM + wn * TN * 16 + fr) * KB;
     const uint32_t fc = ((uint32_t)fg ^ ((uint32_t)fr & 7u)) * 16u;
-
-    auto compute = [&](uint32_t buf) __attribute__((always_inline)) {
-        const unsigned char* at = lds + buf * STAGE;
+    const uint32_t fa = (uint32_t)(wm * TM * 16 + fr) * KB + fc, fb = (uint32_t)(BM + wn * TN * 16 + fr) * KB + fc;
+    struct Step {
+        u32x4 a[TM], b[TN];
+    };
+    Step f0, f1;
+    auto read = [&](Step& f, uint32_t buf, uint32_t s, int i) __attribute__((always_inline)) {   // 0 .. TM + TN - 1
+        const unsigned char* from = lds + buf * STAGE;
+        if (i < TN) f.b[i] = *reinterpret_cast<const u32x4*>(from + (fb ^ (s * 64)) + i * 16 * KB);
+        else f.a[i - TN] = *reinterpret_cast<const u32x4*>(from + (fa ^ (s * 64)) + (i - TN) * 16 * KB);
+    };
+    // One step's products, the next step's operands and, in the second step, a tile's loads
+    // between them.
+    auto multiply = [&](const Step& f, Step& next, uint32_t buf, uint32_t s, auto loads) __attribute__((always_inline)) {
+        constexpr int N = TM * TN, GAP = N / (TM + TN) - 1, EVERY = N / (2 * LOADS);
 #pragma unroll
-        for (int s = 0; s < 2; ++s) {
-            u32x4 a[TM], b[TN];
-            const uint32_t c = fc ^ (uint32_t)(s * 64);
+        for (int i = 0; i < TM; ++i)
 #pragma unroll
-            for (int j = 0; j < TN; ++j) b[j] = *reinterpret_cast<const u32x4*>(at + fb + j * 16 * KB + c);
+            for (int j = 0; j < TN; ++j) {
+                const int x = i * TN + j;
+                if (x % GAP == 0 && x / GAP < TM + TN) read(next, buf, s, x / GAP);
+                if (decltype(loads)::value && x % EVERY == EVERY - 1) load(x / EVERY);
+                if constexpr (T == 8) A::mfma_agpr(f.b[j], f.a[i], acc[i][j]);
+                else A::mfma(f.b[j], f.a[i], acc[i][j]);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+    };
+    if (k_first < k_last) {
+        aim(k_first, 0);
 #pragma unroll
-            for (int i = 0; i < TM; ++i) a[i] = *reinterpret_cast<const u32x4*>(at + fa + i * 16 * KB + c);
+        for (int i = 0; i < 2 * LOADS; ++i) load(i);
+        aim(k_first + 1, 1);
+#pragma unroll
+        for (int i = 0; i < 2 * LOADS; ++i) load(i);
+        asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" :: "i"(2 * LOADS) : "memory");
+#pragma unroll
+        for (int i = 0; i < TM + TN; ++i) read(f0, 0, 0, i);
+        uint32_t buf = 0;
+        for (uint32_t kt = k_first; kt < k_last; ++kt, buf ^= 1) {
+            multiply(f0, f1, buf, 1, Flag<false>{});
+            // every wave has read this tile, and the next one has landed
+            asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+            aim(kt + 2, buf);
+            multiply(f1, f0, buf ^ 1, 0, Flag<true>{});
+        }
+        // zeros for tiles past the range; and the last products, whose results the
+        // compiler does not know to wait for
+        asm volatile("s_waitcnt vmcnt(0)\n\ts_nop 15\n\ts_nop 15" ::: "memory");
+        if constexpr (T == 8) {
 #pragma unroll
             for (int i = 0; i < TM; ++i)
 #pragma unroll
-                for (int j = 0; j < TN; ++j) acc[i][j] = A::mfma(b[j], a[i], acc[i][j]);
-        }
-    };
-
-    if (k_first < k_last) {
-        issue(k_first, 0);
-        uint32_t buf = 0;
-        for (uint32_t kt = k_first; kt < k_last; ++kt, buf ^= 1) {
-            // this tile has landed, and every wave has read the last one
-            asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
-            if (kt + 1 < k_last) issue(kt + 1, buf ^ 1);
-            if (E == E_I8 && (p.kb & 15u) && kt + 1 == tiles_k) {
-                // the last piece ends inside: A's bytes past the sum are cleared, and
-                // what B has there is multiplied by zero
-                if (tid < BM) {
-                    const uint32_t c = (p.kb % KB) / 16u, have = p.kb & 15u;
-                    uint32_t* piece = reinterpret_cast<uint32_t*>(lds + buf * STAGE + tid * KB + ((c ^ (tid & 7u)) * 16u));
-#pragma unroll
-                    for (uint32_t e = 0; e < 4; ++e) {
-                        const uint32_t bytes = have > 4u * e ? min(have - 4u * e, 4u) : 0u;
-                        if (bytes < 4u) piece[e] &= (1u << (8u * bytes)) - 1u;
-                    }
-                }
-                __syncthreads();
-            }
-            compute(buf);
+                for (int j = 0; j < TN; ++j) asm volatile("" : "+a"(acc[i][j]));    // no sum is read before that
         }
     }
 
@@ -231,49 +253,67 @@ __global__ void __launch_bounds__(WM * WN * 64, OCC) product_kernel(const Produc
     }
 
     // D: a lane holds four consecutive columns of a row; each wave turns 16 rows at a
-    // time in its own part of LDS into whole pieces of rows.
-    const uint32_t wrow = row0 + (uint32_t)(wm * TM * 16), wcol = col0 + (uint32_t)(wn * TN * 16);
-    float factor = 1.0f;
-    if (E == E_F16 && p.alpha) factor = p.alpha[1];
+    // time in its own part of LDS, so that a lane then has eight columns, the same ones in
+    // every row.
     __syncthreads();
     float* stage = reinterpret_cast<float*>(lds) + wave * 16 * OUTP;
-#pragma unroll
-    for (int i = 0; i < TM; ++i) {
-        const float sx = E == E_I8 ? p.sx[min(wrow + (uint32_t)(i * 16 + fr), p.m - 1)] : factor;
-#pragma unroll
-        for (int j = 0; j < TN; ++j) {
-            f32x4 v;
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                v[e] = out_value(acc[i][j][e]) * sx;
-                if constexpr (E == E_I8) {
-                    const uint32_t c = min(wcol + (uint32_t)(j * 16 + fg * 4 + e), p.n - 1);
-                    v[e] = v[e] * p.sw[c] + (p.bias ? bias_at(p, c) : 0.0f);
-                }
-            }
-            *reinterpret_cast<f32x4*>(stage + fr * OUTP + j * 16 + fg * 4) = v;
-        }
-        __builtin_amdgcn_wave_barrier();
+    const uint32_t wrow = row0 + (uint32_t)(wm * TM * 16), wcol = col0 + (uint32_t)(wn * TN * 16);
+    auto finish = [&](auto type) __attribute__((always_inline)) {
+        constexpr int DT = decltype(type)::value;
+        typedef typename Type<DT>::T Out;
         constexpr int LPR = TN * 2, RPI = 64 / LPR;             // lanes to a row of eights, rows at once
+        const int lrow = lane / LPR, lcol = lane % LPR * 8;
+        const uint32_t col = wcol + (uint32_t)lcol;
+        const bool on = col < p.n;
+        float sw[8], bias[8];
 #pragma unroll
-        for (int q = 0; q < 16 / RPI; ++q) {
-            const int r = q * RPI + lane / LPR, c = lane % LPR * 8;
-            float v[8];
-#pragma unroll
-            for (int e = 0; e < 8; e += 4) {
-                const f32x4 w = *reinterpret_cast<const f32x4*>(stage + r * OUTP + c + e);
-#pragma unroll
-                for (int k = 0; k < 4; ++k) v[e + k] = w[k];
-            }
-            const uint32_t row = wrow + (uint32_t)(i * 16 + r), col = wcol + (uint32_t)c;
-            if (row < p.m && col < p.n) {
-                if (p.out == Q8_F32) put_out<Q8_F32>(p, row, col, v);
-                else if (E != E_BF16 && p.out == Q8_F16) put_out<Q8_F16>(p, row, col, v);
-                else if (E != E_F16) put_out<Q8_BF16>(p, row, col, v);
-            }
+        for (int e = 0; e < 8; ++e) { sw[e] = 1.0f; bias[e] = 0.0f; }
+        if constexpr (E == E_I8) {
+            if (on) load_part<Q8_F32>(p.sw, col, p.n, sw);
+            if (on && p.bias) load_part<DT>((const Out*)p.bias, col, p.n, bias);
         }
-        __builtin_amdgcn_wave_barrier();
-    }
+        float factor = 1.0f;
+        if (E == E_F16 && p.alpha) factor = p.alpha[1];
+#pragma unroll
+        for (int i = 0; i < TM; ++i) {
+#pragma unroll
+            for (int j = 0; j < TN; ++j)
+                *reinterpret_cast<f32x4*>(stage + fr * OUTP + j * 16 + fg * 4) =
+                    f32x4{out_value(acc[i][j][0]), out_value(acc[i][j][1]), out_value(acc[i][j][2]), out_value(acc[i][j][3])};
+            __builtin_amdgcn_wave_barrier();
+#pragma unroll
+            for (int q = 0; q < 16 / RPI; ++q) {
+                const int r = q * RPI + lrow;
+                float v[8];
+#pragma unroll
+                for (int e = 0; e < 8; e += 4) {
+                    const f32x4 w = *reinterpret_cast<const f32x4*>(stage + r * OUTP + lcol + e);
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) v[e + k] = w[k];
+                }
+                const uint32_t row = wrow + (uint32_t)(i * 16 + r);
+                if (!on || row >= p.m) continue;
+                Out* y = (Out*)p.y + (uint64_t)row * p.ldy;
+                const float sx = E == E_I8 ? p.sx[row] : factor;
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    v[e] *= sx;
+                    if constexpr (E == E_I8) v[e] = __builtin_fmaf(v[e], sw[e], bias[e]);
+                }
+                if (E != E_I8 && p.accumulate) {
+                    float old[8];
+                    load_part<DT>(y, col, p.n, old);
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) v[e] += old[e];
+                }
+                store_part<DT>(y, col, p.n, v);
+            }
+            __builtin_amdgcn_wave_barrier();
+        }
+    };
+    if (p.out == Q8_F32) finish(Int<Q8_F32>{});
+    else if (E != E_BF16 && p.out == Q8_F16) finish(Int<Q8_F16>{});
+    else if (E != E_F16) finish(Int<Q8_BF16>{});
 }
 
 // Few tokens (m <= 64).  A work-group owns 16 * NT channels and all of K, in
@@ -325,7 +365,7 @@ __global__ void __launch_bounds__(WAVES * 64) few_kernel(const Product p) {
 #pragma unroll
             for (int i = 0; i < MT; ++i)
 #pragma unroll
-                for (int j = 0; j < NT; ++j) acc[i][j] = A::mfma(wv[s][j], xv[s][i], acc[i][j]);
+                for (int j = 0; j < NT; ++j) A::mfma(wv[s][j], xv[s][i], acc[i][j]);
     }
     if (p.kb % 64 && wave == WAVES - 1) {   // the rest, byte by byte
         const uint32_t k0 = whole * 64 + fg * 16;
@@ -344,7 +384,7 @@ __global__ void __launch_bounds__(WAVES * 64) few_kernel(const Product p) {
 #pragma unroll
         for (int i = 0; i < MT; ++i)
 #pragma unroll
-            for (int j = 0; j < NT; ++j) acc[i][j] = A::mfma(wv[j], xv[i], acc[i][j]);
+            for (int j = 0; j < NT; ++j) A::mfma(wv[j], xv[i], acc[i][j]);
     }
 #pragma unroll
     for (int i = 0; i < MT; ++i)
@@ -383,8 +423,8 @@ template <int E> hipError_t product_any(const Route& r, Product p, hipStream_t s
     p.splits = r.splits;
     p.tiles_per_split = (uint32_t)ceil_div(ceil_div(p.kb, KB), r.splits);
     const dim3 grid(p.nwgx * p.nwgy, r.splits);
-    if (r.kind == 0) return launch((const void*)&product_kernel<E, 2, 4, 8, 4, 2>, grid, 512, p, s);
-    return launch((const void*)&product_kernel<E, 2, 2, 4, 4, 2>, grid, 256, p, s);
+    if (r.kind == 0) return launch((const void*)&product_kernel<E, 8, 1>, grid, 256, p, s);
+    return launch((const void*)&product_kernel<E, 4, 2>, grid, 256, p, s);
 }
 
 template <int MT> hipError_t few_any(const Product& p, hipStream_t s) {
@@ -404,7 +444,7 @@ hipError_t launch_few(const Product& p, hipStream_t s) {
 
 hipError_t prepare_products() {
     hipFuncAttributes a;
-    return hipFuncGetAttributes(&a, (const void*)&product_kernel<E_I8, 2, 2, 4, 4, 2>);
+    return hipFuncGetAttributes(&a, (const void*)&product_kernel<E_I8, 4, 2>);
 }
 
 }  // namespace q8

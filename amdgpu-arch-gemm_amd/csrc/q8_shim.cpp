@@ -160,7 +160,8 @@ uint64_t round_up(uint64_t x, uint64_t to) { return (x + to - 1) / to * to; }
 struct Grad {
     uint64_t cp;        // values of the summed index in a laid-out row
     uint32_t terms;
-    uint64_t kb;
+    uint64_t kb;        // its bytes
+    uint64_t pitch;     // and those from one row to the next
     ProductPlan plan;
     Layout at;
 };
@@ -172,10 +173,13 @@ int plan_grad(int dtype, uint64_t rows, uint64_t cols, uint64_t sum, bool copy_a
     if (g.kb > kMaxRowBytes)
         return fail(SGEMM_E_SHAPE, "a sum over %llu products is too long: at most %llu", (unsigned long long)sum,
                     (unsigned long long)(kMaxRowBytes / (2 * g.terms)));
+    // an odd number of lines: rows of a power of two apart meet in few memory channels
+    g.pitch = (g.kb / 128 | 1) * 128;
+    if (g.pitch < g.kb) g.pitch += 256;
     g.plan = plan_product(rows, cols, g.kb);
     g.at = Layout();
-    if (copy_a || dtype == Q8_F32) g.at.add(g.at.a, rows * g.kb);
-    g.at.add(g.at.b, cols * g.kb);
+    if (copy_a || dtype == Q8_F32) g.at.add(g.at.a, rows * g.pitch);
+    g.at.add(g.at.b, cols * g.pitch);
     if (dtype == Q8_F16) g.at.add(g.at.pair, 8);
     if (g.plan.partial_bytes) g.at.add(g.at.partial, g.plan.partial_bytes);
     return SGEMM_OK;
@@ -423,7 +427,9 @@ int q8_gemm(q8_handle* h, int dtype, const int8_t* qx, uint32_t ldx, const float
     for (const Span& s : in) CHECK(check(s));
     CHECK(check(out));
     for (const Span& s : in) CHECK(check_apart(out, s));
-    const GemmPlan g = plan_gemm(m, n, k, !rows_aligned(qx, ldx), !rows_aligned(qw, ldw));
+    // a sum that ends inside a piece of 16 bytes: qx's copy has zeros there, and what qw has
+    // is multiplied by them
+    const GemmPlan g = plan_gemm(m, n, k, !rows_aligned(qx, ldx) || k % 16, !rows_aligned(qw, ldw));
     if (!g.few) CHECK(check_grid(m, n, g.plan));
     OnDevice on(h->device);
     HIP_TRY(on.status());
@@ -468,19 +474,19 @@ int q8_grad_input(q8_handle* h, int dtype, const void* dy, uint32_t lddy, const 
     const Element e = dtype == Q8_F16 ? E_F16 : E_BF16;
     float* pair = dtype == Q8_F16 ? reinterpret_cast<float*>(h->workspace + g.at.pair) : nullptr;
     if (pair) HIP_TRY(launch_scale_pair(sw, n, pair, h->stream));
-    const PackWeights pw = {qw, dtype == Q8_F32 ? nullptr : sw, pair, h->workspace + g.at.b, ldw, g.cp * g.terms, n, k,
+    const PackWeights pw = {qw, dtype == Q8_F32 ? nullptr : sw, pair, h->workspace + g.at.b, ldw, g.pitch / 2, n, k,
                             (uint32_t)g.cp, g.terms};
     if (n) HIP_TRY(launch_pack_weights(e, pw, h->stream));
     if (copy && n) {
-        const PackGradient pg = {dy, dtype == Q8_F32 ? sw : nullptr, h->workspace + g.at.a, lddy, g.cp * g.terms, m, n,
+        const PackGradient pg = {dy, dtype == Q8_F32 ? sw : nullptr, h->workspace + g.at.a, lddy, g.pitch / 2, m, n,
                                  (uint32_t)g.cp, 0};
         HIP_TRY(launch_pack_gradient(dtype, pg, h->stream));
     }
     Product p = {};
     p.a = copy ? h->workspace + g.at.a : dy;
-    p.lda = copy ? g.kb : (uint64_t)lddy * size;
+    p.lda = copy ? g.pitch : (uint64_t)lddy * size;
     p.b = h->workspace + g.at.b;
-    p.ldb = g.kb;
+    p.ldb = g.pitch;
     p.m = m; p.n = k; p.kb = (uint32_t)g.kb;
     p.alpha = pair; p.y = dx; p.ldy = lddx; p.out = dtype;
     set_common(p, h, g.plan, g.at);
@@ -511,17 +517,17 @@ int q8_grad_weight(q8_handle* h, int dtype, const void* dy, uint32_t lddy, const
     float* pair = dtype == Q8_F16 ? reinterpret_cast<float*>(h->workspace + g.at.pair) : nullptr;
     if (pair) HIP_TRY(launch_scale_pair(sx, m, pair, h->stream));
     if (m) {
-        const PackWeights pw = {qx, dtype == Q8_F32 ? nullptr : sx, pair, h->workspace + g.at.b, ldx, g.cp * g.terms, m, k,
+        const PackWeights pw = {qx, dtype == Q8_F32 ? nullptr : sx, pair, h->workspace + g.at.b, ldx, g.pitch / 2, m, k,
                                 (uint32_t)g.cp, g.terms};
         HIP_TRY(launch_pack_weights(e, pw, h->stream));
-        const PackGradient pg = {dy, dtype == Q8_F32 ? sx : nullptr, h->workspace + g.at.a, lddy, g.cp * g.terms, n, m,
+        const PackGradient pg = {dy, dtype == Q8_F32 ? sx : nullptr, h->workspace + g.at.a, lddy, g.pitch / 2, n, m,
                                  (uint32_t)g.cp, 1};
         HIP_TRY(launch_pack_gradient(dtype, pg, h->stream));
     }
     Product p = {};
     p.a = h->workspace + g.at.a;
     p.b = h->workspace + g.at.b;
-    p.lda = p.ldb = g.kb;
+    p.lda = p.ldb = g.pitch;
     p.m = n; p.n = k; p.kb = (uint32_t)g.kb;
     p.alpha = pair; p.y = dw; p.ldy = lddw; p.out = out_dtype; p.accumulate = accumulate != 0;
     set_common(p, h, g.plan, g.at);
