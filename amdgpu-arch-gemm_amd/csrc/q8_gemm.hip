@@ -56,9 +56,11 @@ __device__ __forceinline__ uint32_t xcd_order(uint32_t id, uint32_t total) {
     const uint32_t x = id % XCDS, q = total / XCDS, r = total % XCDS;
     return x * q + (x < r ? x : r) + id / XCDS;
 }
-// Tiles in groups of eight rows of them, column by column within a group.
+// Tiles in groups of six rows of them, column by column within a group: the 32 tiles of
+// 256 x 256 that an XCD works on at a time are then 6 x 5.3 and read the fewest
+// lines (8192^3 in 8-bit integers: six 388 us, four 436, eight 443, sixteen 452).
 __device__ __forceinline__ void tile_of(uint32_t z, uint32_t nx, uint32_t ny, uint32_t& tx, uint32_t& ty) {
-    constexpr uint32_t GROUP = 8;
+    constexpr uint32_t GROUP = 6;
     const uint32_t group = z / (GROUP * ny), first = group * GROUP;
     const uint32_t width = min(nx - first, GROUP), in = z - group * GROUP * ny;
     tx = first + in % width;
@@ -83,6 +85,12 @@ __device__ __forceinline__ void load_lds(__amdgpu_buffer_rsrc_t rsrc, uint32_t l
     uint32_t from;
     asm volatile("s_add_u32 m0, %2, %6\n\ts_mov_b32 %0, %1\n\ts_add_u32 %1, %1, %5\n\tbuffer_load_dwordx4 %3, %4, %0 offen lds"
                  : "=&s"(from), "+s"(soff) : "s"(lds), "v"(voff), "s"(rsrc), "s"(step), "i"(at) : "scc");
+}
+
+// One dword a lane, 256 bytes of LDS.
+__device__ __forceinline__ void touch(__amdgpu_buffer_rsrc_t rsrc, uint32_t lds, uint32_t voff, uint32_t soff) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dword %1, %2, %3 offen lds"
+                 :: "s"(lds), "v"(voff), "s"(rsrc), "s"(soff));
 }
 
 template <bool V> struct Flag { static constexpr bool value = V; };
@@ -115,7 +123,9 @@ __global__ void __launch_bounds__(256, OCC) product_kernel(const Product p) {
     constexpr int STAGE = (BM + BN) * KB;
     constexpr int OUTP = TN * 16 + 4;                           // floats of a staged row of D
     constexpr int OUT = WAVES * 16 * OUTP * 4;
-    constexpr int LDS = 2 * STAGE > OUT ? 2 * STAGE : OUT;
+    constexpr int AHEAD = 3;                                    // tiles that L2 is ahead
+    constexpr int LDS = 2 * STAGE + WAVES * 256;
+    static_assert(OUT <= LDS, "D's rows are staged where the tiles were");
     __shared__ __attribute__((aligned(128))) unsigned char lds[LDS];
 
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -151,6 +161,20 @@ __global__ void __launch_bounds__(256, OCC) product_kernel(const Product p) {
         const int r = i / 2 * (WAVES * 1024);
         if (i & 1) load_lds(rb, at, BM * KB + r, ub, sb, stepb);
         else load_lds(ra, at, r, ua, sa, stepa);
+    };
+
+    // A tile's loads have the time of one tile, which L2 keeps and memory does not: a dword of
+    // each of its lines is asked for one tile before, into LDS that nobody reads.  The
+    // work-groups beside this one on the XCD share its rows of A or of B, so each
+    // asks for a quarter of them.  (Gradients of 16384 x 4096 x 4096: 365 + 368 -> 316 + 293
+    // us; each asking for all of its lines: 342 + 333.)
+    const uint32_t share = BM / 4;
+    const uint32_t pr = (wave < 2 ? ty % 4 : tx % 4) * share + (uint32_t)(wave & 1) * (share / 2) + (uint32_t)lane;
+    const uint32_t pp = (uint32_t)lane < share / 2 ? pr * (wave < 2 ? lda : ldb) : NOWHERE;
+    auto ask = [&](uint32_t kt) __attribute__((always_inline)) {
+        const uint32_t v = kt < k_last ? pp : NOWHERE;
+        if (wave < 2) touch(ra, lds0 + 2 * STAGE + (uint32_t)wave * 256u, v, kt * KB);
+        else touch(rb, lds0 + 2 * STAGE + (uint32_t)wave * 256u, v, kt * KB);
     };
 
     Acc acc[TM][TN];
@@ -194,16 +218,19 @@ __global__ void __launch_bounds__(256, OCC) product_kernel(const Product p) {
         aim(k_first + 1, 1);
 #pragma unroll
         for (int i = 0; i < 2 * LOADS; ++i) load(i);
-        asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" :: "i"(2 * LOADS) : "memory");
+#pragma unroll
+        for (int i = 2; i < AHEAD; ++i) ask(k_first + i);
+        asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" :: "i"(2 * LOADS + AHEAD - 2) : "memory");
 #pragma unroll
         for (int i = 0; i < TM + TN; ++i) read(f0, 0, 0, i);
         uint32_t buf = 0;
         for (uint32_t kt = k_first; kt < k_last; ++kt, buf ^= 1) {
             multiply(f0, f1, buf, 1, Flag<false>{});
             // every wave has read this tile, and the next one has landed
-            asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+            asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" :: "i"(1) : "memory");
             aim(kt + 2, buf);
             multiply(f1, f0, buf ^ 1, 0, Flag<true>{});
+            ask(kt + AHEAD);
         }
         // zeros for tiles past the range; and the last products, whose results the
         // compiler does not know to wait for
