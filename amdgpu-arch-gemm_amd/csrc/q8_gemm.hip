@@ -16,7 +16,6 @@ typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 
 constexpr int BUFFER_RSRC_WORD3 = 0x00020000;
-constexpr int CPOL_SC1 = 0x10;
 constexpr int XCDS = 8;
 constexpr uint32_t NOWHERE = 0x80000000u;    // an offset past every descriptor's end: loads give 0
 constexpr int KB = kTileBytes;
@@ -93,6 +92,9 @@ __device__ __forceinline__ void touch(__amdgpu_buffer_rsrc_t rsrc, uint32_t lds,
                  :: "s"(lds), "v"(voff), "s"(rsrc), "s"(soff));
 }
 
+// Waits for the wave's reads of LDS, which the compiler then knows (lgkmcnt 0).
+__device__ __forceinline__ void wait_lds() { __builtin_amdgcn_s_waitcnt(0xc07f); }
+
 template <bool V> struct Flag { static constexpr bool value = V; };
 template <int V> struct Int { static constexpr int value = V; };
 
@@ -113,26 +115,21 @@ __device__ __forceinline__ float bias_at(const Product& p, uint32_t col) {
 // operands are read from LDS between the matrix instructions; a tile's buffer is
 // free once its second step has been read, in the middle of the tile, and takes the
 // tile after next then.  So there is one barrier a tile, and a load has the time of a whole
-// tile to land.
-template <int E, int T, int OCC>
+// tile to land.  AHEAD: see `ask`.  DT: D's type.
+template <int E, int DT, int T, int OCC, bool AHEAD>
 __global__ void __launch_bounds__(256, OCC) product_kernel(const Product p) {
     typedef Atom<E> A;
     typedef typename A::Acc Acc;
     constexpr int TM = T, TN = T, WAVES = 4, BM = 2 * T * 16, BN = BM;
     constexpr int LOADS = BM / 8 / WAVES;                       // of 8 rows a wave, K tile and operand
     constexpr int STAGE = (BM + BN) * KB;
-    constexpr int OUTP = TN * 16 + 4;                           // floats of a staged row of D
-    constexpr int OUT = WAVES * 16 * OUTP * 4;
-    constexpr int AHEAD = 3;                                    // tiles that L2 is ahead
-    constexpr int LDS = 2 * STAGE + WAVES * 256;
-    static_assert(OUT <= LDS, "D's rows are staged where the tiles were");
+    constexpr int LDS = 2 * STAGE + (AHEAD ? WAVES * 256 : 0);
     __shared__ __attribute__((aligned(128))) unsigned char lds[LDS];
 
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int wm = wave & 1, wn = wave >> 1;
     uint32_t tx, ty;
-    const uint32_t total = p.nwgx * p.nwgy;
-    tile_of(xcd_order(blockIdx.x, total), p.nwgx, p.nwgy, tx, ty);
+    tile_of(xcd_order(blockIdx.x, p.nwgx * p.nwgy), p.nwgx, p.nwgy, tx, ty);
     const uint32_t row0 = tx * BM, col0 = ty * BN;
     const uint32_t tiles_k = (p.kb + KB - 1) / KB;
     const uint32_t k_first = blockIdx.y * p.tiles_per_split;
@@ -141,20 +138,21 @@ __global__ void __launch_bounds__(256, OCC) product_kernel(const Product p) {
     const __amdgpu_buffer_rsrc_t ra = rows_rsrc(p.a, p.lda, row0, p.m, p.kb), rb = rows_rsrc(p.b, p.ldb, col0, p.n, p.kb);
     const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) unsigned char*)lds;
 
-    // Row r of a tile keeps its piece c of 16 bytes at piece c ^ (r & 7): the
-    // eight lanes that read one piece of eight rows at a time meet all banks.  A load's
-    // lanes fill LDS in order, so it is the address in memory that is permuted.
-    const uint32_t lr = (uint32_t)lane >> 3, lc = ((uint32_t)lane & 7u) ^ lr;
+    // Row r of a tile keeps its piece c of 16 bytes at piece c ^ key(r), so that the lanes that
+    // read LDS together meet all banks: rows fr of A, and those of B that `read` says.
+    // A load's lanes fill LDS in order, so it is the address in memory that is permuted.
+    const uint32_t lr = (uint32_t)lane >> 3;
+    const uint32_t ca = ((uint32_t)lane & 7u) ^ lr, cb = ((uint32_t)lane & 7u) ^ ((lr & 3u) | ((uint32_t)wave & 1u) << 2);
     const uint32_t lda = (uint32_t)p.lda, ldb = (uint32_t)p.ldb;
-    const uint32_t va = (uint32_t)(wave * 8 + lr) * lda + lc * 16u, vb = (uint32_t)(wave * 8 + lr) * ldb + lc * 16u;
+    const uint32_t va = (uint32_t)(wave * 8 + lr) * lda + ca * 16u, vb = (uint32_t)(wave * 8 + lr) * ldb + cb * 16u;
     const uint32_t stepa = WAVES * 8u * lda, stepb = WAVES * 8u * ldb;
+    // past which byte of a row nothing is read: pieces from there on are zeros
+    const uint32_t k_end = min(k_last * KB, p.kb);
     uint32_t ua = 0, ub = 0, sa = 0, sb = 0, at = 0;    // of the tile that is being loaded
     auto aim = [&](uint32_t kt, uint32_t buf) __attribute__((always_inline)) {
-        // pieces past the rows' end, and tiles past the range, are zeros
         sa = sb = kt * KB;
-        const bool have = kt < k_last && sa + lc * 16u < p.kb;
-        ua = have ? va : NOWHERE;
-        ub = have ? vb : NOWHERE;
+        ua = sa + ca * 16u < k_end ? va : NOWHERE;
+        ub = sa + cb * 16u < k_end ? vb : NOWHERE;
         at = lds0 + buf * STAGE + (uint32_t)wave * 1024u;
     };
     auto load = [&](int i) __attribute__((always_inline)) {     // 0 .. 2 * LOADS - 1, A and B in turn
@@ -166,11 +164,10 @@ __global__ void __launch_bounds__(256, OCC) product_kernel(const Product p) {
     // A tile's loads have the time of one tile, which L2 keeps and memory does not: a dword of
     // each of its lines is asked for one tile before, into LDS that nobody reads.  The
     // work-groups beside this one on the XCD share its rows of A or of B, so each
-    // asks for a quarter of them.  (Gradients of 16384 x 4096 x 4096: 365 + 368 -> 316 + 293
-    // us; each asking for all of its lines: 342 + 333.)
-    const uint32_t share = BM / 4;
-    const uint32_t pr = (wave < 2 ? ty % 4 : tx % 4) * share + (uint32_t)(wave & 1) * (share / 2) + (uint32_t)lane;
-    const uint32_t pp = (uint32_t)lane < share / 2 ? pr * (wave < 2 ? lda : ldb) : NOWHERE;
+    // asks for a quarter of them.
+    constexpr uint32_t SHARE = BM / 4;
+    const uint32_t pr = (wave < 2 ? ty % 4 : tx % 4) * SHARE + (uint32_t)(wave & 1) * (SHARE / 2) + (uint32_t)lane;
+    const uint32_t pp = (uint32_t)lane < SHARE / 2 ? pr * (wave < 2 ? lda : ldb) : NOWHERE;
     auto ask = [&](uint32_t kt) __attribute__((always_inline)) {
         const uint32_t v = kt < k_last ? pp : NOWHERE;
         if (wave < 2) touch(ra, lds0 + 2 * STAGE + (uint32_t)wave * 256u, v, kt * KB);
@@ -183,16 +180,20 @@ __global__ void __launch_bounds__(256, OCC) product_kernel(const Product p) {
 #pragma unroll
         for (int j = 0; j < TN; ++j) acc[i][j] = Acc{0, 0, 0, 0};
 
-    const int fr = lane & 15, fg = lane >> 4;
-    const uint32_t fc = ((uint32_t)fg ^ ((uint32_t)fr & 7u)) * 16u;
-    const uint32_t fa = (uint32_t)(wm * TM * 16 + fr) * KB + fc, fb = (uint32_t)(BM + wn * TN * 16 + fr) * KB + fc;
+    // The wave's operands: a lane has row fr of a tile of A, and of a tile of B the row with
+    // which its results are columns next to one another: in a pair of tiles, row fr of tile j
+    // is row fr / 4 * 8 + j * 4 + fr % 4, and a lane's eight results are columns fg * 8 .. + 7.
+    const uint32_t fr = (uint32_t)lane & 15u, fg = (uint32_t)lane >> 4;
+    const uint32_t fa = (uint32_t)(wm * TM * 16) * KB + fr * KB + (fg ^ (fr & 7u)) * 16u;
+    const uint32_t fb = (uint32_t)(BM + wn * TN * 16) * KB + ((fr >> 2) * 8u + (fr & 3u)) * KB +
+                        (fg ^ ((fr & 3u) | ((fr >> 2) & 1u) << 2)) * 16u;
     struct Step {
         u32x4 a[TM], b[TN];
     };
     Step f0, f1;
     auto read = [&](Step& f, uint32_t buf, uint32_t s, int i) __attribute__((always_inline)) {   // 0 .. TM + TN - 1
         const unsigned char* from = lds + buf * STAGE;
-        if (i < TN) f.b[i] = *reinterpret_cast<const u32x4*>(from + (fb ^ (s * 64)) + i * 16 * KB);
+        if (i < TN) f.b[i] = *reinterpret_cast<const u32x4*>(from + (fb ^ (s * 64)) + (i / 2 * 32 + i % 2 * 4) * KB);
         else f.a[i - TN] = *reinterpret_cast<const u32x4*>(from + (fa ^ (s * 64)) + (i - TN) * 16 * KB);
     };
     // One step's products, the next step's operands and, in the second step, a tile's loads
@@ -218,114 +219,99 @@ __global__ void __launch_bounds__(256, OCC) product_kernel(const Product p) {
         aim(k_first + 1, 1);
 #pragma unroll
         for (int i = 0; i < 2 * LOADS; ++i) load(i);
-#pragma unroll
-        for (int i = 2; i < AHEAD; ++i) ask(k_first + i);
-        asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" :: "i"(2 * LOADS + AHEAD - 2) : "memory");
+        if constexpr (AHEAD) ask(k_first + 2);
+        asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" :: "i"(2 * LOADS + (AHEAD ? 1 : 0)) : "memory");
 #pragma unroll
         for (int i = 0; i < TM + TN; ++i) read(f0, 0, 0, i);
+        wait_lds();
         uint32_t buf = 0;
         for (uint32_t kt = k_first; kt < k_last; ++kt, buf ^= 1) {
             multiply(f0, f1, buf, 1, Flag<false>{});
             // every wave has read this tile, and the next one has landed
-            asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" :: "i"(1) : "memory");
+            wait_lds();
+            asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" :: "i"(AHEAD ? 1 : 0) : "memory");
             aim(kt + 2, buf);
             multiply(f1, f0, buf ^ 1, 0, Flag<true>{});
-            ask(kt + AHEAD);
+            if constexpr (AHEAD) ask(kt + 3);
+            wait_lds();
         }
         // zeros for tiles past the range; and the last products, whose results the
         // compiler does not know to wait for
         asm volatile("s_waitcnt vmcnt(0)\n\ts_nop 15\n\ts_nop 15" ::: "memory");
-        if constexpr (T == 8) {
-#pragma unroll
-            for (int i = 0; i < TM; ++i)
-#pragma unroll
-                for (int j = 0; j < TN; ++j) asm volatile("" : "+a"(acc[i][j]));    // no sum is read before that
-        }
     }
+    // A sum, read no earlier than here: not before the wait above, and not all of them at once.
+    auto sum = [&](int i, int j) __attribute__((always_inline)) {
+        if constexpr (T == 8) asm volatile("" : "+a"(acc[i][j]));
+        return acc[i][j];
+    };
 
-    // The K ranges meet: partial sums go past the XCD's L2, the last work-group of a tile
-    // to arrive adds them in range order.
+    const uint32_t wrow = row0 + (uint32_t)(wm * TM * 16), wcol = col0 + (uint32_t)(wn * TN * 16);
     if (p.splits > 1) {
-        constexpr uint32_t PART = BM * BN * 4;
-        const uint32_t tile = tx + ty * p.nwgx;
-        char* ws = (char*)p.partial + (uint64_t)tile * p.splits * PART;
-        auto part = [&](uint32_t s) __attribute__((always_inline)) {
-            return __builtin_amdgcn_make_buffer_rsrc(ws + (uint64_t)s * PART, (short)0, (int)PART, BUFFER_RSRC_WORD3);
-        };
-        const __amdgpu_buffer_rsrc_t mine = part(blockIdx.y);
+        // a K range's sums, whole tiles: finish_kernel adds the ranges
+        char* first = (char*)p.partial + (((uint64_t)blockIdx.y * p.rows + wrow + fr) * p.pitch + wcol + fg * 8u) * 4u;
 #pragma unroll
         for (int i = 0; i < TM; ++i)
 #pragma unroll
             for (int j = 0; j < TN; ++j)
-                __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, acc[i][j]), mine,
-                                                       ((i * TN + j) * WAVES * 64 + tid) * 16, 0, CPOL_SC1);
-        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-        __shared__ uint32_t arrived;
-        __syncthreads();
-        if (tid == 0) arrived = __hip_atomic_fetch_add(p.tickets + tile, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        __syncthreads();
-        if (arrived + 1 != p.splits) return;
-        for (uint32_t s = 0; s < p.splits; ++s) {
-            const __amdgpu_buffer_rsrc_t r = part(s);
-#pragma unroll
-            for (int i = 0; i < TM; ++i)
-#pragma unroll
-                for (int j = 0; j < TN; ++j) {
-                    const Acc v = __builtin_bit_cast(
-                        Acc, __builtin_amdgcn_raw_buffer_load_b128(r, ((i * TN + j) * WAVES * 64 + tid) * 16, 0, CPOL_SC1));
-                    acc[i][j] = s ? acc[i][j] + v : v;
-                }
-        }
-        if (tid == 0) __hip_atomic_store(p.tickets + tile, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+                *reinterpret_cast<Acc*>(first + (uint64_t)i * 64u * p.pitch + (j / 2 * 32 + j % 2 * 4) * 4) = sum(i, j);
+        return;
     }
-
-    // D: a lane holds four consecutive columns of a row; each wave turns 16 rows at a
-    // time in its own part of LDS, so that a lane then has eight columns, the same ones in
-    // every row.
-    __syncthreads();
-    float* stage = reinterpret_cast<float*>(lds) + wave * 16 * OUTP;
-    const uint32_t wrow = row0 + (uint32_t)(wm * TM * 16), wcol = col0 + (uint32_t)(wn * TN * 16);
-    auto finish = [&](auto type) __attribute__((always_inline)) {
-        constexpr int DT = decltype(type)::value;
-        typedef typename Type<DT>::T Out;
-        constexpr int LPR = TN * 2, RPI = 64 / LPR;             // lanes to a row of eights, rows at once
-        const int lrow = lane / LPR, lcol = lane % LPR * 8;
-        const uint32_t col = wcol + (uint32_t)lcol;
-        const bool on = col < p.n;
-        float sw[8], bias[8];
+    // D: a lane has eight columns of a row in a pair of tiles, four lanes 32.  Each wave turns 16
+    // rows of 64 columns at a time in its own part of LDS, where the tiles were, and stores
+    // whole rows, eight lanes each.  All scales are loaded before the first of them.
+    constexpr int PITCH = 64 + 4;
+    static_assert(WAVES * 16 * PITCH * 4 <= LDS, "D's rows are staged where the tiles were");
+    typedef typename Type<DT>::T Out;
+    const uint32_t lrow = (uint32_t)lane / 8u, lcol = (uint32_t)lane % 8u * 8u;
+    float sx[TM][2], sw[TN / 4][8], bias[TN / 4][8];
+    if constexpr (E == E_I8) {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) { sw[e] = 1.0f; bias[e] = 0.0f; }
-        if constexpr (E == E_I8) {
-            if (on) load_part<Q8_F32>(p.sw, col, p.n, sw);
-            if (on && p.bias) load_part<DT>((const Out*)p.bias, col, p.n, bias);
+        for (int h = 0; h < TN / 4; ++h) {
+            const uint32_t col = wcol + h * 64u + lcol;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) bias[h][e] = 0.0f;
+            if (col < p.n) {
+                load_part<Q8_F32>(p.sw, col, p.n, sw[h]);
+                if (p.bias) load_part<DT>((const Out*)p.bias, col, p.n, bias[h]);
+            }
         }
-        float factor = 1.0f;
-        if (E == E_F16 && p.alpha) factor = p.alpha[1];
+#pragma unroll
+        for (int i = 0; i < TM; ++i)
+#pragma unroll
+            for (int q = 0; q < 2; ++q) sx[i][q] = p.sx[min(wrow + i * 16u + q * 8u + lrow, p.m - 1)];
+    }
+    const float factor = E == E_F16 && p.alpha ? p.alpha[1] : 1.0f;
+    __syncthreads();
+    float* const stage = reinterpret_cast<float*>(lds) + wave * 16 * PITCH;
+#pragma unroll
+    for (int h = 0; h < TN / 4; ++h) {
+        const uint32_t col = wcol + h * 64u + lcol;
+        const bool on = col < p.n;
 #pragma unroll
         for (int i = 0; i < TM; ++i) {
 #pragma unroll
-            for (int j = 0; j < TN; ++j)
-                *reinterpret_cast<f32x4*>(stage + fr * OUTP + j * 16 + fg * 4) =
-                    f32x4{out_value(acc[i][j][0]), out_value(acc[i][j][1]), out_value(acc[i][j][2]), out_value(acc[i][j][3])};
+            for (int j = 0; j < 4; ++j) {
+                const Acc x = sum(i, 4 * h + j);
+                *reinterpret_cast<f32x4*>(stage + fr * PITCH + j / 2 * 32 + fg * 8u + j % 2 * 4) =
+                    f32x4{out_value(x[0]), out_value(x[1]), out_value(x[2]), out_value(x[3])};
+            }
             __builtin_amdgcn_wave_barrier();
 #pragma unroll
-            for (int q = 0; q < 16 / RPI; ++q) {
-                const int r = q * RPI + lrow;
+            for (int q = 0; q < 2; ++q) {
+                const uint32_t r = q * 8u + lrow, row = wrow + i * 16u + r;
                 float v[8];
 #pragma unroll
                 for (int e = 0; e < 8; e += 4) {
-                    const f32x4 w = *reinterpret_cast<const f32x4*>(stage + r * OUTP + lcol + e);
+                    const f32x4 w = *reinterpret_cast<const f32x4*>(stage + r * PITCH + lcol + e);
 #pragma unroll
                     for (int k = 0; k < 4; ++k) v[e + k] = w[k];
                 }
-                const uint32_t row = wrow + (uint32_t)(i * 16 + r);
                 if (!on || row >= p.m) continue;
                 Out* y = (Out*)p.y + (uint64_t)row * p.ldy;
-                const float sx = E == E_I8 ? p.sx[row] : factor;
 #pragma unroll
                 for (int e = 0; e < 8; ++e) {
-                    v[e] *= sx;
-                    if constexpr (E == E_I8) v[e] = __builtin_fmaf(v[e], sw[e], bias[e]);
+                    v[e] *= E == E_I8 ? sx[i][q] : factor;
+                    if constexpr (E == E_I8) v[e] = __builtin_fmaf(v[e], sw[h][e], bias[h][e]);
                 }
                 if (E != E_I8 && p.accumulate) {
                     float old[8];
@@ -337,10 +323,44 @@ __global__ void __launch_bounds__(256, OCC) product_kernel(const Product p) {
             }
             __builtin_amdgcn_wave_barrier();
         }
-    };
-    if (p.out == Q8_F32) finish(Int<Q8_F32>{});
-    else if (E != E_BF16 && p.out == Q8_F16) finish(Int<Q8_F16>{});
-    else if (E != E_F16) finish(Int<Q8_BF16>{});
+    }
+}
+
+// The K ranges' sums of a product, added in range order and finished as the product kernel finishes
+// its own: a work-group has 8 rows of 256 columns, a thread eight columns.
+template <int E, int DT> __global__ void __launch_bounds__(256) finish_kernel(const Product p) {
+    typedef typename Atom<E>::Acc Acc;
+    typedef typename Type<DT>::T Out;
+    const uint32_t blocks = (p.n + 255) / 256;
+    const uint32_t row = blockIdx.x / blocks * 8 + threadIdx.x / 32, col = blockIdx.x % blocks * 256 + threadIdx.x % 32 * 8;
+    if (row >= p.m || col >= p.n) return;
+    const uint64_t range = (uint64_t)p.rows * p.pitch;
+    const Acc* from = reinterpret_cast<const Acc*>((const char*)p.partial + ((uint64_t)row * p.pitch + col) * 4);
+    Acc lo = from[0], hi = from[1];
+#pragma unroll 4
+    for (uint32_t s = 1; s < p.splits; ++s) {
+        from += range / 4;
+        lo += from[0];
+        hi += from[1];
+    }
+    float v[8];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) { v[e] = out_value(lo[e]); v[4 + e] = out_value(hi[e]); }
+    const float sx = E == E_I8 ? p.sx[row] : E == E_F16 && p.alpha ? p.alpha[1] : 1.0f;
+    Out* y = (Out*)p.y + (uint64_t)row * p.ldy;
+    float add[8] = {}, sw[8];
+    if constexpr (E == E_I8) {
+        load_part<Q8_F32>(p.sw, col, p.n, sw);
+        if (p.bias) load_part<DT>((const Out*)p.bias, col, p.n, add);
+    } else if (p.accumulate) {
+        load_part<DT>(y, col, p.n, add);
+    }
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        v[e] *= sx;
+        v[e] = E == E_I8 ? __builtin_fmaf(v[e], sw[e], add[e]) : v[e] + add[e];
+    }
+    store_part<DT>(y, col, p.n, v);
 }
 
 // Few tokens (m <= 64).  A work-group owns 16 * NT channels and all of K, in
@@ -443,15 +463,24 @@ hipError_t launch(const void* f, dim3 grid, uint32_t threads, const Product& p, 
     return hipLaunchKernel(f, grid, dim3(threads), args, 0, stream);
 }
 
-template <int E> hipError_t product_any(const Route& r, Product p, hipStream_t s) {
+template <int E, int DT> hipError_t product_any(const Route& r, Product p, hipStream_t s) {
     const Tile& t = kTiles[r.kind];
     p.nwgx = (uint32_t)ceil_div(p.m, t.m);
     p.nwgy = (uint32_t)ceil_div(p.n, t.n);
-    p.splits = r.splits;
-    p.tiles_per_split = (uint32_t)ceil_div(ceil_div(p.kb, KB), r.splits);
-    const dim3 grid(p.nwgx * p.nwgy, r.splits);
-    if (r.kind == 0) return launch((const void*)&product_kernel<E, 8, 1>, grid, 256, p, s);
-    return launch((const void*)&product_kernel<E, 4, 2>, grid, 256, p, s);
+    p.rows = p.nwgx * t.m;
+    p.pitch = p.nwgy * t.n;
+    const uint32_t tiles_k = (uint32_t)ceil_div(p.kb, KB);
+    p.tiles_per_split = (uint32_t)ceil_div(tiles_k, r.splits);
+    p.splits = tiles_k ? (uint32_t)ceil_div(tiles_k, p.tiles_per_split) : 1;    // none is empty
+    // A second round of work-groups finds its lines in memory, and in a deep K they drift apart;
+    // one round of few K tiles is 2% faster unasked.
+    const bool ahead = (uint64_t)p.nwgx * p.nwgy * p.splits > kComputeUnits || p.tiles_per_split > 32;
+    const void* f = r.kind ? (const void*)&product_kernel<E, DT, 4, 2, false>
+                           : ahead ? (const void*)&product_kernel<E, DT, 8, 1, true>
+                                   : (const void*)&product_kernel<E, DT, 8, 1, false>;
+    const hipError_t e = launch(f, dim3(p.nwgx * p.nwgy, p.splits), 256, p, s);
+    if (e != hipSuccess || p.splits == 1) return e;
+    return launch((const void*)&finish_kernel<E, DT>, dim3((uint32_t)(ceil_div(p.m, 8) * ceil_div(p.n, 256))), 256, p, s);
 }
 
 template <int MT> hipError_t few_any(const Product& p, hipStream_t s) {
@@ -462,7 +491,12 @@ template <int MT> hipError_t few_any(const Product& p, hipStream_t s) {
 }  // namespace
 
 hipError_t launch_product(Element e, const Route& r, const Product& p, hipStream_t s) {
-    return e == E_I8 ? product_any<E_I8>(r, p, s) : e == E_F16 ? product_any<E_F16>(r, p, s) : product_any<E_BF16>(r, p, s);
+    if (e == E_F16)
+        return p.out == Q8_F32 ? product_any<E_F16, Q8_F32>(r, p, s) : product_any<E_F16, Q8_F16>(r, p, s);
+    if (e == E_BF16)
+        return p.out == Q8_F32 ? product_any<E_BF16, Q8_F32>(r, p, s) : product_any<E_BF16, Q8_BF16>(r, p, s);
+    return p.out == Q8_F32 ? product_any<E_I8, Q8_F32>(r, p, s)
+                           : p.out == Q8_F16 ? product_any<E_I8, Q8_F16>(r, p, s) : product_any<E_I8, Q8_BF16>(r, p, s);
 }
 
 hipError_t launch_few(const Product& p, hipStream_t s) {
@@ -471,7 +505,7 @@ hipError_t launch_few(const Product& p, hipStream_t s) {
 
 hipError_t prepare_products() {
     hipFuncAttributes a;
-    return hipFuncGetAttributes(&a, (const void*)&product_kernel<E_I8, 4, 2>);
+    return hipFuncGetAttributes(&a, (const void*)&product_kernel<E_I8, Q8_BF16, 4, 2, false>);
 }
 
 }  // namespace q8

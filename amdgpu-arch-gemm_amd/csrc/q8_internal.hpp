@@ -74,9 +74,10 @@ struct Product {
     int out;
     int accumulate;
     // set by the launcher
-    uint32_t nwgx, nwgy, splits, tiles_per_split, vec;
+    uint32_t nwgx, nwgy, splits, tiles_per_split;
+    uint32_t rows, pitch; // of a K range's sums: whole tiles
+    // by the caller: splits sums of whole tiles, where the route has more than one
     void* partial;
-    uint32_t* tickets;
 };
 
 // How a product runs: `kind` of q8_plan.hpp, and the K ranges.

@@ -25,7 +25,6 @@ struct ProductPlan {
     int kind = 0;
     uint32_t splits = 1;
     size_t partial_bytes = 0;
-    size_t tickets = 0;
 };
 
 constexpr uint64_t div_up(uint64_t a, uint64_t b) { return (a + b - 1) / b; }
@@ -60,7 +59,6 @@ inline ProductPlan plan_product(uint64_t m, uint64_t n, uint64_t kb) {
     best.splits = (uint32_t)div_up(tiles_k, div_up(tiles_k, best.splits));
     if (best.splits > 1) {
         best.partial_bytes = (size_t)(tiles * best.splits * t.m * t.n * 4);
-        best.tickets = (size_t)tiles;
     }
     return best;
 }

@@ -18,7 +18,6 @@ struct q8_handle {
     hipStream_t own_stream = nullptr;
     char* workspace = nullptr;
     size_t workspace_bytes = 0;
-    uint32_t* tickets = nullptr;   // kMaxTickets, zero between calls
     Retired* retired = nullptr;    // workspaces that captured calls may still use
     bool captured = false;         // a call that used the workspace was captured
 };
@@ -26,9 +25,6 @@ struct q8_handle {
 namespace {
 
 using namespace q8;
-
-// K ranges are only made where the tiles leave work-groups idle.
-constexpr size_t kMaxTickets = 2 * kComputeUnits;
 
 int fail(int code, const char* fmt, ...) __attribute__((format(printf, 2, 3)));
 int fail(int code, const char* fmt, ...) {
@@ -223,7 +219,6 @@ int check_type(int dtype) { return is_type(dtype) ? SGEMM_OK : fail(SGEMM_E_INVA
 
 void set_common(Product& p, q8_handle* h, const ProductPlan& plan, const Layout& at) {
     p.partial = plan.partial_bytes ? h->workspace + at.partial : nullptr;
-    p.tickets = h->tickets;
 }
 
 }  // namespace
@@ -237,20 +232,14 @@ int q8_open(q8_handle** out) {
     if (hipGetDeviceCount(&count) != hipSuccess || count < 1) return fail(SGEMM_E_NO_DEVICE, "no HIP device is visible");
     q8_handle* h = new (std::nothrow) q8_handle;
     if (!h) return fail(SGEMM_E_INVALID, "out of host memory");
-    void* tickets = nullptr;
     hipError_t e = hipGetDevice(&h->device);
     if (e == hipSuccess) e = hipStreamCreate(&h->own_stream);
-    if (e == hipSuccess) e = hipMalloc(&tickets, kMaxTickets * sizeof(uint32_t));
-    if (e == hipSuccess) e = hipMemset(tickets, 0, kMaxTickets * sizeof(uint32_t));
-    if (e == hipSuccess) e = hipDeviceSynchronize();
     if (e == hipSuccess) e = prepare_products();
     if (e != hipSuccess) {
-        if (tickets) (void)hipFree(tickets);
         if (h->own_stream) (void)hipStreamDestroy(h->own_stream);
         delete h;
         return hip_fail(e, "q8_open");
     }
-    h->tickets = static_cast<uint32_t*>(tickets);
     h->stream = h->own_stream;
     *out = h;
     return SGEMM_OK;
@@ -267,7 +256,6 @@ void q8_close(q8_handle* h) {
         (void)hipFree(r->memory);
         delete r;
     }
-    if (h->tickets) (void)hipFree(h->tickets);
     if (h->own_stream) (void)hipStreamDestroy(h->own_stream);
     delete h;
 }
