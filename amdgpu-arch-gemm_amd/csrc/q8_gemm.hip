@@ -115,15 +115,16 @@ __device__ __forceinline__ float bias_at(const Product& p, uint32_t col) {
 // operands are read from LDS between the matrix instructions; a tile's buffer is
 // free once its second step has been read, in the middle of the tile, and takes the
 // tile after next then.  So there is one barrier a tile, and a load has the time of a whole
-// tile to land.  AHEAD: see `ask`.  DT: D's type.
-template <int E, int DT, int T, int OCC, bool AHEAD>
-__global__ void __launch_bounds__(256, OCC) product_kernel(const Product p) {
+// tile to land.  AHEAD: see `ask`.  DT: D's type.  NBUF: buffers; with more than two the loads
+// are as many tiles further ahead.
+template <int E, int DT, int T, int NBUF, bool AHEAD>
+__global__ void __launch_bounds__(256, T == 4 ? 2 : 1) product_kernel(const Product p) {
     typedef Atom<E> A;
     typedef typename A::Acc Acc;
     constexpr int TM = T, TN = T, WAVES = 4, BM = 2 * T * 16, BN = BM;
     constexpr int LOADS = BM / 8 / WAVES;                       // of 8 rows a wave, K tile and operand
     constexpr int STAGE = (BM + BN) * KB;
-    constexpr int LDS = 2 * STAGE + (AHEAD ? WAVES * 256 : 0);
+    constexpr int LDS = NBUF * STAGE + (AHEAD ? WAVES * 256 : 0);
     __shared__ __attribute__((aligned(128))) unsigned char lds[LDS];
 
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -170,8 +171,8 @@ __global__ void __launch_bounds__(256, OCC) product_kernel(const Product p) {
     const uint32_t pp = (uint32_t)lane < SHARE / 2 ? pr * (wave < 2 ? lda : ldb) : NOWHERE;
     auto ask = [&](uint32_t kt) __attribute__((always_inline)) {
         const uint32_t v = kt < k_last ? pp : NOWHERE;
-        if (wave < 2) touch(ra, lds0 + 2 * STAGE + (uint32_t)wave * 256u, v, kt * KB);
-        else touch(rb, lds0 + 2 * STAGE + (uint32_t)wave * 256u, v, kt * KB);
+        if (wave < 2) touch(ra, lds0 + NBUF * STAGE + (uint32_t)wave * 256u, v, kt * KB);
+        else touch(rb, lds0 + NBUF * STAGE + (uint32_t)wave * 256u, v, kt * KB);
     };
 
     Acc acc[TM][TN];
@@ -213,27 +214,30 @@ __global__ void __launch_bounds__(256, OCC) product_kernel(const Product p) {
             }
     };
     if (k_first < k_last) {
-        aim(k_first, 0);
 #pragma unroll
-        for (int i = 0; i < 2 * LOADS; ++i) load(i);
-        aim(k_first + 1, 1);
+        for (int b = 0; b < NBUF; ++b) {
+            aim(k_first + b, b);
 #pragma unroll
-        for (int i = 0; i < 2 * LOADS; ++i) load(i);
-        if constexpr (AHEAD) ask(k_first + 2);
-        asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" :: "i"(2 * LOADS + (AHEAD ? 1 : 0)) : "memory");
+            for (int i = 0; i < 2 * LOADS; ++i) load(i);
+        }
+        if constexpr (AHEAD) ask(k_first + NBUF);
+        constexpr int LATER = 2 * LOADS * (NBUF - 2) + (AHEAD ? 1 : 0);     // loads that a tile's barrier leaves
+        asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" :: "i"(2 * LOADS + LATER) : "memory");
 #pragma unroll
         for (int i = 0; i < TM + TN; ++i) read(f0, 0, 0, i);
         wait_lds();
         uint32_t buf = 0;
-        for (uint32_t kt = k_first; kt < k_last; ++kt, buf ^= 1) {
+        for (uint32_t kt = k_first; kt < k_last; ++kt) {
+            const uint32_t next = buf + 1 == NBUF ? 0 : buf + 1;
             multiply(f0, f1, buf, 1, Flag<false>{});
             // every wave has read this tile, and the next one has landed
             wait_lds();
-            asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" :: "i"(AHEAD ? 1 : 0) : "memory");
-            aim(kt + 2, buf);
-            multiply(f1, f0, buf ^ 1, 0, Flag<true>{});
-            if constexpr (AHEAD) ask(kt + 3);
+            asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" :: "i"(LATER) : "memory");
+            aim(kt + NBUF, buf);
+            multiply(f1, f0, next, 0, Flag<true>{});
+            if constexpr (AHEAD) ask(kt + NBUF + 1);
             wait_lds();
+            buf = next;
         }
         // zeros for tiles past the range; and the last products, whose results the
         // compiler does not know to wait for
@@ -475,9 +479,10 @@ template <int E, int DT> hipError_t product_any(const Route& r, Product p, hipSt
     // A second round of work-groups finds its lines in memory, and in a deep K they drift apart;
     // one round of few K tiles is 2% faster unasked.
     const bool ahead = (uint64_t)p.nwgx * p.nwgy * p.splits > kComputeUnits || p.tiles_per_split > 32;
-    const void* f = r.kind ? (const void*)&product_kernel<E, DT, 4, 2, false>
-                           : ahead ? (const void*)&product_kernel<E, DT, 8, 1, true>
-                                   : (const void*)&product_kernel<E, DT, 8, 1, false>;
+    const void* f = r.kind == K_SMALL        ? (const void*)&product_kernel<E, DT, 4, 2, false>
+                    : r.kind == K_SMALL_DEEP ? (const void*)&product_kernel<E, DT, 4, 3, false>
+                    : ahead                  ? (const void*)&product_kernel<E, DT, 8, 2, true>
+                                             : (const void*)&product_kernel<E, DT, 8, 2, false>;
     const hipError_t e = launch(f, dim3(p.nwgx * p.nwgy, p.splits), 256, p, s);
     if (e != hipSuccess || p.splits == 1) return e;
     return launch((const void*)&finish_kernel<E, DT>, dim3((uint32_t)(ceil_div(p.m, 8) * ceil_div(p.n, 256))), 256, p, s);
@@ -505,7 +510,7 @@ hipError_t launch_few(const Product& p, hipStream_t s) {
 
 hipError_t prepare_products() {
     hipFuncAttributes a;
-    return hipFuncGetAttributes(&a, (const void*)&product_kernel<E_I8, Q8_BF16, 4, 2, false>);
+    return hipFuncGetAttributes(&a, (const void*)&product_kernel<E_I8, Q8_BF16, 8, 2, false>);
 }
 
 }  // namespace q8

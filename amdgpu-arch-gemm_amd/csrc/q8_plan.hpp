@@ -16,10 +16,12 @@ constexpr uint64_t kMaxRowBytes = 1u << 22;
 constexpr uint32_t kFewTokens = 64;
 
 struct Tile {
-    uint32_t m, n, resident;   // resident: work-groups of it on a CU
+    uint32_t m, n;
 };
-constexpr Tile kTiles[] = {{256, 256, 1}, {128, 128, 2}};
-constexpr int kTileKinds = 2;
+// The kernels of a product: 256 x 256 tiles, one work-group a CU; 128 x 128 ones, two work-groups a
+// CU with two buffers each; the same with three buffers, one work-group a CU.
+enum Kind { K_LARGE = 0, K_SMALL = 1, K_SMALL_DEEP = 2, K_KINDS = 3 };
+constexpr Tile kTiles[K_KINDS] = {{256, 256}, {128, 128}, {128, 128}};
 
 struct ProductPlan {
     int kind = 0;
@@ -29,25 +31,38 @@ struct ProductPlan {
 
 constexpr uint64_t div_up(uint64_t a, uint64_t b) { return (a + b - 1) / b; }
 
+// Microseconds of `groups` work-groups of `tiles_k` K tiles each on a kernel, fitted to launches
+// back to back: a K tile's time and a fixed one for each round of work-groups.  The large
+// tiles take 1.47 us a K tile whether one or all CUs have one (4096^3 in 8-bit integers: 59
+// us).  Of the small ones, a CU with two takes 1.0 us for a K tile of both; one alone waits for
+// its loads, 0.57 us.  Three buffers make that 0.36 on `spread` rows, those laid out an odd number
+// of lines apart (2048^3 in BF16: 24.8 -> 18.5 us; 1024^3, 8 K tiles: 7.7 -> 10.3, as launches
+// overlap less); rows 4096 bytes apart meet in few memory channels, and it stays (256 x
+// 4096 x 4096 in 8-bit integers: 23.5 against 25.6).
+inline double product_time(int kind, bool spread, uint64_t groups, uint64_t tiles_k) {
+    const double k = (double)tiles_k;
+    if (kind == K_LARGE) return (double)div_up(groups, kComputeUnits) * (1.47 * k + 10.0);
+    if (kind == K_SMALL_DEEP) return (double)div_up(groups, kComputeUnits) * ((spread ? 0.36 : 0.57) * k + 7.0);
+    const uint64_t slots = 2 * kComputeUnits, rest = groups % slots;
+    return (double)(groups / slots) * (1.0 * k + 6.0) + (!rest ? 0.0 : rest <= kComputeUnits ? 0.57 * k + 4.5 : 1.0 * k + 6.0);
+}
+
 // m x n outputs over kb bytes of the summed index.
-inline ProductPlan plan_product(uint64_t m, uint64_t n, uint64_t kb) {
+inline ProductPlan plan_product(uint64_t m, uint64_t n, uint64_t kb, bool spread) {
     ProductPlan best;
     double least = 1e300;
     const uint64_t tiles_k = div_up(kb ? kb : 1, kTileBytes);
-    for (int kind = 0; kind < kTileKinds; ++kind) {
+    for (int kind = 0; kind < K_KINDS; ++kind) {
         const Tile& t = kTiles[kind];
         const uint64_t tiles = div_up(m, t.m) * div_up(n, t.n);
-        const uint64_t slots = (uint64_t)kComputeUnits * t.resident;
-        // a K tile of 256 x 256 takes a work-group about four times as long as one
-        // of 128 x 128 on a CU of its own, and two of the latter share a CU
-        const double step = kind == 0 ? 1.0 : 0.62;
         for (uint32_t s = 1; s <= kMaxSplits; ++s) {
-            if (s > 1 && (tiles >= slots || tiles_k / s < 4)) break;
-            const double rounds = (double)div_up(tiles * s, slots);
-            const double fixed = 3.0 + (s > 1 ? 3.0 + 0.5 * s : 0.0);
-            const double cost = rounds * ((double)div_up(tiles_k, s) + fixed) * step;
-            if (cost < least * 0.999) {
-                least = cost;
+            // K ranges only where work-groups are idle
+            if (s > 1 && (tiles * s > 2 * kComputeUnits || tiles_k / s < 4)) break;
+            // the ranges' sums: written, read and finished by another kernel
+            const double join = s > 1 ? 3.0 + (s + 1.0) * (double)m * (double)n * 4.0 / 3e6 : 0.0;
+            const double time = product_time(kind, spread, tiles * s, div_up(tiles_k, s)) + join;
+            if (time < least * 0.999) {
+                least = time;
                 best.kind = kind;
                 best.splits = s;
             }
@@ -57,9 +72,7 @@ inline ProductPlan plan_product(uint64_t m, uint64_t n, uint64_t kb) {
     const uint64_t tiles = div_up(m, t.m) * div_up(n, t.n);
     // whole ranges: none of the splits is empty
     best.splits = (uint32_t)div_up(tiles_k, div_up(tiles_k, best.splits));
-    if (best.splits > 1) {
-        best.partial_bytes = (size_t)(tiles * best.splits * t.m * t.n * 4);
-    }
+    if (best.splits > 1) best.partial_bytes = (size_t)(tiles * best.splits * t.m * t.n * 4);
     return best;
 }
 

@@ -172,7 +172,7 @@ int plan_grad(int dtype, uint64_t rows, uint64_t cols, uint64_t sum, bool copy_a
     // an odd number of lines: rows of a power of two apart meet in few memory channels
     g.pitch = (g.kb / 128 | 1) * 128;
     if (g.pitch < g.kb) g.pitch += 256;
-    g.plan = plan_product(rows, cols, g.kb);
+    g.plan = plan_product(rows, cols, g.kb, true);
     g.at = Layout();
     if (copy_a || dtype == Q8_F32) g.at.add(g.at.a, rows * g.pitch);
     g.at.add(g.at.b, cols * g.pitch);
@@ -205,7 +205,7 @@ GemmPlan plan_gemm(uint64_t m, uint64_t n, uint64_t k, bool copy_a, bool copy_b)
     g.ldc = round_up(k, 16);
     if (copy_a) g.at.add(g.at.a, m * g.ldc);
     if (copy_b) g.at.add(g.at.b, n * g.ldc);
-    g.plan = plan_product(m, n, k);
+    g.plan = plan_product(m, n, k, false);
     if (g.plan.partial_bytes) g.at.add(g.at.partial, g.plan.partial_bytes);
     return g;
 }
