@@ -4,7 +4,7 @@
 // integers (int32 sums) or 16-bit floats (FP32 sums).  All three have operands of 16
 // bytes a lane and rows of 128 bytes a K tile, so one kernel serves them:
 //   HBM --buffer_load ... lds, 16 bytes a lane--> LDS, two buffers --> MFMA
-// few_kernel: few tokens; the weights go from memory to the matrix cores once.
+// direct_kernel: few tokens; the weights go from memory to the matrix cores once.
 #include "q8_device.hpp"
 #include "q8_internal.hpp"
 #include "q8_plan.hpp"
@@ -100,13 +100,6 @@ template <int V> struct Int { static constexpr int value = V; };
 
 __device__ __forceinline__ float out_value(int v) { return (float)v; }
 __device__ __forceinline__ float out_value(float v) { return v; }
-
-template <int DT> __device__ __forceinline__ float bias_of(const Product& p, uint32_t col) {
-    return Type<DT>::get((const typename Type<DT>::T*)p.bias + col);
-}
-__device__ __forceinline__ float bias_at(const Product& p, uint32_t col) {
-    return p.out == Q8_F32 ? bias_of<Q8_F32>(p, col) : p.out == Q8_F16 ? bias_of<Q8_F16>(p, col) : bias_of<Q8_BF16>(p, col);
-}
 
 // 2 x 2 waves of T x T tiles of 16 x 16: 256 x 256 outputs with T = 8, one wave a SIMD,
 // or 128 x 128 with T = 4, two work-groups a CU.
@@ -367,17 +360,19 @@ template <int E, int DT> __global__ void __launch_bounds__(256) finish_kernel(co
     store_part<DT>(y, col, p.n, v);
 }
 
-// Few tokens (m <= 64).  A work-group owns 16 * NT channels and all of K, in
-// steps of 64 bytes that its waves take in runs of RUN; each lane's weights go from
-// memory straight into an operand.  The waves' sums meet in LDS.
-template <int MT, int NT, int WAVES>
-__global__ void __launch_bounds__(WAVES * 64) few_kernel(const Product p) {
+// Few tokens, or a small product (direct_kind).  A work-group owns 16 * NT channels, 16 * MT tokens and all of K, in
+// runs of four steps of 64 bytes that its waves take in turn; operands go from memory
+// straight to the matrix cores, from rows that start anywhere, with a run's loads in flight
+// while the one before is multiplied.  The waves' sums meet in LDS.
+template <int MT, int NT, int WAVES, int DT>
+__global__ void __launch_bounds__(WAVES * 64) direct_kernel(const Product p) {
     constexpr int RUN = 4;
     typedef Atom<E_I8> A;
+    typedef typename Type<DT>::T Out;
     __shared__ __attribute__((aligned(16))) i32x4 red[WAVES][MT * NT][64];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
     const int fr = lane & 15, fg = lane >> 4;
-    const uint32_t col0 = blockIdx.x * (16 * NT);
+    const uint32_t col0 = blockIdx.x * (16 * NT), row0 = blockIdx.y * (16 * MT);
     const uint32_t whole = p.kb / 64;             // steps without an end inside
     const char* w[NT];
     const char* x[MT];
@@ -390,7 +385,7 @@ __global__ void __launch_bounds__(WAVES * 64) few_kernel(const Product p) {
     }
 #pragma unroll
     for (int i = 0; i < MT; ++i) {
-        const uint32_t r = (uint32_t)(i * 16 + fr);
+        const uint32_t r = row0 + (uint32_t)(i * 16 + fr);
         xok[i] = r < p.m;
         x[i] = (const char*)p.a + (uint64_t)(xok[i] ? r : 0u) * p.lda + fg * 16;
     }
@@ -399,24 +394,38 @@ __global__ void __launch_bounds__(WAVES * 64) few_kernel(const Product p) {
     for (int i = 0; i < MT; ++i)
 #pragma unroll
         for (int j = 0; j < NT; ++j) acc[i][j] = i32x4{0, 0, 0, 0};
+    struct Run {
+        u32x4 w[RUN][NT], x[RUN][MT];
+    };
     const u32x4 zero = {0, 0, 0, 0};
-    for (uint32_t s0 = (uint32_t)wave * RUN; s0 < whole; s0 += WAVES * RUN) {
-        u32x4 wv[RUN][NT], xv[RUN][MT];
+    auto fetch = [&](Run& v, uint32_t s0) __attribute__((always_inline)) {
 #pragma unroll
         for (int s = 0; s < RUN; ++s) {
             const uint64_t at = (uint64_t)(s0 + s) * 64;
             const bool on = s0 + s < whole;
 #pragma unroll
-            for (int j = 0; j < NT; ++j) wv[s][j] = on && wok[j] ? (u32x4)*reinterpret_cast<const u32x4_at1*>(w[j] + at) : zero;
+            for (int j = 0; j < NT; ++j) v.w[s][j] = on && wok[j] ? (u32x4)*reinterpret_cast<const u32x4_at1*>(w[j] + at) : zero;
 #pragma unroll
-            for (int i = 0; i < MT; ++i) xv[s][i] = on && xok[i] ? (u32x4)*reinterpret_cast<const u32x4_at1*>(x[i] + at) : zero;
+            for (int i = 0; i < MT; ++i) v.x[s][i] = on && xok[i] ? (u32x4)*reinterpret_cast<const u32x4_at1*>(x[i] + at) : zero;
         }
+    };
+    auto multiply = [&](const Run& v) __attribute__((always_inline)) {
 #pragma unroll
         for (int s = 0; s < RUN; ++s)
 #pragma unroll
             for (int i = 0; i < MT; ++i)
 #pragma unroll
-                for (int j = 0; j < NT; ++j) A::mfma(wv[s][j], xv[s][i], acc[i][j]);
+                for (int j = 0; j < NT; ++j) A::mfma(v.w[s][j], v.x[s][i], acc[i][j]);
+    };
+    constexpr uint32_t STRIDE = WAVES * RUN;
+    Run v0, v1;
+    uint32_t s0 = (uint32_t)wave * RUN;
+    if (s0 < whole) fetch(v0, s0);
+    for (; s0 < whole; s0 += 2 * STRIDE) {
+        fetch(v1, s0 + STRIDE);     // nothing past the rows' end
+        multiply(v0);
+        fetch(v0, s0 + 2 * STRIDE);
+        multiply(v1);
     }
     if (p.kb % 64 && wave == WAVES - 1) {   // the rest, byte by byte
         const uint32_t k0 = whole * 64 + fg * 16;
@@ -441,24 +450,33 @@ __global__ void __launch_bounds__(WAVES * 64) few_kernel(const Product p) {
     for (int i = 0; i < MT; ++i)
 #pragma unroll
         for (int j = 0; j < NT; ++j) red[wave][i * NT + j][lane] = acc[i][j];
+    // the scales, before the wait for the other waves
+    const int t0 = wave;
+    float sx = 0.0f, sw[4] = {}, bias[4] = {};
+    auto aim = [&](int t) __attribute__((always_inline)) {
+        const uint32_t row = row0 + (uint32_t)(t / NT * 16 + fr), col = col0 + (uint32_t)(t % NT * 16 + fg * 4);
+        if (row >= p.m) return;
+        sx = p.sx[row];
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            if (col + e < p.n) {
+                sw[e] = p.sw[col + e];
+                if (p.bias) bias[e] = Type<DT>::get((const Out*)p.bias + col + e);
+            }
+    };
+    if (t0 < MT * NT) aim(t0);
     __syncthreads();
-    for (int t = wave; t < MT * NT; t += WAVES) {
+    for (int t = t0; t < MT * NT; t += WAVES) {
+        if (t != t0) aim(t);
         i32x4 v = red[0][t][lane];
 #pragma unroll
         for (int k = 1; k < WAVES; ++k) v += red[k][t][lane];
-        const uint32_t row = (uint32_t)(t / NT * 16 + fr), col = col0 + (uint32_t)(t % NT * 16 + fg * 4);
+        const uint32_t row = row0 + (uint32_t)(t / NT * 16 + fr), col = col0 + (uint32_t)(t % NT * 16 + fg * 4);
         if (row >= p.m) continue;
-        const float sx = p.sx[row];
+        Out* y = (Out*)p.y + row * p.ldy + col;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            const uint32_t c = col + e;
-            if (c >= p.n) break;
-            const float y = (float)v[e] * sx * p.sw[c] + (p.bias ? bias_at(p, c) : 0.0f);
-            const uint64_t at = row * p.ldy + c;
-            if (p.out == Q8_F32) ((float*)p.y)[at] = y;
-            else if (p.out == Q8_F16) ((_Float16*)p.y)[at] = (_Float16)y;
-            else ((__bf16*)p.y)[at] = (__bf16)y;
-        }
+        for (int e = 0; e < 4; ++e)
+            if (col + e < p.n) Type<DT>::put(y + e, __builtin_fmaf((float)v[e] * sx, sw[e], bias[e]));
     }
 }
 
@@ -488,9 +506,11 @@ template <int E, int DT> hipError_t product_any(const Route& r, Product p, hipSt
     return launch((const void*)&finish_kernel<E, DT>, dim3((uint32_t)(ceil_div(p.m, 8) * ceil_div(p.n, 256))), 256, p, s);
 }
 
-template <int MT> hipError_t few_any(const Product& p, hipStream_t s) {
-    constexpr int WAVES = 16;
-    return launch((const void*)&few_kernel<MT, 1, WAVES>, dim3((uint32_t)ceil_div(p.n, 16)), WAVES * 64, p, s);
+template <int MT, int NT, int WAVES> hipError_t direct_any(const Product& p, hipStream_t s) {
+    const void* f = p.out == Q8_F32   ? (const void*)&direct_kernel<MT, NT, WAVES, Q8_F32>
+                    : p.out == Q8_F16 ? (const void*)&direct_kernel<MT, NT, WAVES, Q8_F16>
+                                      : (const void*)&direct_kernel<MT, NT, WAVES, Q8_BF16>;
+    return launch(f, dim3((uint32_t)ceil_div(p.n, 16 * NT), (uint32_t)ceil_div(p.m, 16 * MT)), WAVES * 64, p, s);
 }
 
 }  // namespace
@@ -504,8 +524,17 @@ hipError_t launch_product(Element e, const Route& r, const Product& p, hipStream
                            : p.out == Q8_F16 ? product_any<E_I8, Q8_F16>(r, p, s) : product_any<E_I8, Q8_BF16>(r, p, s);
 }
 
-hipError_t launch_few(const Product& p, hipStream_t s) {
-    return p.m <= 16 ? few_any<1>(p, s) : p.m <= 32 ? few_any<2>(p, s) : few_any<4>(p, s);
+hipError_t launch_direct(const Product& p, hipStream_t s) {
+    switch (direct_kind(p.m, p.n, p.kb)) {
+        case D_1x1_16: return direct_any<1, 1, 16>(p, s);
+        case D_1x1_8: return direct_any<1, 1, 8>(p, s);
+        case D_1x4_8: return direct_any<1, 4, 8>(p, s);
+        case D_2x1_8: return direct_any<2, 1, 8>(p, s);
+        case D_2x4_8: return direct_any<2, 4, 8>(p, s);
+        case D_2x2_8: return direct_any<2, 2, 8>(p, s);
+        case D_4x4_4: return direct_any<4, 4, 4>(p, s);
+    }
+    return hipErrorInvalidValue;
 }
 
 hipError_t prepare_products() {

@@ -86,7 +86,7 @@ struct Route {
     uint32_t splits;
 };
 Q8_INTERNAL hipError_t launch_product(Element e, const Route& r, const Product& p, hipStream_t stream);
-Q8_INTERNAL hipError_t launch_few(const Product& p, hipStream_t stream);   // E_I8, m <= 64
+Q8_INTERNAL hipError_t launch_direct(const Product& p, hipStream_t stream);   // E_I8, rows that start anywhere
 Q8_INTERNAL hipError_t prepare_products();   // loads the kernels on the current device
 
 // 8-bit rows to rows of whole 16 bytes: dst[r][0 .. cols) and zeros up to dst_ld.

@@ -12,7 +12,7 @@ constexpr uint32_t kTileBytes = 128;         // of the summed index, a K tile
 constexpr uint32_t kMaxSplits = 16;
 // A tile's rows are addressed with 32-bit offsets from its first one.
 constexpr uint64_t kMaxRowBytes = 1u << 22;
-// Fewest tokens that the tile kernels are used for; below, the weights are streamed once.
+// Up to so many tokens the weights are streamed once, from rows that start anywhere.
 constexpr uint32_t kFewTokens = 64;
 
 struct Tile {
@@ -27,6 +27,7 @@ struct ProductPlan {
     int kind = 0;
     uint32_t splits = 1;
     size_t partial_bytes = 0;
+    double time = 0.0;
 };
 
 constexpr uint64_t div_up(uint64_t a, uint64_t b) { return (a + b - 1) / b; }
@@ -68,12 +69,41 @@ inline ProductPlan plan_product(uint64_t m, uint64_t n, uint64_t kb, bool spread
             }
         }
     }
+    best.time = least;
     const Tile& t = kTiles[best.kind];
     const uint64_t tiles = div_up(m, t.m) * div_up(n, t.n);
     // whole ranges: none of the splits is empty
     best.splits = (uint32_t)div_up(tiles_k, div_up(tiles_k, best.splits));
     if (best.splits > 1) best.partial_bytes = (size_t)(tiles * best.splits * t.m * t.n * 4);
     return best;
+}
+
+// The direct kernel's tiles, 16 MT tokens x 16 NT channels a work-group of WAVES waves:
+//   1 x 1, 16 waves  a small product: a work-group a CU (333 x 129 x 517: 4.2 us, 2 x 1 5.2)
+//   1 x 1, 8 waves   up to 16 tokens (16 x 4096 x 4096: 6.9 us; 16 waves 7.2), and 16 waves over
+//                    a deep K of few channels (1 x 4096 x 16384: 14.5 against 16.9)
+//   1 x 4, 8 waves   up to 16 tokens into many channels: the tokens are read a quarter as often
+//                    (16 x 16384 x 4096: 15.8 us, 1 x 1 19.0)
+//   2 x 1, 2 x 4     the same up to 32 tokens (32 x 16384 x 4096: 18.4 us, 2 x 1 26.8)
+//   2 x 2, 4 x 4     and up to 64 (64 x 4096 x 4096: 10.4 us, 2 x 1 14.1, 4 x 1 12.5;
+//                    64 x 16384 x 4096: 25.2 us, 2 x 2 40.8)
+enum Direct { D_1x1_16, D_1x1_8, D_1x4_8, D_2x1_8, D_2x4_8, D_2x2_8, D_4x4_4 };
+inline Direct direct_kind(uint64_t m, uint64_t n, uint64_t k) {
+    const bool wide = n >= 12288;
+    if (m <= 16) return wide ? D_1x4_8 : n <= 4096 && k > 8192 ? D_1x1_16 : D_1x1_8;
+    if (div_up(m, 16) * div_up(n, 16) <= kComputeUnits) return D_1x1_16;
+    if (m <= 32) return wide ? D_2x4_8 : D_2x1_8;
+    if (m <= kFewTokens) return wide ? D_4x4_4 : D_2x2_8;
+    return D_2x1_8;
+}
+// Whether more tokens run on it too: a small product, which the tile kernels would spend on
+// whole tiles and on copies of rows that are not theirs (`copies` launches, `copy_bytes` in all).
+inline bool direct_for_many(uint64_t m, uint64_t n, uint64_t k, double tile_time, int copies, uint64_t copy_bytes) {
+    if (m > (1u << 20)) return false;   // a grid's second dimension ends at 65535
+    const uint64_t t = div_up(m, 16) * div_up(n, 16);
+    const double rows = t <= kComputeUnits ? 32.0 * (double)t : 48.0 * (double)(div_up(m, 32) * div_up(n, 16));
+    const double direct = 3.8 + rows * (double)k / 7e6;     // each work-group's rows, out of L2
+    return direct < tile_time + 3.0 * copies + 2.0 * (double)copy_bytes / 3e6;
 }
 
 }  // namespace q8

@@ -191,21 +191,22 @@ int check_grid(uint64_t m, uint64_t n, const ProductPlan& p) {
 }
 
 struct GemmPlan {
-    bool few = false, copy_a = false, copy_b = false;
+    bool direct = false, copy_a = false, copy_b = false;
     uint64_t ldc = 0;   // bytes of a copied row
     ProductPlan plan;
     Layout at;
 };
 GemmPlan plan_gemm(uint64_t m, uint64_t n, uint64_t k, bool copy_a, bool copy_b) {
     GemmPlan g;
-    g.few = m <= kFewTokens;
-    if (g.few) return g;
+    g.ldc = round_up(k, 16);
+    g.plan = plan_product(m, n, k, false);
+    g.direct = m <= kFewTokens || direct_for_many(m, n, k, g.plan.time, (int)copy_a + (int)copy_b,
+                                                  (copy_a ? m * g.ldc : 0) + (copy_b ? n * g.ldc : 0));
+    if (g.direct) return g;
     g.copy_a = copy_a;
     g.copy_b = copy_b;
-    g.ldc = round_up(k, 16);
     if (copy_a) g.at.add(g.at.a, m * g.ldc);
     if (copy_b) g.at.add(g.at.b, n * g.ldc);
-    g.plan = plan_product(m, n, k, false);
     if (g.plan.partial_bytes) g.at.add(g.at.partial, g.plan.partial_bytes);
     return g;
 }
@@ -298,7 +299,10 @@ int q8_workspace_size(int call, int dtype, uint32_t m, uint32_t n, uint32_t k, s
     if (call == Q8_CALL_RMSNORM_BACKWARD) {
         *bytes = piece((size_t)norm_backward_parts(m, k) * k * sizeof(float));
     } else if (call == Q8_CALL_GEMM) {
-        *bytes = plan_gemm(m, n, k, true, true).at.total;
+        for (int copies = 0; copies < 4; ++copies) {    // the route depends on them
+            const size_t need = plan_gemm(m, n, k, copies & 1, copies & 2).at.total;
+            if (need > *bytes) *bytes = need;
+        }
     } else if (call == Q8_CALL_GRAD_INPUT || call == Q8_CALL_GRAD_WEIGHT) {
         Grad g;
         if (call == Q8_CALL_GRAD_INPUT) CHECK(plan_grad(dtype, m, k, n, true, g));
@@ -418,14 +422,15 @@ int q8_gemm(q8_handle* h, int dtype, const int8_t* qx, uint32_t ldx, const float
     // a sum that ends inside a piece of 16 bytes: qx's copy has zeros there, and what qw has
     // is multiplied by them
     const GemmPlan g = plan_gemm(m, n, k, !rows_aligned(qx, ldx) || k % 16, !rows_aligned(qw, ldw));
-    if (!g.few) CHECK(check_grid(m, n, g.plan));
+    if (!g.direct) CHECK(check_grid(m, n, g.plan));
+    else if (n >= (1u << 28)) return fail(SGEMM_E_SHAPE, "%u channels are more than a grid holds", n);
     OnDevice on(h->device);
     HIP_TRY(on.status());
     CHECK(take_workspace(h, g.at.total));
     Product p = {};
     p.a = qx; p.b = qw; p.lda = ldx; p.ldb = ldw; p.m = m; p.n = n; p.kb = k;
     p.sx = sx; p.sw = sw; p.bias = bias; p.y = y; p.ldy = ldy; p.out = dtype;
-    if (g.few) return launched(launch_few(p, h->stream), "launch of the product failed");
+    if (g.direct) return launched(launch_direct(p, h->stream), "launch of the product failed");
     if (g.copy_a) {
         p.a = h->workspace + g.at.a;
         p.lda = g.ldc;
