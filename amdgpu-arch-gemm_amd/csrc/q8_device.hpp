@@ -20,6 +20,7 @@ typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 // alignment, so rows may start anywhere
 typedef u32x4 u32x4_at2 __attribute__((aligned(2)));
 typedef f32x4 f32x4_at4 __attribute__((aligned(4)));
+typedef uint32_t u32_at1 __attribute__((aligned(1)));
 typedef u32x2 u32x2_at1 __attribute__((aligned(1)));
 typedef u32x4 u32x4_at1 __attribute__((aligned(1)));
 

@@ -92,30 +92,31 @@ Q8_INTERNAL hipError_t prepare_products();   // loads the kernels on the current
 // 8-bit rows to rows of whole 16 bytes: dst[r][0 .. cols) and zeros up to dst_ld.
 Q8_INTERNAL hipError_t launch_copy_rows(const int8_t* src, uint64_t src_ld, int8_t* dst, uint64_t dst_ld, uint32_t rows,
                                         uint32_t cols, hipStream_t stream);
-// dst[j][t * cp + c] = scale_c q_cj (times pair[0] where pair is not null) in `e`
-// for c < rows, 0 up to cp; E_BF16 with terms == 3: q_cj alone, three times.
+// The two operands of a gradient, laid out with the summed index along the rows, `cp` values of
+// it (a multiple of eight; zeros past the `rows` or `cols` of the source).
+//   weights:  dst[j][t * cp + c] = scale_c q_cj, rounded to 16 bits; with scale == null (F32)
+//             q_cj alone, `terms` times.  F16: times pair[0] = 2^-e, and pair[1] = 2^e, such that
+//             the largest finite scale * 2^-e is in [2^7, 2^8); both are set here.
+//   gradient: dst[i][t * cp + c] = term t of src_ic (transposed: src_ci).  16-bit types: one term,
+//             copied; F32: scaled by scale_c, three BF16 terms.
+// dst_ld and src_ld in elements.
 struct PackWeights {
     const int8_t* q;
-    const float* scale;   // null: 1
-    const float* pair;
+    const float* scale;
+    float* pair;
     void* dst;
-    uint64_t ldq, dst_ld; // dst_ld in elements
+    uint64_t ldq, dst_ld;
     uint32_t rows, cols, cp, terms;
 };
-Q8_INTERNAL hipError_t launch_pack_weights(Element e, const PackWeights& p, hipStream_t stream);
-// dst[i][t * cp + c] = term t of src_ic (transposed: src_ci), scaled by scale_c
-// where scale is not null, 0 up to cp.  16-bit types: one term, copied.  F32: three
-// BF16 terms.
 struct PackGradient {
     const void* src;
     const float* scale;
     void* dst;
-    uint64_t src_ld, dst_ld;  // elements
+    uint64_t src_ld, dst_ld;
     uint32_t rows, cols, cp;  // rows: of dst; cols: values of the summed index
     int transposed;
 };
-Q8_INTERNAL hipError_t launch_pack_gradient(int dtype, const PackGradient& p, hipStream_t stream);
-// pair[0] = 2^-e, pair[1] = 2^e with the largest finite scale * 2^-e in [2^7, 2^8)
-Q8_INTERNAL hipError_t launch_scale_pair(const float* scale, uint32_t count, float* pair, hipStream_t stream);
+// gradient: null where it is read as it is.
+Q8_INTERNAL hipError_t launch_pack(int dtype, const PackWeights& weights, const PackGradient* gradient, hipStream_t stream);
 
 }  // namespace q8

@@ -40,151 +40,161 @@ __device__ __forceinline__ uint16_t bits16(float x, bool half) {
     if (half) return __builtin_bit_cast(uint16_t, (_Float16)x);
     return __builtin_bit_cast(uint16_t, (__bf16)x);
 }
+template <bool HALF> __device__ __forceinline__ uint32_t pair16(float x, float y) {
+    return HALF ? Type<Q8_F16>::pair(x, y) : Type<Q8_BF16>::pair(x, y);
+}
 
-// A tile of 64 x 64 turned in LDS: values are written as [column][row], rows of
-// 64 + 8 so that neither side's accesses of 16 bytes share banks more than they must.
-constexpr int TILE = 64, PITCH = TILE + 8;
+// Turning needs no LDS: a lane takes eight rows of the source, W values of each, and has eight
+// consecutive values of the summed index for each of its columns, a store of 16 bytes.
+// Eight lanes side by side read a piece of a row, and eight others with the next rows
+// store 128 bytes of a column.  A wave turns 64 rows.
 
-// q: rows (summed index) x cols; dst: cols rows of cp (times terms).
-template <bool HALF> __global__ void __launch_bounds__(256) pack_weights_kernel(const PackWeights p) {
-    __shared__ __attribute__((aligned(16))) uint16_t tile[TILE * PITCH];
-    const uint32_t tr = (p.cp + TILE - 1) / TILE, tc = (p.cols + TILE - 1) / TILE;
-    const float factor = p.pair ? p.pair[0] : 1.0f;
-    for (uint64_t t = blockIdx.x; t < (uint64_t)tr * tc; t += gridDim.x) {
-        const uint32_t r0 = (uint32_t)(t % tr) * TILE, c0 = (uint32_t)(t / tr) * TILE;
-        const uint32_t r = r0 + threadIdx.x / 4, c = c0 + threadIdx.x % 4 * 16;
-        int8_t v[16];
-        float s = 1.0f;
+// q: rows (summed index) x cols; dst: cols rows of cp (times terms).  W = 16 bytes a lane, or 4 where
+// that leaves CUs without waves.
+template <bool HALF, int W>
+__device__ __forceinline__ void pack_weights(const PackWeights& p, uint32_t wave_id, float factor) {
+    const uint32_t tr = (p.cp + 63) / 64;
+    const uint32_t lane = threadIdx.x & 63;
+    const uint32_t r = wave_id % tr * 64 + lane % 8 * 8, c = wave_id / tr * (8 * W) + lane / 8 * W;
+    if (r >= p.cp || c >= p.cols) return;
+    uint32_t in[8][W / 4];
+    float s[8];
 #pragma unroll
-        for (int e = 0; e < 16; ++e) v[e] = 0;
-        if (r < p.rows && c < p.cols) {
-            const int8_t* src = p.q + (uint64_t)r * p.ldq + c;
-            if (c + 16 <= p.cols) {
-                const u32x4 w = *reinterpret_cast<const u32x4_at1*>(src);
+    for (int k = 0; k < 8; ++k) {
 #pragma unroll
-                for (int e = 0; e < 16; ++e) v[e] = (int8_t)(w[e / 4] >> (8 * (e % 4)));
+        for (int e = 0; e < W / 4; ++e) in[k][e] = 0;
+        s[k] = 0.0f;
+        if (r + k < p.rows) {
+            const int8_t* src = p.q + (uint64_t)(r + k) * p.ldq + c;
+            if (c + W <= p.cols) {
+                if constexpr (W == 16) {
+                    const u32x4 w = *reinterpret_cast<const u32x4_at1*>(src);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) in[k][e] = w[e];
+                } else {
+                    in[k][0] = *reinterpret_cast<const u32_at1*>(src);
+                }
             } else {
 #pragma unroll
-                for (int e = 0; e < 16; ++e)
-                    if (c + e < p.cols) v[e] = src[e];
+                for (int e = 0; e < W; ++e)
+                    if (c + e < p.cols) in[k][e / 4] |= (uint32_t)(uint8_t)src[e] << (8 * (e % 4));
             }
-            if (p.scale) s = p.scale[r] * factor;
+            s[k] = p.scale ? p.scale[r + k] * factor : 1.0f;
         }
-        __syncthreads();
+    }
+    uint16_t* dst = (uint16_t*)p.dst + (uint64_t)c * p.dst_ld + r;
 #pragma unroll
-        for (int e = 0; e < 16; ++e) {
-            // a scale that is not a number takes its whole row along, zeros too
-            const float x = r < p.rows ? (float)v[e] * s : 0.0f;
-            tile[(threadIdx.x % 4 * 16 + e) * PITCH + threadIdx.x / 4] = bits16(x, HALF);
-        }
-        __syncthreads();
+    for (int e = 0; e < W; ++e) {
+        if (c + e >= p.cols) break;
+        float v[8];
+        // a scale that is not a number takes its whole row along, zeros too
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            const uint32_t oc = threadIdx.x / 8 + 32 * i, k = threadIdx.x % 8 * 8;
-            if (c0 + oc < p.cols && r0 + k < p.cp) {
-                const u32x4 w = *reinterpret_cast<const u32x4*>(&tile[oc * PITCH + k]);
-                uint16_t* d = (uint16_t*)p.dst + (uint64_t)(c0 + oc) * p.dst_ld + r0 + k;
-                for (uint32_t q = 0; q < p.terms; ++q) *reinterpret_cast<u32x4*>(d + (uint64_t)q * p.cp) = w;
-            }
-        }
+        for (int k = 0; k < 8; ++k) v[k] = (float)(int8_t)(in[k][e / 4] >> (8 * (e % 4))) * s[k];
+        const u32x4 w = {pair16<HALF>(v[0], v[1]), pair16<HALF>(v[2], v[3]), pair16<HALF>(v[4], v[5]), pair16<HALF>(v[6], v[7])};
+        uint16_t* d = dst + (uint64_t)e * p.dst_ld;
+        for (uint32_t q = 0; q < p.terms; ++q) *reinterpret_cast<u32x4*>(d + (uint64_t)q * p.cp) = w;
     }
 }
 
 // x = hi + mid + lo in BF16: both differences are exact, and three terms of 8 bits
 // hold the 24 of FP32.  Infinities and NaN stay in the first term.
 __device__ __forceinline__ void three(float x, uint16_t (&b)[3]) {
-    const bool fine = magnitude(x) < 0x7f7f8000u;    // rounds to a finite BF16
-    if (!fine && magnitude(x) < 0x7f800000u) {
-        // finite, but the nearest BF16 is not: cut the first term off instead
-        const uint32_t u = __builtin_bit_cast(uint32_t, x) & 0xffff0000u;
-        b[0] = (uint16_t)(u >> 16);
-        const float r = x - __builtin_bit_cast(float, u);
-        b[1] = bits16(r, false);
-        b[2] = bits16(r - __builtin_bit_cast(float, (uint32_t)b[1] << 16), false);
-        return;
-    }
-    b[0] = bits16(x, false);
-    const float r = fine ? x - __builtin_bit_cast(float, (uint32_t)b[0] << 16) : 0.0f;
+    const uint32_t size = magnitude(x);
+    uint32_t hi = (uint32_t)bits16(x, false) << 16;
+    // finite, but the nearest BF16 is not: the first term is cut off instead
+    if (size >= 0x7f7f8000u && size < 0x7f800000u) hi = __builtin_bit_cast(uint32_t, x) & 0xffff0000u;
+    const float r = size < 0x7f800000u ? x - __builtin_bit_cast(float, hi) : 0.0f;
+    b[0] = (uint16_t)(hi >> 16);
     b[1] = bits16(r, false);
     b[2] = bits16(r - __builtin_bit_cast(float, (uint32_t)b[1] << 16), false);
 }
 
-template <int DT, bool TURN> __global__ void __launch_bounds__(256) pack_gradient_kernel(const PackGradient p) {
+// Eight 16-bit patterns of a row from column c (0 past `cols`), for FP32 in three terms.
+template <int DT, int TERMS>
+__device__ __forceinline__ void eight(const void* src, uint64_t ld, uint32_t row, uint32_t c, uint32_t cols, const float* scale,
+                                      bool scale_by_row, uint32_t (&out)[TERMS][4]) {
     typedef typename Type<DT>::T T;
-    constexpr int TERMS = DT == Q8_F32 ? 3 : 1;
-    __shared__ __attribute__((aligned(16))) uint16_t tile[TERMS][TILE * PITCH];
-    const uint32_t tk = (p.cp + TILE - 1) / TILE, tr = (p.rows + TILE - 1) / TILE;
-    for (uint64_t t = blockIdx.x; t < (uint64_t)tk * tr; t += gridDim.x) {
-        const uint32_t k0 = (uint32_t)(t % tk) * TILE, r0 = (uint32_t)(t / tk) * TILE;
-        __syncthreads();
+    const T* line = (const T*)src + (uint64_t)row * ld;
+    if constexpr (DT == Q8_F32) {
+        float v[8];
+        load_part<DT>(line, c, cols, v);
+        if (scale) {
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            // eight values along the source's rows
-            const uint32_t line = threadIdx.x / 8 + 32 * i, at = threadIdx.x % 8 * 8;
-            const uint32_t sr = (TURN ? k0 : r0) + line, sc = (TURN ? r0 : k0) + at;
-            const uint32_t srows = TURN ? p.cols : p.rows, scols = TURN ? p.rows : p.cols;
-            float v[8];
-            uint16_t raw[8];
-#pragma unroll
-            for (int e = 0; e < 8; ++e) { v[e] = 0.0f; raw[e] = 0; }
-            if (sr < srows && sc < scols) {
-                const T* src = (const T*)p.src + (uint64_t)sr * p.src_ld + sc;
-                if constexpr (DT == Q8_F32) {
-                    load_part<DT>(src - sc, sc, scols, v);
-                    if (p.scale) {
-#pragma unroll
-                        for (int e = 0; e < 8; ++e) {
-                            const uint32_t k = TURN ? sr : sc + e;
-                            if (sc + e < scols) v[e] *= p.scale[k];
-                        }
-                    }
-                } else {
-                    if (sc + 8 <= scols) {
-                        const u32x4 w = *reinterpret_cast<const u32x4_at2*>(src);
-#pragma unroll
-                        for (int e = 0; e < 8; ++e) raw[e] = (uint16_t)(w[e / 2] >> (16 * (e % 2)));
-                    } else {
-#pragma unroll
-                        for (int e = 0; e < 8; ++e)
-                            if (sc + e < scols) raw[e] = __builtin_bit_cast(uint16_t, src[e]);
-                    }
-                }
-            }
-            uint16_t b[8][3];
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                if constexpr (DT == Q8_F32) three(v[e], b[e]);
-                else b[e][0] = raw[e];
-            }
-#pragma unroll
-            for (int q = 0; q < TERMS; ++q)
-#pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    if constexpr (TURN) tile[q][(at + e) * PITCH + line] = b[e][q];
-                    else tile[q][line * PITCH + at + e] = b[e][q];
-                }
+            for (int e = 0; e < 8; ++e)
+                if (c + e < cols) v[e] *= scale[scale_by_row ? row : c + e];
         }
-        __syncthreads();
+        uint16_t b[8][3];
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            const uint32_t row = threadIdx.x / 8 + 32 * i, k = threadIdx.x % 8 * 8;
-            if (r0 + row < p.rows && k0 + k < p.cp) {
-                uint16_t* d = (uint16_t*)p.dst + (uint64_t)(r0 + row) * p.dst_ld + k0 + k;
+        for (int e = 0; e < 8; ++e) three(v[e], b[e]);
 #pragma unroll
-                for (int q = 0; q < TERMS; ++q)
-                    *reinterpret_cast<u32x4*>(d + (uint64_t)q * p.cp) = *reinterpret_cast<const u32x4*>(&tile[q][row * PITCH + k]);
+        for (int q = 0; q < TERMS; ++q)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) out[q][e] = (uint32_t)b[2 * e][q] | (uint32_t)b[2 * e + 1][q] << 16;
+    } else {
+        if (cols - c >= 8) {
+            const u32x4 w = *reinterpret_cast<const u32x4_at2*>(line + c);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) out[0][e] = w[e];
+        } else {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) out[0][e] = 0;
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+                if (c + e < cols) out[0][e / 2] |= (uint32_t)__builtin_bit_cast(uint16_t, line[c + e]) << (16 * (e % 2));
+        }
+    }
+}
+
+// dst[i][c] from src[i][c]: eight values a lane.
+template <int DT> __device__ __forceinline__ void pack_rows(const PackGradient& p, uint64_t id) {
+    constexpr int TERMS = DT == Q8_F32 ? 3 : 1;
+    const uint32_t pieces = p.cp / 8;
+    const uint64_t row = id / pieces;
+    const uint32_t c = (uint32_t)(id % pieces) * 8;
+    if (row >= p.rows) return;
+    uint32_t v[TERMS][4] = {};
+    if (c < p.cols) eight<DT, TERMS>(p.src, p.src_ld, (uint32_t)row, c, p.cols, p.scale, false, v);
+#pragma unroll
+    for (int q = 0; q < TERMS; ++q)
+        *reinterpret_cast<u32x4*>((uint16_t*)p.dst + row * p.dst_ld + (uint64_t)q * p.cp + c) =
+            u32x4{v[q][0], v[q][1], v[q][2], v[q][3]};
+}
+
+// dst[i][c] from src[c][i]: a wave turns 64 x 64.
+template <int DT> __device__ __forceinline__ void pack_turned(const PackGradient& p, uint32_t wave_id) {
+    constexpr int TERMS = DT == Q8_F32 ? 3 : 1;
+    const uint32_t tk = (p.cp + 63) / 64;
+    const uint32_t lane = threadIdx.x & 63;
+    const uint32_t k0 = wave_id % tk * 64 + lane % 8 * 8, r = wave_id / tk * 64 + lane / 8 * 8;
+    if (k0 >= p.cp || r >= p.rows) return;
+    uint32_t in[8][TERMS][4] = {};
+#pragma unroll
+    for (int k = 0; k < 8; ++k)
+        if (k0 + k < p.cols) eight<DT, TERMS>(p.src, p.src_ld, k0 + k, r, p.rows, p.scale, true, in[k]);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        if (r + e >= p.rows) break;
+#pragma unroll
+        for (int q = 0; q < TERMS; ++q) {
+            uint32_t w[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const uint32_t lo = in[2 * k][q][e / 2], hi = in[2 * k + 1][q][e / 2];
+                w[k] = e % 2 ? lo >> 16 | (hi & 0xffff0000u) : (lo & 0xffffu) | hi << 16;
             }
+            *reinterpret_cast<u32x4*>((uint16_t*)p.dst + (uint64_t)(r + e) * p.dst_ld + (uint64_t)q * p.cp + k0) =
+                u32x4{w[0], w[1], w[2], w[3]};
         }
     }
 }
 
 // Half precision keeps 2^-14 .. 2^15 with all its bits, and the weights' values are
 // q scale: a power of two brings the largest scale to 2^7 .. 2^8 (127 times it still fits),
-// and the product is multiplied by its inverse in 32 bits.
-__global__ void __launch_bounds__(1024) scale_pair_kernel(const float* scale, uint32_t count, float* pair) {
-    __shared__ uint32_t red[16];
+// and the product is multiplied by its inverse in 32 bits.  The largest finite scale over a
+// work-group:
+template <int THREADS> __device__ __forceinline__ uint32_t largest(const float* scale, uint32_t count, uint32_t (&red)[THREADS / 64]) {
     uint32_t top = 0;
-    for (uint32_t i = threadIdx.x; i < count; i += 1024) {
+    for (uint32_t i = threadIdx.x; i < count; i += THREADS) {
         const uint32_t a = magnitude(scale[i]);
         if (a < 0x7f800000u) top = top > a ? top : a;
     }
@@ -192,13 +202,55 @@ __global__ void __launch_bounds__(1024) scale_pair_kernel(const float* scale, ui
     wave_sum_max(none, top);
     if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = top;
     __syncthreads();
-    if (threadIdx.x == 0) {
 #pragma unroll
-        for (int w = 1; w < 16; ++w) top = top > red[w] ? top : red[w];
-        int e = (int)(top >> 23) - 127 - 7;           // scale in [2^(e + 7), 2^(e + 8))
-        e = e < -126 ? -126 : e > 126 ? 126 : e;      // both powers stay normal
-        pair[0] = __builtin_bit_cast(float, (uint32_t)(127 - e) << 23);
-        pair[1] = __builtin_bit_cast(float, (uint32_t)(127 + e) << 23);
+    for (int w = 0; w < THREADS / 64; ++w) top = top > red[w] ? top : red[w];
+    return top;
+}
+// 2^-e and 2^e
+__device__ __forceinline__ void powers(uint32_t top, float& down, float& up) {
+    int e = (int)(top >> 23) - 127 - 7;           // scale in [2^(e + 7), 2^(e + 8))
+    e = e < -126 ? -126 : e > 126 ? 126 : e;      // both powers stay normal
+    down = __builtin_bit_cast(float, (uint32_t)(127 - e) << 23);
+    up = __builtin_bit_cast(float, (uint32_t)(127 + e) << 23);
+}
+__global__ void __launch_bounds__(1024) scale_pair_kernel(const float* scale, uint32_t count, float* pair) {
+    __shared__ uint32_t red[16];
+    const uint32_t top = largest<1024>(scale, count, red);
+    if (threadIdx.x == 0) powers(top, pair[0], pair[1]);
+}
+
+// Both operands of a gradient in one launch: the first work-groups lay out the weights, the
+// others the gradient.  Few scales (KNOWN == false) are looked through by every work-group
+// that needs their largest, which costs less than a launch.
+struct PackBoth {
+    PackWeights w;
+    PackGradient g;
+    uint64_t weight_groups, groups;
+    int wide;   // pack_weights' W is 16
+};
+constexpr uint32_t kFewScales = 4096;
+template <int DT, bool TURN, bool KNOWN> __global__ void __launch_bounds__(256) pack_kernel(const PackBoth p) {
+    constexpr bool HALF = DT == Q8_F16;
+    __shared__ uint32_t red[4];
+    float factor = 1.0f;
+    if constexpr (HALF) {
+        if (KNOWN) {
+            factor = p.w.pair[0];
+        } else if (blockIdx.x < p.weight_groups) {
+            float up;
+            powers(largest<256>(p.w.scale, p.w.rows, red), factor, up);
+            if (blockIdx.x == 0 && threadIdx.x == 0) { p.w.pair[0] = factor; p.w.pair[1] = up; }
+        }
+    }
+    for (uint64_t b = blockIdx.x; b < p.groups; b += gridDim.x) {
+        if (b < p.weight_groups) {
+            if (p.wide) pack_weights<HALF, 16>(p.w, (uint32_t)b * 4 + threadIdx.x / 64, factor);
+            else pack_weights<HALF, 4>(p.w, (uint32_t)b * 4 + threadIdx.x / 64, factor);
+        } else if (TURN) {
+            pack_turned<DT>(p.g, (uint32_t)(b - p.weight_groups) * 4 + threadIdx.x / 64);
+        } else {
+            pack_rows<DT>(p.g, (b - p.weight_groups) * 256 + threadIdx.x);
+        }
     }
 }
 
@@ -209,9 +261,19 @@ hipError_t launch(void (*f)(P), uint64_t groups, const P& p, hipStream_t stream)
                            dim3(256), args, 0, stream);
 }
 
-template <int DT> hipError_t pack_gradient_any(const PackGradient& p, uint64_t groups, hipStream_t s) {
-    return p.transposed ? launch(pack_gradient_kernel<DT, true>, groups, p, s)
-                        : launch(pack_gradient_kernel<DT, false>, groups, p, s);
+template <int DT> hipError_t pack_any(const PackBoth& p, hipStream_t s) {
+    const bool known = DT != Q8_F16 || p.w.rows > kFewScales;
+    if (DT == Q8_F16 && known) {
+        const float* scale = p.w.scale;
+        uint32_t count = p.w.rows;
+        float* pair = p.w.pair;
+        void* args[] = {&scale, &count, &pair};
+        const hipError_t e = hipLaunchKernel(reinterpret_cast<const void*>(&scale_pair_kernel), dim3(1), dim3(1024), args, 0, s);
+        if (e != hipSuccess) return e;
+    }
+    if (p.g.transposed)
+        return known ? launch(pack_kernel<DT, true, true>, p.groups, p, s) : launch(pack_kernel<DT, true, false>, p.groups, p, s);
+    return known ? launch(pack_kernel<DT, false, true>, p.groups, p, s) : launch(pack_kernel<DT, false, false>, p.groups, p, s);
 }
 
 }  // namespace
@@ -222,20 +284,19 @@ hipError_t launch_copy_rows(const int8_t* src, uint64_t src_ld, int8_t* dst, uin
     return launch(copy_rows_kernel, ceil_div((uint64_t)rows * (dst_ld / 16), 256), p, s);
 }
 
-hipError_t launch_pack_weights(Element e, const PackWeights& p, hipStream_t s) {
-    const uint64_t groups = ceil_div(p.cp, TILE) * ceil_div(p.cols, TILE);
-    return e == E_F16 ? launch(pack_weights_kernel<true>, groups, p, s) : launch(pack_weights_kernel<false>, groups, p, s);
-}
-
-hipError_t launch_pack_gradient(int dtype, const PackGradient& p, hipStream_t s) {
-    const uint64_t groups = ceil_div(p.cp, TILE) * ceil_div(p.rows, TILE);
-    return dtype == Q8_F32 ? pack_gradient_any<Q8_F32>(p, groups, s)
-                           : dtype == Q8_F16 ? pack_gradient_any<Q8_F16>(p, groups, s) : pack_gradient_any<Q8_BF16>(p, groups, s);
-}
-
-hipError_t launch_scale_pair(const float* scale, uint32_t count, float* pair, hipStream_t s) {
-    void* args[] = {&scale, &count, &pair};
-    return hipLaunchKernel(reinterpret_cast<const void*>(&scale_pair_kernel), dim3(1), dim3(1024), args, 0, s);
+hipError_t launch_pack(int dtype, const PackWeights& w, const PackGradient* g, hipStream_t s) {
+    PackBoth p = {};
+    p.w = w;
+    // 8 waves a CU, or pieces a quarter as large
+    p.wide = ceil_div(w.cp, 64) * ceil_div(w.cols, 128) >= 2048;
+    p.weight_groups = ceil_div(ceil_div(w.cp, 64) * ceil_div(w.cols, p.wide ? 128 : 32), 4);
+    p.groups = p.weight_groups;
+    if (g) {
+        p.g = *g;
+        p.groups += g->transposed ? ceil_div(ceil_div(g->cp, 64) * ceil_div(g->rows, 64), 4)
+                                  : ceil_div((uint64_t)g->rows * (g->cp / 8), 256);
+    }
+    return dtype == Q8_F32 ? pack_any<Q8_F32>(p, s) : dtype == Q8_F16 ? pack_any<Q8_F16>(p, s) : pack_any<Q8_BF16>(p, s);
 }
 
 }  // namespace q8

@@ -466,14 +466,14 @@ int q8_grad_input(q8_handle* h, int dtype, const void* dy, uint32_t lddy, const 
     CHECK(take_workspace(h, g.at.total));
     const Element e = dtype == Q8_F16 ? E_F16 : E_BF16;
     float* pair = dtype == Q8_F16 ? reinterpret_cast<float*>(h->workspace + g.at.pair) : nullptr;
-    if (pair) HIP_TRY(launch_scale_pair(sw, n, pair, h->stream));
-    const PackWeights pw = {qw, dtype == Q8_F32 ? nullptr : sw, pair, h->workspace + g.at.b, ldw, g.pitch / 2, n, k,
-                            (uint32_t)g.cp, g.terms};
-    if (n) HIP_TRY(launch_pack_weights(e, pw, h->stream));
-    if (copy && n) {
+    if (n) {
+        const PackWeights pw = {qw, dtype == Q8_F32 ? nullptr : sw, pair, h->workspace + g.at.b, ldw, g.pitch / 2, n, k,
+                                (uint32_t)g.cp, g.terms};
         const PackGradient pg = {dy, dtype == Q8_F32 ? sw : nullptr, h->workspace + g.at.a, lddy, g.pitch / 2, m, n,
                                  (uint32_t)g.cp, 0};
-        HIP_TRY(launch_pack_gradient(dtype, pg, h->stream));
+        HIP_TRY(launch_pack(dtype, pw, copy ? &pg : nullptr, h->stream));
+    } else {
+        pair = nullptr;
     }
     Product p = {};
     p.a = copy ? h->workspace + g.at.a : dy;
@@ -508,14 +508,14 @@ int q8_grad_weight(q8_handle* h, int dtype, const void* dy, uint32_t lddy, const
     CHECK(take_workspace(h, g.at.total));
     const Element e = dtype == Q8_F16 ? E_F16 : E_BF16;
     float* pair = dtype == Q8_F16 ? reinterpret_cast<float*>(h->workspace + g.at.pair) : nullptr;
-    if (pair) HIP_TRY(launch_scale_pair(sx, m, pair, h->stream));
     if (m) {
         const PackWeights pw = {qx, dtype == Q8_F32 ? nullptr : sx, pair, h->workspace + g.at.b, ldx, g.pitch / 2, m, k,
                                 (uint32_t)g.cp, g.terms};
-        HIP_TRY(launch_pack_weights(e, pw, h->stream));
         const PackGradient pg = {dy, dtype == Q8_F32 ? sx : nullptr, h->workspace + g.at.a, lddy, g.pitch / 2, n, m,
                                  (uint32_t)g.cp, 1};
-        HIP_TRY(launch_pack_gradient(dtype, pg, h->stream));
+        HIP_TRY(launch_pack(dtype, pw, &pg, h->stream));
+    } else {
+        pair = nullptr;
     }
     Product p = {};
     p.a = h->workspace + g.at.a;
