@@ -21,8 +21,8 @@ __global__ void __launch_bounds__(256) copy_rows_kernel(const CopyRows p) {
     const uint32_t pieces = (uint32_t)(p.dst_ld / 16);
     const uint64_t total = (uint64_t)p.rows * pieces;
     for (uint64_t i = (uint64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (uint64_t)gridDim.x * 256) {
-        const uint64_t row = i / pieces;
-        const uint32_t c = (uint32_t)(i % pieces) * 16;
+        const uint64_t row = i >> 32 ? i / pieces : (uint32_t)i / pieces;
+        const uint32_t c = (uint32_t)(i - row * pieces) * 16;
         const int8_t* s = p.src + row * p.src_ld + c;
         u32x4 v = {0, 0, 0, 0};
         if (c + 16 <= p.cols) {
@@ -149,8 +149,9 @@ __device__ __forceinline__ void eight(const void* src, uint64_t ld, uint32_t row
 template <int DT> __device__ __forceinline__ void pack_rows(const PackGradient& p, uint64_t id) {
     constexpr int TERMS = DT == Q8_F32 ? 3 : 1;
     const uint32_t pieces = p.cp / 8;
-    const uint64_t row = id / pieces;
-    const uint32_t c = (uint32_t)(id % pieces) * 8;
+    // (a division of 64 bits is a hundred instructions)
+    const uint64_t row = id >> 32 ? id / pieces : (uint32_t)id / pieces;
+    const uint32_t c = (uint32_t)(id - row * pieces) * 8;
     if (row >= p.rows) return;
     uint32_t v[TERMS][4] = {};
     if (c < p.cols) eight<DT, TERMS>(p.src, p.src_ld, (uint32_t)row, c, p.cols, p.scale, false, v);

@@ -9,9 +9,12 @@
 // elements.
 #include "q8_device.hpp"
 #include "q8_internal.hpp"
+#include "q8_plan.hpp"
 
 namespace q8 {
 namespace {
+
+template <int V> struct Int { static constexpr int value = V; };
 
 // Work-groups that a launch has at most; they take their rows in turn.
 constexpr uint32_t kMostGroups = 1u << 20;
@@ -37,31 +40,32 @@ __device__ __forceinline__ void row_sum_max(float& f, uint32_t& u, float (&redf)
     }
 }
 
-// q_j = rint(n_j / s), n_j = u_j rstd, s = max|n| / 127 and at least 2^-126.  The
-// largest |u| of the row gives s without a second sum over it: n differs from u by a
-// factor of the row.  One multiplication by 1 / s for each value: at most
-// 2^126, so it does not overflow.
+// q_j = rint(n_j / s), n_j = u_j rstd, s = max|n| / 127 and at least 2^-126.  rstd is a factor of the row,
+// so q_j = rint(u_j 127 / max|u|): the largest |u| gives the scale without a second sum over the row, and
+// the quotient rounds twice, not four times.  It is taken in two factors where one would leave FP32's range:
+// rows below 2^-118, and rows whose scale is the least one.
 struct Scale {
-    float s, inv;
+    float s, f1, f2;
     bool ok;
 };
-__device__ __forceinline__ Scale scale_of(uint32_t top, float rstd) {
+__device__ __forceinline__ Scale scale_of(uint32_t top_bits, float rstd) {
     Scale r;
-    const float most = __builtin_bit_cast(float, top) * rstd / 127.0f;
+    const float top = __builtin_bit_cast(float, top_bits), most = top * rstd / 127.0f;
     r.ok = most < __builtin_huge_valf();     // false for infinities and NaN
-    r.s = most > 0x1p-126f ? most : 0x1p-126f;
-    r.inv = 1.0f / r.s;
-    if (!r.ok) r.s = __builtin_nanf("");
+    const bool least = !(most > 0x1p-126f), tiny = top < 0x1p-118f;
+    r.s = !r.ok ? __builtin_nanf("") : least ? 0x1p-126f : most;
+    r.f1 = least ? rstd : tiny ? 0x1p60f : 127.0f / top;
+    r.f2 = least ? 0x1p126f : tiny ? 127.0f / (top * 0x1p60f) : 1.0f;
     return r;
 }
-__device__ __forceinline__ uint32_t to8(float n, const Scale& r) {
-    const float q = __builtin_rintf(n * r.inv);
+__device__ __forceinline__ uint32_t to8(float u, const Scale& r) {
+    const float q = __builtin_rintf(u * r.f1 * r.f2);
     return r.ok ? (uint32_t)(int)__builtin_amdgcn_fmed3f(q, -127.0f, 127.0f) & 0xffu : 0u;
 }
-__device__ __forceinline__ void put8(int8_t* row, uint32_t c, uint32_t cols, const float (&n)[8], const Scale& r) {
+__device__ __forceinline__ void put8(int8_t* row, uint32_t c, uint32_t cols, const float (&u)[8], const Scale& r) {
     uint32_t q[8];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) q[e] = to8(n[e], r);
+    for (int e = 0; e < 8; ++e) q[e] = to8(u[e], r);
     if (cols - c >= 8) {
         *reinterpret_cast<u32x2_at1*>(row + c) =
             u32x2{q[0] | q[1] << 8 | q[2] << 16 | q[3] << 24, q[4] | q[5] << 8 | q[6] << 16 | q[7] << 24};
@@ -153,18 +157,11 @@ __global__ void __launch_bounds__(G < 256 ? 256 : G) quantize_kernel(const Quant
             if (NORM && p.rstd) p.rstd[row] = rstd;
         }
         int8_t* q = p.q + row * p.ldq;
-        auto last = [&](uint32_t c, float (&n)[8]) __attribute__((always_inline)) {
-            if constexpr (NORM) {
-#pragma unroll
-                for (int e = 0; e < 8; ++e) n[e] *= rstd;
-            }
-            put8(q, c, p.cols, n, s);
-        };
         if constexpr (R > 0) {
 #pragma unroll
             for (int i = 0; i < R; ++i) {
                 const uint32_t c = (i * G + lane) * 8;
-                if (on && c < p.cols) last(c, v[i]);
+                if (on && c < p.cols) put8(q, c, p.cols, v[i], s);
             }
         } else {
             for (uint32_t i = 0; i < pieces; ++i) {
@@ -173,7 +170,7 @@ __global__ void __launch_bounds__(G < 256 ? 256 : G) quantize_kernel(const Quant
                 if (hid) load_part<DT>(hid, c, p.cols, v[0]);   // x may be gone: hidden may be x itself
                 else first(c, v[0]);
                 weigh(c, v[0]);
-                last(c, v[0]);
+                put8(q, c, p.cols, v[0], s);
             }
         }
     }
@@ -303,22 +300,23 @@ __global__ void __launch_bounds__(G) norm_backward_kernel(const NormBackward p) 
     }
 }
 
-// dgain_j = the parts' sums in part order: 64 columns a work-group, 16 slices of
-// parts that meet in LDS.
+// dgain_j = the parts' sums in part order: 32 columns a work-group, 32 slices of parts that meet in
+// LDS, so that few columns still reach many CUs (512 x 999: 64 columns and 16 slices 6.8 us).
 __global__ void __launch_bounds__(1024) column_sum_kernel(const float* partial, float* dgain, uint32_t parts, uint32_t cols) {
-    __shared__ float red[16][64];
-    const uint32_t c = blockIdx.x * 64 + threadIdx.x % 64, slice = threadIdx.x / 64;
-    const uint32_t per = (parts + 15) / 16, end = min(parts, (slice + 1) * per);
+    __shared__ float red[32][33];
+    const uint32_t lane = threadIdx.x % 32, slice = threadIdx.x / 32, c = blockIdx.x * 32 + lane;
+    const uint32_t per = (parts + 31) / 32, end = min(parts, (slice + 1) * per);
     float s = 0.0f;
     if (c < cols) {
-#pragma unroll 8
+#pragma unroll 16
         for (uint32_t i = slice * per; i < end; ++i) s += partial[(uint64_t)i * cols + c];
     }
-    red[slice][threadIdx.x % 64] = s;
+    red[slice][lane] = s;
     __syncthreads();
     if (slice == 0 && c < cols) {
+        s = red[0][lane];
 #pragma unroll
-        for (int i = 1; i < 16; ++i) s += red[i][threadIdx.x];
+        for (int i = 1; i < 32; ++i) s += red[i][lane];
         dgain[c] = s;
     }
 }
@@ -334,17 +332,28 @@ uint32_t groups_for(uint64_t rows, uint32_t rows_per_group) {
     return (uint32_t)(g < kMostGroups ? g : kMostGroups);
 }
 
+// The threads of a row and their pieces of eight values: the least G * R that holds the row, and
+// of those the most threads.  (16384 rows, F16, G x R: 4096 columns 512 x 1 85.7 us, 256 x 2 91.7, 1024 x
+// 1 127; 8192 columns 1024 x 1 175 us, 5.4 TB/s, 256 x 4 189.  1000 x 4097: 256 x 3 8.9 us, 1024 x 1 9.9.
+// 8192 x 11008: 512 x 3 133 us, 1024 x 2 175.)
 template <int DT, bool NORM> hipError_t quantize_any(const Quantize& p, hipStream_t s) {
-    // the fewest threads that hold a row in one piece each, then more pieces
-    const uint32_t c = p.cols;
-    if (c <= 512) return launch(quantize_kernel<DT, NORM, 64, 1>, groups_for(p.rows, 4), 256, p, s);
-    if (c <= 1024) return launch(quantize_kernel<DT, NORM, 128, 1>, groups_for(p.rows, 2), 256, p, s);
-    if (c <= 2048) return launch(quantize_kernel<DT, NORM, 256, 1>, groups_for(p.rows, 1), 256, p, s);
-    if (c <= 4096) return launch(quantize_kernel<DT, NORM, 512, 1>, groups_for(p.rows, 1), 512, p, s);
-    if (c <= 8192) return launch(quantize_kernel<DT, NORM, 1024, 1>, groups_for(p.rows, 1), 1024, p, s);
-    if (c <= 16384) return launch(quantize_kernel<DT, NORM, 1024, 2>, groups_for(p.rows, 1), 1024, p, s);
-    if (c <= 32768) return launch(quantize_kernel<DT, NORM, 1024, 4>, groups_for(p.rows, 1), 1024, p, s);
-    return launch(quantize_kernel<DT, NORM, 1024, 0>, groups_for(p.rows, 1), 1024, p, s);
+    const uint32_t pieces = (uint32_t)ceil_div(p.cols, 8);
+    auto on = [&](auto g, auto r) {
+        constexpr int G = decltype(g)::value, R = decltype(r)::value;
+        return launch(quantize_kernel<DT, NORM, G, R>, groups_for(p.rows, G < 256 ? 256 / G : 1), G < 256 ? 256 : G, p, s);
+    };
+    if (pieces <= 64) return on(Int<64>{}, Int<1>{});
+    if (pieces <= 128) return on(Int<128>{}, Int<1>{});
+    if (pieces <= 192) return on(Int<64>{}, Int<3>{});
+    if (pieces <= 256) return on(Int<256>{}, Int<1>{});
+    if (pieces <= 384) return on(Int<128>{}, Int<3>{});
+    if (pieces <= 512) return on(Int<512>{}, Int<1>{});
+    if (pieces <= 768) return on(Int<256>{}, Int<3>{});
+    if (pieces <= 1024) return on(Int<1024>{}, Int<1>{});
+    if (pieces <= 1536) return on(Int<512>{}, Int<3>{});
+    if (pieces <= 2048) return on(Int<1024>{}, Int<2>{});
+    if (pieces <= 4096) return on(Int<1024>{}, Int<4>{});
+    return on(Int<1024>{}, Int<0>{});
 }
 
 template <int DT> hipError_t dequantize_any(const Dequantize& p, hipStream_t s) {
@@ -352,24 +361,39 @@ template <int DT> hipError_t dequantize_any(const Dequantize& p, hipStream_t s) 
     return launch(dequantize_kernel<DT, 256>, groups_for(p.rows, 1), 256, p, s);
 }
 
+// As for quantize_any.
+uint32_t backward_threads(uint32_t cols) {
+    const uint32_t pieces = (uint32_t)ceil_div(cols, 8);
+    return pieces <= 64 ? 64 : pieces <= 128 ? 128 : pieces <= 192 ? 64 : pieces <= 256 ? 256 : pieces <= 384 ? 128 :
+           pieces <= 512 ? 512 : pieces <= 768 ? 256 : 1024;
+}
 template <int DT> hipError_t backward_any(const NormBackward& p, hipStream_t s) {
-    const uint32_t c = p.cols;
-    if (c <= 512) return launch(norm_backward_kernel<DT, 64, 1>, p.parts, 64, p, s);
-    if (c <= 1024) return launch(norm_backward_kernel<DT, 128, 1>, p.parts, 128, p, s);
-    if (c <= 2048) return launch(norm_backward_kernel<DT, 256, 1>, p.parts, 256, p, s);
-    if (c <= 4096) return launch(norm_backward_kernel<DT, 512, 1>, p.parts, 512, p, s);
-    if (c <= 8192) return launch(norm_backward_kernel<DT, 1024, 1>, p.parts, 1024, p, s);
-    if (c <= 16384) return launch(norm_backward_kernel<DT, 1024, 2>, p.parts, 1024, p, s);
-    return launch(norm_backward_kernel<DT, 1024, 0>, p.parts, 1024, p, s);
+    const uint32_t pieces = (uint32_t)ceil_div(p.cols, 8);
+    auto on = [&](auto g, auto r) {
+        constexpr int G = decltype(g)::value, R = decltype(r)::value;
+        return launch(norm_backward_kernel<DT, G, R>, p.parts, G, p, s);
+    };
+    if (pieces <= 64) return on(Int<64>{}, Int<1>{});
+    if (pieces <= 128) return on(Int<128>{}, Int<1>{});
+    if (pieces <= 192) return on(Int<64>{}, Int<3>{});
+    if (pieces <= 256) return on(Int<256>{}, Int<1>{});
+    if (pieces <= 384) return on(Int<128>{}, Int<3>{});
+    if (pieces <= 512) return on(Int<512>{}, Int<1>{});
+    if (pieces <= 768) return on(Int<256>{}, Int<3>{});
+    if (pieces <= 1024) return on(Int<1024>{}, Int<1>{});
+    if (pieces <= 2048) return on(Int<1024>{}, Int<2>{});
+    return on(Int<1024>{}, Int<0>{});
 }
 
 }  // namespace
 
 uint32_t norm_backward_parts(uint32_t rows, uint32_t cols) {
-    // as many work-groups as are resident at once, 2048 threads a CU
-    const uint32_t threads = cols <= 512 ? 64 : cols <= 1024 ? 128 : cols <= 2048 ? 256 : cols <= 4096 ? 512 : 1024;
-    const uint32_t most = 256u * 2048u / threads;
-    const uint32_t parts = most < 1024u ? most : 1024u;
+    // as many work-groups as are resident at once, 2048 threads a CU, up to 1024, but two rows each
+    // where there are 512 of those: every range is written, read and added once more
+    const uint32_t resident = kComputeUnits * 2048u / backward_threads(cols);
+    uint32_t parts = resident < 1024u ? resident : 1024u;
+    const uint32_t two = (rows + 1) / 2 < 512u ? 512u : (rows + 1) / 2;
+    if (parts > two) parts = two;
     return rows < parts ? rows : parts;
 }
 
@@ -396,7 +420,7 @@ hipError_t launch_norm_backward(int dtype, const NormBackward& p, hipStream_t s)
     float* dgain = p.dgain;
     uint32_t parts = p.parts, cols = p.cols;
     void* args[] = {&partial, &dgain, &parts, &cols};
-    return hipLaunchKernel(reinterpret_cast<const void*>(&column_sum_kernel), dim3((cols + 63) / 64), dim3(1024), args, 0, s);
+    return hipLaunchKernel(reinterpret_cast<const void*>(&column_sum_kernel), dim3((cols + 31) / 32), dim3(1024), args, 0, s);
 }
 
 }  // namespace q8
