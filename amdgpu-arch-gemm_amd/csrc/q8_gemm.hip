@@ -12,40 +12,37 @@
 namespace q8 {
 namespace {
 
-typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
-typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
-
 constexpr int BUFFER_RSRC_WORD3 = 0x00020000;
 constexpr int XCDS = 8;
 constexpr uint32_t NOWHERE = 0x80000000u;    // an offset past every descriptor's end: loads give 0
 constexpr int KB = kTileBytes;
 
+// The matrix instructions: `in_place` keeps a sum in its registers (the compiler else copies
+// between the two halves of the register file, up to an instruction for each of them), and its
+// user waits for the results.
 template <int E> struct Atom;
 template <> struct Atom<E_I8> {
     typedef i32x4 Acc;
     static __device__ __forceinline__ void mfma(u32x4 a, u32x4 b, Acc& c) {
         c = __builtin_amdgcn_mfma_i32_16x16x64_i8(__builtin_bit_cast(i32x4, a), __builtin_bit_cast(i32x4, b), c, 0, 0, 0);
     }
-    static __device__ __forceinline__ void mfma_agpr(u32x4 a, u32x4 b, Acc& c) {
-        asm("v_mfma_i32_16x16x64_i8 %0, %1, %2, %0" : "+a"(c) : "v"(a), "v"(b));
+    template <bool AGPR> static __device__ __forceinline__ void in_place(u32x4 a, u32x4 b, Acc& c) {
+        if constexpr (AGPR) asm("v_mfma_i32_16x16x64_i8 %0, %1, %2, %0" : "+a"(c) : "v"(a), "v"(b));
+        else asm("v_mfma_i32_16x16x64_i8 %0, %1, %2, %0" : "+v"(c) : "v"(a), "v"(b));
     }
 };
 template <> struct Atom<E_F16> {
     typedef f32x4 Acc;
-    static __device__ __forceinline__ void mfma(u32x4 a, u32x4 b, Acc& c) {
-        c = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
-    }
-    static __device__ __forceinline__ void mfma_agpr(u32x4 a, u32x4 b, Acc& c) {
-        asm("v_mfma_f32_16x16x32_f16 %0, %1, %2, %0" : "+a"(c) : "v"(a), "v"(b));
+    template <bool AGPR> static __device__ __forceinline__ void in_place(u32x4 a, u32x4 b, Acc& c) {
+        if constexpr (AGPR) asm("v_mfma_f32_16x16x32_f16 %0, %1, %2, %0" : "+a"(c) : "v"(a), "v"(b));
+        else asm("v_mfma_f32_16x16x32_f16 %0, %1, %2, %0" : "+v"(c) : "v"(a), "v"(b));
     }
 };
 template <> struct Atom<E_BF16> {
     typedef f32x4 Acc;
-    static __device__ __forceinline__ void mfma(u32x4 a, u32x4 b, Acc& c) {
-        c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
-    }
-    static __device__ __forceinline__ void mfma_agpr(u32x4 a, u32x4 b, Acc& c) {
-        asm("v_mfma_f32_16x16x32_bf16 %0, %1, %2, %0" : "+a"(c) : "v"(a), "v"(b));
+    template <bool AGPR> static __device__ __forceinline__ void in_place(u32x4 a, u32x4 b, Acc& c) {
+        if constexpr (AGPR) asm("v_mfma_f32_16x16x32_bf16 %0, %1, %2, %0" : "+a"(c) : "v"(a), "v"(b));
+        else asm("v_mfma_f32_16x16x32_bf16 %0, %1, %2, %0" : "+v"(c) : "v"(a), "v"(b));
     }
 };
 
@@ -201,8 +198,7 @@ __global__ void __launch_bounds__(256, T == 4 ? 2 : 1) product_kernel(const Prod
                 const int x = i * TN + j;
                 if (x % GAP == 0 && x / GAP < TM + TN) read(next, buf, s, x / GAP);
                 if (decltype(loads)::value && x % EVERY == EVERY - 1) load(x / EVERY);
-                if constexpr (T == 8) A::mfma_agpr(f.b[j], f.a[i], acc[i][j]);
-                else A::mfma(f.b[j], f.a[i], acc[i][j]);
+                A::template in_place<T == 8>(f.b[j], f.a[i], acc[i][j]);
                 __builtin_amdgcn_sched_barrier(0);
             }
     };
@@ -239,6 +235,7 @@ __global__ void __launch_bounds__(256, T == 4 ? 2 : 1) product_kernel(const Prod
     // A sum, read no earlier than here: not before the wait above, and not all of them at once.
     auto sum = [&](int i, int j) __attribute__((always_inline)) {
         if constexpr (T == 8) asm volatile("" : "+a"(acc[i][j]));
+        else asm volatile("" : "+v"(acc[i][j]));
         return acc[i][j];
     };
 

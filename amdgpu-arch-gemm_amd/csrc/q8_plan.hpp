@@ -36,20 +36,18 @@ constexpr uint64_t div_up(uint64_t a, uint64_t b) { return (a + b - 1) / b; }
 // back to back: a K tile's time and a fixed one for each round of work-groups.  The large
 // tiles take 1.47 us a K tile whether one or all CUs have one (4096^3 in 8-bit integers: 59
 // us).  Of the small ones, a CU with two takes 1.0 us for a K tile of both; one alone waits for
-// its loads, 0.57 us.  Three buffers make that 0.36 on `spread` rows, those laid out an odd number
-// of lines apart (2048^3 in BF16: 24.8 -> 18.5 us; 1024^3, 8 K tiles: 7.7 -> 10.3, as launches
-// overlap less); rows 4096 bytes apart meet in few memory channels, and it stays (256 x
-// 4096 x 4096 in 8-bit integers: 23.5 against 25.6).
-inline double product_time(int kind, bool spread, uint64_t groups, uint64_t tiles_k) {
+// its loads, 0.57 us, and three buffers make that 0.36 (16384 x 128 x 4096 in 8-bit integers: 25.3 ->
+// 17.8 us, 2048^3 in BF16: 24.8 -> 18.5; 1024^3, 8 K tiles: 8.0 -> 10.5, as launches overlap less).
+inline double product_time(int kind, uint64_t groups, uint64_t tiles_k) {
     const double k = (double)tiles_k;
     if (kind == K_LARGE) return (double)div_up(groups, kComputeUnits) * (1.47 * k + 10.0);
-    if (kind == K_SMALL_DEEP) return (double)div_up(groups, kComputeUnits) * ((spread ? 0.36 : 0.57) * k + 7.0);
+    if (kind == K_SMALL_DEEP) return (double)div_up(groups, kComputeUnits) * (0.36 * k + 7.0);
     const uint64_t slots = 2 * kComputeUnits, rest = groups % slots;
     return (double)(groups / slots) * (1.0 * k + 6.0) + (!rest ? 0.0 : rest <= kComputeUnits ? 0.57 * k + 4.5 : 1.0 * k + 6.0);
 }
 
 // m x n outputs over kb bytes of the summed index.
-inline ProductPlan plan_product(uint64_t m, uint64_t n, uint64_t kb, bool spread) {
+inline ProductPlan plan_product(uint64_t m, uint64_t n, uint64_t kb) {
     ProductPlan best;
     double least = 1e300;
     const uint64_t tiles_k = div_up(kb ? kb : 1, kTileBytes);
@@ -61,7 +59,7 @@ inline ProductPlan plan_product(uint64_t m, uint64_t n, uint64_t kb, bool spread
             if (s > 1 && (tiles * s > 2 * kComputeUnits || tiles_k / s < 4)) break;
             // the ranges' sums: written, read and finished by another kernel
             const double join = s > 1 ? 3.0 + (s + 1.0) * (double)m * (double)n * 4.0 / 3e6 : 0.0;
-            const double time = product_time(kind, spread, tiles * s, div_up(tiles_k, s)) + join;
+            const double time = product_time(kind, tiles * s, div_up(tiles_k, s)) + join;
             if (time < least * 0.999) {
                 least = time;
                 best.kind = kind;

@@ -140,6 +140,7 @@ int take_workspace(q8_handle* h, size_t bytes) {
     return SGEMM_OK;
 }
 
+uint64_t round_up(uint64_t x, uint64_t to) { return (x + to - 1) / to * to; }
 size_t piece(size_t bytes) { return (bytes + 255) & ~(size_t)255; }
 
 // A call's parts of the workspace, one after the other.
@@ -150,8 +151,6 @@ struct Layout {
         total += piece(bytes);
     }
 };
-
-uint64_t round_up(uint64_t x, uint64_t to) { return (x + to - 1) / to * to; }
 
 struct Grad {
     uint64_t cp;        // values of the summed index in a laid-out row
@@ -169,10 +168,11 @@ int plan_grad(int dtype, uint64_t rows, uint64_t cols, uint64_t sum, bool copy_a
     if (g.kb > kMaxRowBytes)
         return fail(SGEMM_E_SHAPE, "a sum over %llu products is too long: at most %llu", (unsigned long long)sum,
                     (unsigned long long)(kMaxRowBytes / (2 * g.terms)));
-    // an odd number of lines: rows of a power of two apart meet in few memory channels
-    g.pitch = (g.kb / 128 | 1) * 128;
-    if (g.pitch < g.kb) g.pitch += 256;
-    g.plan = plan_product(rows, cols, g.kb, true);
+    // whole lines, and not a multiple of 4096 bytes (F16, 4096 x 4096 x 16384: 396 us as it is, 386 with 512
+    // bytes more; 1024 x 1024 x 16384 in four ranges: 46 and 47, but 60 with 128)
+    g.pitch = round_up(g.kb, 128);
+    if (g.pitch % 4096 == 0) g.pitch += 512;
+    g.plan = plan_product(rows, cols, g.kb);
     g.at = Layout();
     if (copy_a || dtype == Q8_F32) g.at.add(g.at.a, rows * g.pitch);
     g.at.add(g.at.b, cols * g.pitch);
@@ -199,7 +199,7 @@ struct GemmPlan {
 GemmPlan plan_gemm(uint64_t m, uint64_t n, uint64_t k, bool copy_a, bool copy_b) {
     GemmPlan g;
     g.ldc = round_up(k, 16);
-    g.plan = plan_product(m, n, k, false);
+    g.plan = plan_product(m, n, k);
     g.direct = m <= kFewTokens || direct_for_many(m, n, k, g.plan.time, (int)copy_a + (int)copy_b,
                                                   (copy_a ? m * g.ldc : 0) + (copy_b ? n * g.ldc : 0));
     if (g.direct) return g;
