@@ -51,12 +51,8 @@ template <bool HALF> __device__ __forceinline__ uint32_t pair16(float x, float y
 
 // q: rows (summed index) x cols; dst: cols rows of cp (times terms).  W = 16 bytes a lane, or 4 where
 // that leaves CUs without waves.
-template <bool HALF, int W>
-__device__ __forceinline__ void pack_weights(const PackWeights& p, uint32_t wave_id, float factor) {
-    const uint32_t tr = (p.cp + 63) / 64;
-    const uint32_t lane = threadIdx.x & 63;
-    const uint32_t r = wave_id % tr * 64 + lane % 8 * 8, c = wave_id / tr * (8 * W) + lane / 8 * W;
-    if (r >= p.cp || c >= p.cols) return;
+template <bool HALF, int W, bool INSIDE>
+__device__ __forceinline__ void pack_piece(const PackWeights& p, uint32_t r, uint32_t c, float factor) {
     uint32_t in[8][W / 4];
     float s[8];
 #pragma unroll
@@ -64,9 +60,9 @@ __device__ __forceinline__ void pack_weights(const PackWeights& p, uint32_t wave
 #pragma unroll
         for (int e = 0; e < W / 4; ++e) in[k][e] = 0;
         s[k] = 0.0f;
-        if (r + k < p.rows) {
+        if (INSIDE || r + k < p.rows) {
             const int8_t* src = p.q + (uint64_t)(r + k) * p.ldq + c;
-            if (c + W <= p.cols) {
+            if (INSIDE || c + W <= p.cols) {
                 if constexpr (W == 16) {
                     const u32x4 w = *reinterpret_cast<const u32x4_at1*>(src);
 #pragma unroll
@@ -79,21 +75,32 @@ __device__ __forceinline__ void pack_weights(const PackWeights& p, uint32_t wave
                 for (int e = 0; e < W; ++e)
                     if (c + e < p.cols) in[k][e / 4] |= (uint32_t)(uint8_t)src[e] << (8 * (e % 4));
             }
-            s[k] = p.scale ? p.scale[r + k] * factor : 1.0f;
+            s[k] = p.scale ? p.scale[r + k] : 1.0f;
         }
     }
     uint16_t* dst = (uint16_t*)p.dst + (uint64_t)c * p.dst_ld + r;
 #pragma unroll
     for (int e = 0; e < W; ++e) {
-        if (c + e >= p.cols) break;
+        if (!INSIDE && c + e >= p.cols) break;
         float v[8];
         // a scale that is not a number takes its whole row along, zeros too
 #pragma unroll
-        for (int k = 0; k < 8; ++k) v[k] = (float)(int8_t)(in[k][e / 4] >> (8 * (e % 4))) * s[k];
+        for (int k = 0; k < 8; ++k) v[k] = (float)(int8_t)(in[k][e / 4] >> (8 * (e % 4))) * (s[k] * factor);
         const u32x4 w = {pair16<HALF>(v[0], v[1]), pair16<HALF>(v[2], v[3]), pair16<HALF>(v[4], v[5]), pair16<HALF>(v[6], v[7])};
         uint16_t* d = dst + (uint64_t)e * p.dst_ld;
-        for (uint32_t q = 0; q < p.terms; ++q) *reinterpret_cast<u32x4*>(d + (uint64_t)q * p.cp) = w;
+        *reinterpret_cast<u32x4*>(d) = w;
+        for (uint32_t q = 1; q < p.terms; ++q) *reinterpret_cast<u32x4*>(d + (uint64_t)q * p.cp) = w;
     }
+}
+template <bool HALF, int W>
+__device__ __forceinline__ void pack_weights(const PackWeights& p, uint32_t wave_id, float factor) {
+    const uint32_t tr = (p.cp + 63) / 64;
+    const uint32_t lane = threadIdx.x & 63;
+    const uint32_t r0 = wave_id % tr * 64, c0 = wave_id / tr * (8 * W);
+    const uint32_t r = r0 + lane % 8 * 8, c = c0 + lane / 8 * W;
+    // whole pieces without a condition for each load
+    if (r0 + 64 <= p.rows && c0 + 8 * W <= p.cols) pack_piece<HALF, W, true>(p, r, c, factor);
+    else if (r < p.cp && c < p.cols) pack_piece<HALF, W, false>(p, r, c, factor);
 }
 
 // x = hi + mid + lo in BF16: both differences are exact, and three terms of 8 bits
@@ -169,9 +176,19 @@ template <int DT> __device__ __forceinline__ void pack_turned(const PackGradient
     const uint32_t k0 = wave_id % tk * 64 + lane % 8 * 8, r = wave_id / tk * 64 + lane / 8 * 8;
     if (k0 >= p.cp || r >= p.rows) return;
     uint32_t in[8][TERMS][4] = {};
+    const uint32_t whole = wave_id % tk * 64 + 64;
+    if (DT != Q8_F32 && whole <= p.cols && wave_id / tk * 64 + 64 <= p.rows) {
 #pragma unroll
-    for (int k = 0; k < 8; ++k)
-        if (k0 + k < p.cols) eight<DT, TERMS>(p.src, p.src_ld, k0 + k, r, p.rows, p.scale, true, in[k]);
+        for (int k = 0; k < 8; ++k) {   // whole pieces without a condition for each load
+            const u32x4 w = *reinterpret_cast<const u32x4_at2*>((const uint16_t*)p.src + (uint64_t)(k0 + k) * p.src_ld + r);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) in[k][0][e] = w[e];
+        }
+    } else {
+#pragma unroll
+        for (int k = 0; k < 8; ++k)
+            if (k0 + k < p.cols) eight<DT, TERMS>(p.src, p.src_ld, k0 + k, r, p.rows, p.scale, true, in[k]);
+    }
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
         if (r + e >= p.rows) break;
