@@ -97,7 +97,8 @@ inline Direct direct_kind(uint64_t m, uint64_t n, uint64_t k) {
 // Whether more tokens run on it too: a small product, which the tile kernels would spend on
 // whole tiles and on copies of rows that are not theirs (`copies` launches, `copy_bytes` in all).
 inline bool direct_for_many(uint64_t m, uint64_t n, uint64_t k, double tile_time, int copies, uint64_t copy_bytes) {
-    if (m > (1u << 20)) return false;   // a grid's second dimension ends at 65535
+    // a grid's second dimension ends at 65535, all of it at 2^32 work-items
+    if (m > (1u << 20) || div_up(m, 32) * div_up(n, 16) > (1u << 22)) return false;
     const uint64_t t = div_up(m, 16) * div_up(n, 16);
     const double rows = t <= kComputeUnits ? 32.0 * (double)t : 48.0 * (double)(div_up(m, 32) * div_up(n, 16));
     const double direct = 3.8 + rows * (double)k / 7e6;     // each work-group's rows, out of L2
