@@ -30,23 +30,34 @@ template <> struct Type<Q8_F32> {
     static __device__ __forceinline__ float get(const T* p) { return *p; }
     static __device__ __forceinline__ void put(T* p, float x) { *p = x; }
     static __device__ __forceinline__ float round(float x) { return x; }
-    static __device__ __forceinline__ void load8(const T* p, float (&v)[8]) {
-        const f32x4 a = *reinterpret_cast<const f32x4_at4*>(p), b = *reinterpret_cast<const f32x4_at4*>(p + 4);
+    // eight values as they are in memory, and spread out
+    struct Eight { f32x4 lo, hi; };
+    static __device__ __forceinline__ Eight get8(const T* p) {
+        return Eight{*reinterpret_cast<const f32x4_at4*>(p), *reinterpret_cast<const f32x4_at4*>(p + 4)};
+    }
+    static __device__ __forceinline__ void spread(const Eight& w, float (&v)[8]) {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) { v[e] = a[e]; v[4 + e] = b[e]; }
+        for (int e = 0; e < 4; ++e) { v[e] = w.lo[e]; v[4 + e] = w.hi[e]; }
     }
-    static __device__ __forceinline__ void store8(T* p, const float (&v)[8]) {
-        *reinterpret_cast<f32x4_at4*>(p) = f32x4{v[0], v[1], v[2], v[3]};
-        *reinterpret_cast<f32x4_at4*>(p + 4) = f32x4{v[4], v[5], v[6], v[7]};
+    static __device__ __forceinline__ void load8(const T* p, float (&v)[8]) { spread(get8(p), v); }
+    static __device__ __forceinline__ Eight eight(const float (&v)[8]) {
+        return Eight{f32x4{v[0], v[1], v[2], v[3]}, f32x4{v[4], v[5], v[6], v[7]}};
     }
+    static __device__ __forceinline__ void put8(T* p, const Eight& w) {
+        *reinterpret_cast<f32x4_at4*>(p) = w.lo;
+        *reinterpret_cast<f32x4_at4*>(p + 4) = w.hi;
+    }
+    static __device__ __forceinline__ void store8(T* p, const float (&v)[8]) { put8(p, eight(v)); }
 };
 template <> struct Type<Q8_F16> {
     typedef _Float16 T;
     static __device__ __forceinline__ float get(const T* p) { return (float)*p; }
     static __device__ __forceinline__ void put(T* p, float x) { *p = (T)x; }
     static __device__ __forceinline__ float round(float x) { return (float)(T)x; }
-    static __device__ __forceinline__ void load8(const T* p, float (&v)[8]) {
-        const u32x4 w = *reinterpret_cast<const u32x4_at2*>(p);
+    typedef u32x4 Eight;
+    static __device__ __forceinline__ Eight get8(const T* p) { return *reinterpret_cast<const u32x4_at2*>(p); }
+    static __device__ __forceinline__ void load8(const T* p, float (&v)[8]) { spread(get8(p), v); }
+    static __device__ __forceinline__ void spread(const Eight& w, float (&v)[8]) {
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
             const f16x2 h = __builtin_bit_cast(f16x2, (uint32_t)w[e]);
@@ -58,17 +69,21 @@ template <> struct Type<Q8_F16> {
         const f16x2 h = {(_Float16)x, (_Float16)y};
         return __builtin_bit_cast(uint32_t, h);
     }
-    static __device__ __forceinline__ void store8(T* p, const float (&v)[8]) {
-        *reinterpret_cast<u32x4_at2*>(p) = u32x4{pair(v[0], v[1]), pair(v[2], v[3]), pair(v[4], v[5]), pair(v[6], v[7])};
+    static __device__ __forceinline__ Eight eight(const float (&v)[8]) {
+        return u32x4{pair(v[0], v[1]), pair(v[2], v[3]), pair(v[4], v[5]), pair(v[6], v[7])};
     }
+    static __device__ __forceinline__ void put8(T* p, const Eight& w) { *reinterpret_cast<u32x4_at2*>(p) = w; }
+    static __device__ __forceinline__ void store8(T* p, const float (&v)[8]) { put8(p, eight(v)); }
 };
 template <> struct Type<Q8_BF16> {
     typedef __bf16 T;
     static __device__ __forceinline__ float get(const T* p) { return (float)*p; }
     static __device__ __forceinline__ void put(T* p, float x) { *p = (T)x; }
     static __device__ __forceinline__ float round(float x) { return (float)(T)x; }
-    static __device__ __forceinline__ void load8(const T* p, float (&v)[8]) {
-        const u32x4 w = *reinterpret_cast<const u32x4_at2*>(p);
+    typedef u32x4 Eight;
+    static __device__ __forceinline__ Eight get8(const T* p) { return *reinterpret_cast<const u32x4_at2*>(p); }
+    static __device__ __forceinline__ void load8(const T* p, float (&v)[8]) { spread(get8(p), v); }
+    static __device__ __forceinline__ void spread(const Eight& w, float (&v)[8]) {
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
             v[2 * e] = __builtin_bit_cast(float, (uint32_t)(w[e] << 16));
@@ -79,9 +94,11 @@ template <> struct Type<Q8_BF16> {
         const f32x2 v = {x, y};
         return __builtin_bit_cast(uint32_t, __builtin_convertvector(v, bf16x2));
     }
-    static __device__ __forceinline__ void store8(T* p, const float (&v)[8]) {
-        *reinterpret_cast<u32x4_at2*>(p) = u32x4{pair(v[0], v[1]), pair(v[2], v[3]), pair(v[4], v[5]), pair(v[6], v[7])};
+    static __device__ __forceinline__ Eight eight(const float (&v)[8]) {
+        return u32x4{pair(v[0], v[1]), pair(v[2], v[3]), pair(v[4], v[5]), pair(v[6], v[7])};
     }
+    static __device__ __forceinline__ void put8(T* p, const Eight& w) { *reinterpret_cast<u32x4_at2*>(p) = w; }
+    static __device__ __forceinline__ void store8(T* p, const float (&v)[8]) { put8(p, eight(v)); }
 };
 
 // Eight values of a row from column c; those past `cols` are 0 (c < cols).

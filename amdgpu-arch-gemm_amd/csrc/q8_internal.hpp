@@ -53,7 +53,7 @@ struct NormBackward {
     uint32_t lddn, ldh, lddr, lddx, rows, cols, parts;
 };
 // Row ranges that the gain's gradient is summed over first.
-Q8_INTERNAL uint32_t norm_backward_parts(uint32_t rows, uint32_t cols);
+Q8_INTERNAL uint32_t norm_backward_parts(uint32_t rows);
 Q8_INTERNAL hipError_t launch_norm_backward(int dtype, const NormBackward& p, hipStream_t stream);
 
 // What the matrix cores multiply.

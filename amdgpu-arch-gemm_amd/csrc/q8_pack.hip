@@ -27,6 +27,19 @@ __global__ void __launch_bounds__(256) copy_rows_kernel(const CopyRows p) {
         u32x4 v = {0, 0, 0, 0};
         if (c + 16 <= p.cols) {
             v = *reinterpret_cast<const u32x4_at1*>(s);
+        } else if (p.cols >= 16) {
+            // a last piece with the bytes before it, moved down
+            const uint32_t down = (c + 16 - p.cols) * 8;
+            const u32x4 w = *reinterpret_cast<const u32x4_at1*>(s - down / 8);
+            uint64_t lo = (uint64_t)w[1] << 32 | w[0], hi = (uint64_t)w[3] << 32 | w[2];
+            if (down >= 64) {
+                lo = hi >> (down - 64);
+                hi = 0;
+            } else {
+                lo = lo >> down | hi << (64 - down);
+                hi >>= down;
+            }
+            v = u32x4{(uint32_t)lo, (uint32_t)(lo >> 32), (uint32_t)hi, (uint32_t)(hi >> 32)};
         } else {
 #pragma unroll
             for (int e = 0; e < 16; ++e)
@@ -51,56 +64,51 @@ template <bool HALF> __device__ __forceinline__ uint32_t pair16(float x, float y
 
 // q: rows (summed index) x cols; dst: cols rows of cp (times terms).  W = 16 bytes a lane, or 4 where
 // that leaves CUs without waves.
-template <bool HALF, int W, bool INSIDE>
-__device__ __forceinline__ void pack_piece(const PackWeights& p, uint32_t r, uint32_t c, float factor) {
+// The last columns are taken with those before them, which are stored twice with the same
+// values: no load or store of a lane has a condition of its own.
+template <bool HALF, int W>
+__device__ __forceinline__ void pack_weights(const PackWeights& p, uint32_t wave_id, float factor) {
+    const uint32_t tr = (p.cp + 63) / 64;
+    const uint32_t lane = threadIdx.x & 63;
+    const uint32_t r = wave_id % tr * 64 + lane % 8 * 8;
+    uint32_t c = wave_id / tr * (8 * W) + lane / 8 * W;
+    if (r >= p.cp || c >= p.cols) return;
+    const bool narrow = p.cols < W;
+    if (!narrow && c + W > p.cols) c = p.cols - W;
     uint32_t in[8][W / 4];
     float s[8];
 #pragma unroll
     for (int k = 0; k < 8; ++k) {
+        const uint32_t row = min(r + k, p.rows - 1);
+        const int8_t* src = p.q + (uint64_t)row * p.ldq + c;
+        if (narrow) {
 #pragma unroll
-        for (int e = 0; e < W / 4; ++e) in[k][e] = 0;
-        s[k] = 0.0f;
-        if (INSIDE || r + k < p.rows) {
-            const int8_t* src = p.q + (uint64_t)(r + k) * p.ldq + c;
-            if (INSIDE || c + W <= p.cols) {
-                if constexpr (W == 16) {
-                    const u32x4 w = *reinterpret_cast<const u32x4_at1*>(src);
+            for (int e = 0; e < W / 4; ++e) in[k][e] = 0;
+            for (uint32_t e = 0; e < p.cols; ++e) in[k][e / 4] |= (uint32_t)(uint8_t)src[e] << (8 * (e % 4));
+        } else if constexpr (W == 16) {
+            const u32x4 w = *reinterpret_cast<const u32x4_at1*>(src);
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) in[k][e] = w[e];
-                } else {
-                    in[k][0] = *reinterpret_cast<const u32_at1*>(src);
-                }
-            } else {
-#pragma unroll
-                for (int e = 0; e < W; ++e)
-                    if (c + e < p.cols) in[k][e / 4] |= (uint32_t)(uint8_t)src[e] << (8 * (e % 4));
-            }
-            s[k] = p.scale ? p.scale[r + k] : 1.0f;
+            for (int e = 0; e < 4; ++e) in[k][e] = w[e];
+        } else {
+            in[k][0] = *reinterpret_cast<const u32_at1*>(src);
         }
+        s[k] = p.scale ? p.scale[row] : 1.0f;
     }
+#pragma unroll
+    for (int k = 0; k < 8; ++k) s[k] = r + k < p.rows ? s[k] * factor : 0.0f;
     uint16_t* dst = (uint16_t*)p.dst + (uint64_t)c * p.dst_ld + r;
 #pragma unroll
     for (int e = 0; e < W; ++e) {
-        if (!INSIDE && c + e >= p.cols) break;
+        if (narrow && (uint32_t)e >= p.cols) break;
         float v[8];
         // a scale that is not a number takes its whole row along, zeros too
 #pragma unroll
-        for (int k = 0; k < 8; ++k) v[k] = (float)(int8_t)(in[k][e / 4] >> (8 * (e % 4))) * (s[k] * factor);
+        for (int k = 0; k < 8; ++k) v[k] = (float)(int8_t)(in[k][e / 4] >> (8 * (e % 4))) * s[k];
         const u32x4 w = {pair16<HALF>(v[0], v[1]), pair16<HALF>(v[2], v[3]), pair16<HALF>(v[4], v[5]), pair16<HALF>(v[6], v[7])};
         uint16_t* d = dst + (uint64_t)e * p.dst_ld;
         *reinterpret_cast<u32x4*>(d) = w;
         for (uint32_t q = 1; q < p.terms; ++q) *reinterpret_cast<u32x4*>(d + (uint64_t)q * p.cp) = w;
     }
-}
-template <bool HALF, int W>
-__device__ __forceinline__ void pack_weights(const PackWeights& p, uint32_t wave_id, float factor) {
-    const uint32_t tr = (p.cp + 63) / 64;
-    const uint32_t lane = threadIdx.x & 63;
-    const uint32_t r0 = wave_id % tr * 64, c0 = wave_id / tr * (8 * W);
-    const uint32_t r = r0 + lane % 8 * 8, c = c0 + lane / 8 * W;
-    // whole pieces without a condition for each load
-    if (r0 + 64 <= p.rows && c0 + 8 * W <= p.cols) pack_piece<HALF, W, true>(p, r, c, factor);
-    else if (r < p.cp && c < p.cols) pack_piece<HALF, W, false>(p, r, c, factor);
 }
 
 // x = hi + mid + lo in BF16: both differences are exact, and three terms of 8 bits
@@ -138,10 +146,22 @@ __device__ __forceinline__ void eight(const void* src, uint64_t ld, uint32_t row
 #pragma unroll
             for (int e = 0; e < 4; ++e) out[q][e] = (uint32_t)b[2 * e][q] | (uint32_t)b[2 * e + 1][q] << 16;
     } else {
-        if (cols - c >= 8) {
-            const u32x4 w = *reinterpret_cast<const u32x4_at2*>(line + c);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) out[0][e] = w[e];
+        if (cols >= 8) {
+            // a last piece with the values before it, moved down
+            const uint32_t at = min(c, cols - 8), down = (c - at) * 16;
+            const u32x4 w = *reinterpret_cast<const u32x4_at2*>(line + at);
+            uint64_t lo = (uint64_t)w[1] << 32 | w[0], hi = (uint64_t)w[3] << 32 | w[2];
+            if (down >= 64) {
+                lo = hi >> (down - 64);
+                hi = 0;
+            } else if (down) {
+                lo = lo >> down | hi << (64 - down);
+                hi >>= down;
+            }
+            out[0][0] = (uint32_t)lo;
+            out[0][1] = (uint32_t)(lo >> 32);
+            out[0][2] = (uint32_t)hi;
+            out[0][3] = (uint32_t)(hi >> 32);
         } else {
 #pragma unroll
             for (int e = 0; e < 4; ++e) out[0][e] = 0;
@@ -173,22 +193,21 @@ template <int DT> __device__ __forceinline__ void pack_turned(const PackGradient
     constexpr int TERMS = DT == Q8_F32 ? 3 : 1;
     const uint32_t tk = (p.cp + 63) / 64;
     const uint32_t lane = threadIdx.x & 63;
-    const uint32_t k0 = wave_id % tk * 64 + lane % 8 * 8, r = wave_id / tk * 64 + lane / 8 * 8;
+    const uint32_t k0 = wave_id % tk * 64 + lane % 8 * 8;
+    uint32_t r = wave_id / tk * 64 + lane / 8 * 8;
     if (k0 >= p.cp || r >= p.rows) return;
-    uint32_t in[8][TERMS][4] = {};
-    const uint32_t whole = wave_id % tk * 64 + 64;
-    if (DT != Q8_F32 && whole <= p.cols && wave_id / tk * 64 + 64 <= p.rows) {
+    // the last columns with those before them, as pack_weights
+    if (p.rows >= 8) r = min(r, p.rows - 8);
+    uint32_t in[8][TERMS][4];
 #pragma unroll
-        for (int k = 0; k < 8; ++k) {   // whole pieces without a condition for each load
-            const u32x4 w = *reinterpret_cast<const u32x4_at2*>((const uint16_t*)p.src + (uint64_t)(k0 + k) * p.src_ld + r);
+    for (int k = 0; k < 8; ++k) eight<DT, TERMS>(p.src, p.src_ld, min(k0 + k, p.cols - 1), r, p.rows, p.scale, true, in[k]);
 #pragma unroll
-            for (int e = 0; e < 4; ++e) in[k][0][e] = w[e];
-        }
-    } else {
+    for (int k = 0; k < 8; ++k)
 #pragma unroll
-        for (int k = 0; k < 8; ++k)
-            if (k0 + k < p.cols) eight<DT, TERMS>(p.src, p.src_ld, k0 + k, r, p.rows, p.scale, true, in[k]);
-    }
+        for (int q = 0; q < TERMS; ++q)
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                if (k0 + k >= p.cols) in[k][q][e] = 0;
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
         if (r + e >= p.rows) break;
@@ -212,9 +231,13 @@ template <int DT> __device__ __forceinline__ void pack_turned(const PackGradient
 // work-group:
 template <int THREADS> __device__ __forceinline__ uint32_t largest(const float* scale, uint32_t count, uint32_t (&red)[THREADS / 64]) {
     uint32_t top = 0;
-    for (uint32_t i = threadIdx.x; i < count; i += THREADS) {
-        const uint32_t a = magnitude(scale[i]);
-        if (a < 0x7f800000u) top = top > a ? top : a;
+    for (uint32_t i = threadIdx.x; i < count; i += THREADS * 4) {
+        uint32_t a[4];      // four loads at once; the last one again past the end
+#pragma unroll
+        for (int k = 0; k < 4; ++k) a[k] = magnitude(scale[min(i + k * THREADS, count - 1)]);
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+            if (a[k] < 0x7f800000u) top = top > a[k] ? top : a[k];
     }
     float none = 0.0f;
     wave_sum_max(none, top);

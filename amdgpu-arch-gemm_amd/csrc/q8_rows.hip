@@ -5,11 +5,12 @@
 //
 // A row belongs to G threads, eight values each at a time, and stays in
 // registers between its sums and its stores.  Rows may start at any address (see
-// q8_device.hpp); only a row's last piece of fewer than eight values goes by
-// elements.
+// q8_device.hpp).  A row's last piece starts where the row has eight values left: those that the
+// piece before it has too count once in sums and are stored twice, the same, so that no access is
+// shorter than eight values (1000 x 999, F16: 6.3 -> 5.2 us).  Rows of fewer than eight values, or
+// of more than the registers hold, have kernels that go by elements at the end and read twice.
 #include "q8_device.hpp"
 #include "q8_internal.hpp"
-#include "q8_plan.hpp"
 
 namespace q8 {
 namespace {
@@ -62,90 +63,80 @@ __device__ __forceinline__ uint32_t to8(float u, const Scale& r) {
     const float q = __builtin_rintf(u * r.f1 * r.f2);
     return r.ok ? (uint32_t)(int)__builtin_amdgcn_fmed3f(q, -127.0f, 127.0f) & 0xffu : 0u;
 }
-__device__ __forceinline__ void put8(int8_t* row, uint32_t c, uint32_t cols, const float (&u)[8], const Scale& r) {
+// Piece i of a row for one of its G threads.
+struct Piece {
+    uint32_t c, twice;   // first column; so many of its values are the piece before's
+    bool on;
+};
+template <int G> __device__ __forceinline__ Piece piece_of(int i, uint32_t lane, uint32_t cols) {
+    const uint32_t c = (uint32_t)(i * G + (int)lane) * 8;
+    Piece p;
+    p.on = c < cols;
+    p.c = min(c, cols - 8);
+    p.twice = c - p.c;
+    return p;
+}
+__device__ __forceinline__ u32x2 bytes8(const float (&u)[8], const Scale& s) {
     uint32_t q[8];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) q[e] = to8(u[e], r);
-    if (cols - c >= 8) {
-        *reinterpret_cast<u32x2_at1*>(row + c) =
-            u32x2{q[0] | q[1] << 8 | q[2] << 16 | q[3] << 24, q[4] | q[5] << 8 | q[6] << 16 | q[7] << 24};
-    } else {
-#pragma unroll
-        for (int e = 0; e < 8; ++e)
-            if (c + e < cols) row[c + e] = (int8_t)q[e];
-    }
+    for (int e = 0; e < 8; ++e) q[e] = to8(u[e], s);
+    return u32x2{q[0] | q[1] << 8 | q[2] << 16 | q[3] << 24, q[4] | q[5] << 8 | q[6] << 16 | q[7] << 24};
 }
 
-// Quantisation (NORM == false) and the norm.  R: pieces of eight values that a
-// thread keeps; 0: rows longer than registers hold, read a second time.
+// Quantisation (NORM == false) and the norm, R pieces a thread.  hidden leaves after the sums: it
+// may be x or the residual, whose last values two threads read.
 template <int DT, bool NORM, int G, int R>
 __global__ void __launch_bounds__(G < 256 ? 256 : G) quantize_kernel(const Quantize p) {
-    constexpr int WG = G < 256 ? 256 : G, ROWS = WG / G, KEEP = R ? R : 1;
-    typedef typename Type<DT>::T T;
+    constexpr int WG = G < 256 ? 256 : G, ROWS = WG / G;
+    typedef Type<DT> Y;
+    typedef typename Y::T T;
     __shared__ float redf[2][WG / 64];
     __shared__ uint32_t redu[2][WG / 64];
-    const int group = threadIdx.x / G;
     const uint32_t lane = threadIdx.x % G;
-    const uint32_t pieces = R ? R : (p.cols + G * 8 - 1) / (G * 8);
+    const T* gain = (const T*)p.gain;
     int set = 0;
     for (uint64_t r0 = (uint64_t)blockIdx.x * ROWS; r0 < p.rows; r0 += (uint64_t)gridDim.x * ROWS, set ^= 1) {
-        const uint64_t row = r0 + group;
+        const uint64_t row = r0 + threadIdx.x / G;
         const bool on = row < p.rows;
         const T* x = (const T*)p.x + row * p.ldx;
         const T* res = NORM && p.residual ? (const T*)p.residual + row * p.ldr : nullptr;
         T* hid = NORM && p.hidden ? (T*)p.hidden + row * p.ldh : nullptr;
-        const T* gain = (const T*)p.gain;
-        float v[KEEP][8];
+        float v[R][8];
+        typename Y::Eight hold[NORM ? R : 1];
         float sum = 0.0f;
         uint32_t top = 0;
-        auto first = [&](uint32_t c, float (&v)[8]) __attribute__((always_inline)) {
-            load_part<DT>(x, c, p.cols, v);
-            if constexpr (NORM) {
-                if (res) {
-                    float w[8];
-                    load_part<DT>(res, c, p.cols, w);
+        // all loads of the row before its first sum
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) v[e] = Type<DT>::round(v[e] + w[e]);
+        for (int i = 0; i < R; ++i) {
+            const Piece c = piece_of<G>(i, lane, p.cols);
+            if (!on || !c.on) continue;
+            Y::load8(x + c.c, v[i]);
+            if (NORM && res) {
+                float w[8];
+                Y::load8(res + c.c, w);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) v[i][e] = Y::round(v[i][e] + w[e]);
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < R; ++i) {
+            const Piece c = piece_of<G>(i, lane, p.cols);
+            if (!on || !c.on) continue;
+            if constexpr (NORM) {
+                hold[i] = Y::eight(v[i]);
+                float g[8];
+                Y::load8(gain + c.c, g);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    const float h = (uint32_t)e < c.twice ? 0.0f : v[i][e];
+                    sum = __builtin_fmaf(h, h, sum);
+                    v[i][e] *= g[e];    // u
                 }
             }
-        };
-        auto weigh = [&](uint32_t c, float (&v)[8]) __attribute__((always_inline)) {   // u = hidden gain
-            if constexpr (NORM) {
-                float g[8];
-                load_part<DT>(gain, c, p.cols, g);
-#pragma unroll
-                for (int e = 0; e < 8; ++e) v[e] *= g[e];
-            }
-        };
-        auto measure = [&](uint32_t c, float (&v)[8]) __attribute__((always_inline)) {
-            if constexpr (NORM) {
-                if (hid) store_part<DT>(hid, c, p.cols, v);
-#pragma unroll
-                for (int e = 0; e < 8; ++e) sum = __builtin_fmaf(v[e], v[e], sum);
-            }
-            weigh(c, v);
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
-                const uint32_t a = magnitude(v[e]);
+                const uint32_t a = magnitude(v[i][e]);
                 top = top > a ? top : a;
-            }
-        };
-        if constexpr (R > 0) {
-            // all loads of the row before its first sum
-#pragma unroll
-            for (int i = 0; i < R; ++i) {
-                const uint32_t c = (i * G + lane) * 8;
-                if (on && c < p.cols) first(c, v[i]);
-            }
-#pragma unroll
-            for (int i = 0; i < R; ++i) {
-                const uint32_t c = (i * G + lane) * 8;
-                if (on && c < p.cols) measure(c, v[i]);
-            }
-        } else {
-            for (uint32_t i = 0; i < pieces; ++i) {
-                const uint32_t c = (i * G + lane) * 8;
-                if (on && c < p.cols) { first(c, v[0]); measure(c, v[0]); }
             }
         }
         row_sum_max<G, WG>(sum, top, redf, redu, set);
@@ -157,20 +148,88 @@ __global__ void __launch_bounds__(G < 256 ? 256 : G) quantize_kernel(const Quant
             if (NORM && p.rstd) p.rstd[row] = rstd;
         }
         int8_t* q = p.q + row * p.ldq;
-        if constexpr (R > 0) {
 #pragma unroll
-            for (int i = 0; i < R; ++i) {
-                const uint32_t c = (i * G + lane) * 8;
-                if (on && c < p.cols) put8(q, c, p.cols, v[i], s);
+        for (int i = 0; i < R; ++i) {
+            const Piece c = piece_of<G>(i, lane, p.cols);
+            if (!on || !c.on) continue;
+            if (NORM && hid) Y::put8(hid + c.c, hold[i]);
+            *reinterpret_cast<u32x2_at1*>(q + c.c) = bytes8(v[i], s);
+        }
+    }
+}
+
+// The same for rows of fewer than eight values and for rows longer than registers hold: each piece is
+// read a second time after the sums.
+template <int DT, bool NORM, int G>
+__global__ void __launch_bounds__(G < 256 ? 256 : G) quantize_any_kernel(const Quantize p) {
+    constexpr int WG = G < 256 ? 256 : G, ROWS = WG / G;
+    typedef typename Type<DT>::T T;
+    __shared__ float redf[2][WG / 64];
+    __shared__ uint32_t redu[2][WG / 64];
+    const uint32_t lane = threadIdx.x % G;
+    const T* gain = (const T*)p.gain;
+    int set = 0;
+    for (uint64_t r0 = (uint64_t)blockIdx.x * ROWS; r0 < p.rows; r0 += (uint64_t)gridDim.x * ROWS, set ^= 1) {
+        const uint64_t row = r0 + threadIdx.x / G;
+        const bool on = row < p.rows;
+        const T* x = (const T*)p.x + row * p.ldx;
+        const T* res = NORM && p.residual ? (const T*)p.residual + row * p.ldr : nullptr;
+        T* hid = NORM && p.hidden ? (T*)p.hidden + row * p.ldh : nullptr;
+        float sum = 0.0f;
+        uint32_t top = 0;
+        auto first = [&](uint32_t c, float (&v)[8]) __attribute__((always_inline)) {
+            load_part<DT>(x, c, p.cols, v);
+            if (NORM && res) {
+                float w[8];
+                load_part<DT>(res, c, p.cols, w);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) v[e] = Type<DT>::round(v[e] + w[e]);
             }
-        } else {
-            for (uint32_t i = 0; i < pieces; ++i) {
-                const uint32_t c = (i * G + lane) * 8;
-                if (!(on && c < p.cols)) continue;
-                if (hid) load_part<DT>(hid, c, p.cols, v[0]);   // x may be gone: hidden may be x itself
-                else first(c, v[0]);
-                weigh(c, v[0]);
-                put8(q, c, p.cols, v[0], s);
+        };
+        auto weigh = [&](uint32_t c, float (&v)[8]) __attribute__((always_inline)) {   // u = hidden gain
+            if constexpr (NORM) {
+                float g[8];
+                load_part<DT>(gain, c, p.cols, g);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) v[e] *= g[e];
+            }
+        };
+        for (uint32_t c = lane * 8; on && c < p.cols; c += G * 8) {
+            float v[8];
+            first(c, v);
+            if constexpr (NORM) {
+                if (hid) store_part<DT>(hid, c, p.cols, v);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) sum = __builtin_fmaf(v[e], v[e], sum);
+            }
+            weigh(c, v);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const uint32_t a = magnitude(v[e]);
+                top = top > a ? top : a;
+            }
+        }
+        row_sum_max<G, WG>(sum, top, redf, redu, set);
+        float rstd = 1.0f;
+        if constexpr (NORM) rstd = 1.0f / __builtin_sqrtf(sum / (float)p.cols + p.eps);
+        const Scale s = scale_of(top, rstd);
+        if (on && lane == 0) {
+            p.scale[row] = s.s;
+            if (NORM && p.rstd) p.rstd[row] = rstd;
+        }
+        int8_t* q = p.q + row * p.ldq;
+        for (uint32_t c = lane * 8; on && c < p.cols; c += G * 8) {
+            float v[8];
+            if (hid) load_part<DT>(hid, c, p.cols, v);   // x may be gone: hidden may be x itself
+            else first(c, v);
+            weigh(c, v);
+            const u32x2 b = bytes8(v, s);
+            if (p.cols - c >= 8) {
+                *reinterpret_cast<u32x2_at1*>(q + c) = b;
+            } else {
+#pragma unroll
+                for (int e = 0; e < 8; ++e)
+                    if (c + e < p.cols) q[c + e] = (int8_t)(b[e / 4] >> (8 * (e % 4)));
             }
         }
     }
@@ -185,38 +244,101 @@ __global__ void __launch_bounds__(G < 256 ? 256 : G) dequantize_kernel(const Deq
         const int8_t* q = p.q + row * p.ldq;
         T* y = (T*)p.y + row * p.ldy;
         const float s = p.scale[row];
-        for (uint32_t c = lane * 8; c < p.cols; c += G * 8) {
+        if (p.cols < 8) {
+            if (lane < p.cols) Type<DT>::put(y + lane, (float)q[lane] * s);
+            continue;
+        }
+        for (uint32_t n = lane * 8; n < p.cols; n += G * 8) {
+            const uint32_t c = min(n, p.cols - 8);
             float v[8];
-            if (p.cols - c >= 8) {
-                const u32x2 w = *reinterpret_cast<const u32x2_at1*>(q + c);
+            const u32x2 w = *reinterpret_cast<const u32x2_at1*>(q + c);
 #pragma unroll
-                for (int e = 0; e < 8; ++e) v[e] = (float)(int8_t)(w[e / 4] >> (8 * (e % 4))) * s;
-            } else {
-#pragma unroll
-                for (int e = 0; e < 8; ++e) v[e] = c + e < p.cols ? (float)q[c + e] * s : 0.0f;
-            }
-            store_part<DT>(y, c, p.cols, v);
+            for (int e = 0; e < 8; ++e) v[e] = (float)(int8_t)(w[e / 4] >> (8 * (e % 4))) * s;
+            Type<DT>::store8(y + c, v);
         }
     }
 }
 
 // dx and, for the work-group's rows blockIdx.x, blockIdx.x + parts, ..., the
 // sums of dn xhat for each column: a thread has the same columns in every row, so
-// they stay in its registers and are added in row order.
+// they stay in its registers and are added in row order.  dx leaves after the sums and dres is read before
+// them: dx may be dn or dres.
 template <int DT, int G, int R>
 __global__ void __launch_bounds__(G) norm_backward_kernel(const NormBackward p) {
-    typedef typename Type<DT>::T T;
-    constexpr int KEEP = R ? R : 1;
+    typedef Type<DT> Y;
+    typedef typename Y::T T;
     __shared__ float redf[2][G / 64];
     __shared__ uint32_t redu[2][G / 64];
     const uint32_t lane = threadIdx.x;
-    const uint32_t pieces = R ? R : (p.cols + G * 8 - 1) / (G * 8);
     const T* gain = (const T*)p.gain;
-    float acc[KEEP][8];
+    float acc[R][8];
 #pragma unroll
-    for (int i = 0; i < KEEP; ++i)
+    for (int i = 0; i < R; ++i)
 #pragma unroll
         for (int e = 0; e < 8; ++e) acc[i][e] = 0.0f;
+    const float per = 1.0f / (float)p.cols;
+    int set = 0;
+    for (uint64_t row = blockIdx.x; row < p.rows; row += p.parts, set ^= 1) {
+        const T* dn = (const T*)p.dn + row * p.lddn;
+        const T* hid = (const T*)p.hidden + row * p.ldh;
+        const T* res = p.dres ? (const T*)p.dres + row * p.lddr : nullptr;
+        T* dx = (T*)p.dx + row * p.lddx;
+        const float rstd = p.rstd[row];
+        float u[R][8], xh[R][8];
+        typename Y::Eight d[R];
+        float sum = 0.0f;
+        uint32_t none = 0;
+#pragma unroll
+        for (int i = 0; i < R; ++i) {
+            const Piece c = piece_of<G>(i, lane, p.cols);
+            if (!c.on) continue;
+            float g[8];
+            Y::load8(dn + c.c, u[i]);
+            Y::load8(hid + c.c, xh[i]);
+            if (res) d[i] = Y::get8(res + c.c);
+            Y::load8(gain + c.c, g);
+            // u = dn gain, xhat; and dn xhat for the gain's gradient
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                xh[i][e] *= rstd;
+                acc[i][e] = __builtin_fmaf(u[i][e], xh[i][e], acc[i][e]);
+                u[i][e] *= g[e];
+                sum = __builtin_fmaf((uint32_t)e < c.twice ? 0.0f : u[i][e], (uint32_t)e < c.twice ? 0.0f : xh[i][e], sum);
+            }
+        }
+        row_sum_max<G, G>(sum, none, redf, redu, set);
+        const float mean = sum * per;
+#pragma unroll
+        for (int i = 0; i < R; ++i) {
+            const Piece c = piece_of<G>(i, lane, p.cols);
+            if (!c.on) continue;
+            float y[8];
+            if (res) Y::spread(d[i], y);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const float z = rstd * (u[i][e] - xh[i][e] * mean);
+                y[e] = res ? z + y[e] : z;
+            }
+            Y::store8(dx + c.c, y);
+        }
+    }
+    if (p.dgain) {
+        float* part = p.partial + (uint64_t)blockIdx.x * p.cols;
+#pragma unroll
+        for (int i = 0; i < R; ++i) {
+            const Piece c = piece_of<G>(i, lane, p.cols);
+            if (c.on) Type<Q8_F32>::store8(part + c.c, acc[i]);
+        }
+    }
+}
+
+// The same for rows of fewer than eight values and for rows longer than registers hold.
+template <int DT, int G> __global__ void __launch_bounds__(G) norm_backward_any_kernel(const NormBackward p) {
+    typedef typename Type<DT>::T T;
+    __shared__ float redf[2][G / 64];
+    __shared__ uint32_t redu[2][G / 64];
+    const uint32_t lane = threadIdx.x;
+    const T* gain = (const T*)p.gain;
     const float per = 1.0f / (float)p.cols;
     float* part = p.dgain ? p.partial + (uint64_t)blockIdx.x * p.cols : nullptr;
     int set = 0;
@@ -226,10 +348,8 @@ __global__ void __launch_bounds__(G) norm_backward_kernel(const NormBackward p) 
         const T* res = p.dres ? (const T*)p.dres + row * p.lddr : nullptr;
         T* dx = (T*)p.dx + row * p.lddx;
         const float rstd = p.rstd[row];
-        float u[KEEP][8], xh[KEEP][8];
         float sum = 0.0f;
         uint32_t none = 0;
-        // u = dn gain, xhat; and dn xhat for the gain's gradient
         auto first = [&](uint32_t c, float (&u)[8], float (&xh)[8], float (&a)[8]) __attribute__((always_inline)) {
             float g[8];
             load_part<DT>(dn, c, p.cols, u);
@@ -240,62 +360,28 @@ __global__ void __launch_bounds__(G) norm_backward_kernel(const NormBackward p) 
                 xh[e] *= rstd;
                 a[e] = __builtin_fmaf(u[e], xh[e], a[e]);
                 u[e] *= g[e];
-                sum = __builtin_fmaf(u[e], xh[e], sum);
             }
         };
-        auto last = [&](uint32_t c, const float (&u)[8], const float (&xh)[8], float mean) __attribute__((always_inline)) {
-            float d[8];
+        // the column sums stay in the partial row, each entry its own thread's
+        for (uint32_t c = lane * 8; c < p.cols; c += G * 8) {
+            float u[8], xh[8], a[8] = {};
+            if (part && row != blockIdx.x) load_part<Q8_F32>(part, c, p.cols, a);
+            first(c, u, xh, a);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) sum = __builtin_fmaf(u[e], xh[e], sum);
+            if (part) store_part<Q8_F32>(part, c, p.cols, a);
+        }
+        row_sum_max<G, G>(sum, none, redf, redu, set);
+        for (uint32_t c = lane * 8; c < p.cols; c += G * 8) {
+            float u[8], xh[8], a[8] = {}, d[8] = {};
+            first(c, u, xh, a);
             if (res) load_part<DT>(res, c, p.cols, d);
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
-                const float y = rstd * (u[e] - xh[e] * mean);
-                d[e] = res ? y + d[e] : y;
+                const float z = rstd * (u[e] - xh[e] * (sum * per));
+                d[e] = res ? z + d[e] : z;
             }
             store_part<DT>(dx, c, p.cols, d);
-        };
-        if constexpr (R > 0) {
-#pragma unroll
-            for (int i = 0; i < R; ++i) {
-                const uint32_t c = (i * G + lane) * 8;
-                if (c < p.cols) first(c, u[i], xh[i], acc[i]);
-            }
-            row_sum_max<G, G>(sum, none, redf, redu, set);
-#pragma unroll
-            for (int i = 0; i < R; ++i) {
-                const uint32_t c = (i * G + lane) * 8;
-                if (c < p.cols) last(c, u[i], xh[i], sum * per);
-            }
-        } else {
-            // the column sums stay in the partial row, each entry its own thread's
-            for (uint32_t i = 0; i < pieces; ++i) {
-                const uint32_t c = (i * G + lane) * 8;
-                if (c >= p.cols) continue;
-                float a[8];
-#pragma unroll
-                for (int e = 0; e < 8; ++e) a[e] = 0.0f;
-                if (part && row != blockIdx.x) load_part<Q8_F32>(part, c, p.cols, a);
-                first(c, u[0], xh[0], a);
-                if (part) store_part<Q8_F32>(part, c, p.cols, a);
-            }
-            row_sum_max<G, G>(sum, none, redf, redu, set);
-            for (uint32_t i = 0; i < pieces; ++i) {
-                const uint32_t c = (i * G + lane) * 8;
-                if (c >= p.cols) continue;
-                const float total = sum;
-                float a[8] = {};   // its column sums are in the partial row already
-                first(c, u[0], xh[0], a);
-                sum = total;
-                last(c, u[0], xh[0], total * per);
-            }
-        }
-    }
-    if constexpr (R > 0) {
-        if (part) {
-#pragma unroll
-            for (int i = 0; i < R; ++i) {
-                const uint32_t c = (i * G + lane) * 8;
-                if (c < p.cols) store_part<Q8_F32>(part, c, p.cols, acc[i]);
-            }
         }
     }
 }
@@ -332,16 +418,17 @@ uint32_t groups_for(uint64_t rows, uint32_t rows_per_group) {
     return (uint32_t)(g < kMostGroups ? g : kMostGroups);
 }
 
-// The threads of a row and their pieces of eight values: the least G * R that holds the row, and
-// of those the most threads.  (16384 rows, F16, G x R: 4096 columns 512 x 1 85.7 us, 256 x 2 91.7, 1024 x
-// 1 127; 8192 columns 1024 x 1 175 us, 5.4 TB/s, 256 x 4 189.  1000 x 4097: 256 x 3 8.9 us, 1024 x 1 9.9.
-// 8192 x 11008: 512 x 3 133 us, 1024 x 2 175.)
+// The threads of a row and their pieces of eight values: the least G * R that holds the row, with the
+// most threads up to 512.  (F16, G x R: 16384 x 8192 512 x 2 178 us, 5.3 TB/s, 1024 x 1 202, 256 x 4 206.
+// 1000 x 4097: 256 x 3 8.5 us, 512 x 2 9.4, 1024 x 1 11.9.  8192 x 6001: 256 x 3 81 us, 512 x 2 85.  1 x 4096:
+// 512 x 1 2.9 us, 128 x 4 4.5.)
 template <int DT, bool NORM> hipError_t quantize_any(const Quantize& p, hipStream_t s) {
     const uint32_t pieces = (uint32_t)ceil_div(p.cols, 8);
     auto on = [&](auto g, auto r) {
         constexpr int G = decltype(g)::value, R = decltype(r)::value;
         return launch(quantize_kernel<DT, NORM, G, R>, groups_for(p.rows, G < 256 ? 256 / G : 1), G < 256 ? 256 : G, p, s);
     };
+    if (p.cols < 8) return launch(quantize_any_kernel<DT, NORM, 64>, groups_for(p.rows, 4), 256, p, s);
     if (pieces <= 64) return on(Int<64>{}, Int<1>{});
     if (pieces <= 128) return on(Int<128>{}, Int<1>{});
     if (pieces <= 192) return on(Int<64>{}, Int<3>{});
@@ -349,11 +436,11 @@ template <int DT, bool NORM> hipError_t quantize_any(const Quantize& p, hipStrea
     if (pieces <= 384) return on(Int<128>{}, Int<3>{});
     if (pieces <= 512) return on(Int<512>{}, Int<1>{});
     if (pieces <= 768) return on(Int<256>{}, Int<3>{});
-    if (pieces <= 1024) return on(Int<1024>{}, Int<1>{});
+    if (pieces <= 1024) return on(Int<512>{}, Int<2>{});
     if (pieces <= 1536) return on(Int<512>{}, Int<3>{});
-    if (pieces <= 2048) return on(Int<1024>{}, Int<2>{});
+    if (pieces <= 2048) return on(Int<512>{}, Int<4>{});
     if (pieces <= 4096) return on(Int<1024>{}, Int<4>{});
-    return on(Int<1024>{}, Int<0>{});
+    return launch(quantize_any_kernel<DT, NORM, 1024>, groups_for(p.rows, 1), 1024, p, s);
 }
 
 template <int DT> hipError_t dequantize_any(const Dequantize& p, hipStream_t s) {
@@ -361,41 +448,29 @@ template <int DT> hipError_t dequantize_any(const Dequantize& p, hipStream_t s) 
     return launch(dequantize_kernel<DT, 256>, groups_for(p.rows, 1), 256, p, s);
 }
 
-// As for quantize_any.
-uint32_t backward_threads(uint32_t cols) {
-    const uint32_t pieces = (uint32_t)ceil_div(cols, 8);
-    return pieces <= 64 ? 64 : pieces <= 128 ? 128 : pieces <= 192 ? 64 : pieces <= 256 ? 256 : pieces <= 384 ? 128 :
-           pieces <= 512 ? 512 : pieces <= 768 ? 256 : 1024;
-}
+// Row ranges that a column's sum is taken over first, one work-group each: two a CU that has 512
+// threads (BF16, 16384 x 4096: 256 / 512 / 1024 ranges 118 / 98 / 116 us, 5.5 TB/s; 16384 x 8192 207 / 194 / 205;
+// 1000 x 999 10.3 / 8.0 / 10.8): each range is written, read and added once more.
+constexpr uint32_t kMostParts = 512;
 template <int DT> hipError_t backward_any(const NormBackward& p, hipStream_t s) {
     const uint32_t pieces = (uint32_t)ceil_div(p.cols, 8);
     auto on = [&](auto g, auto r) {
         constexpr int G = decltype(g)::value, R = decltype(r)::value;
         return launch(norm_backward_kernel<DT, G, R>, p.parts, G, p, s);
     };
+    if (p.cols < 8) return launch(norm_backward_any_kernel<DT, 64>, p.parts, 64, p, s);
     if (pieces <= 64) return on(Int<64>{}, Int<1>{});
     if (pieces <= 128) return on(Int<128>{}, Int<1>{});
-    if (pieces <= 192) return on(Int<64>{}, Int<3>{});
     if (pieces <= 256) return on(Int<256>{}, Int<1>{});
-    if (pieces <= 384) return on(Int<128>{}, Int<3>{});
     if (pieces <= 512) return on(Int<512>{}, Int<1>{});
-    if (pieces <= 768) return on(Int<256>{}, Int<3>{});
-    if (pieces <= 1024) return on(Int<1024>{}, Int<1>{});
+    if (pieces <= 1024) return on(Int<512>{}, Int<2>{});
     if (pieces <= 2048) return on(Int<1024>{}, Int<2>{});
-    return on(Int<1024>{}, Int<0>{});
+    return launch(norm_backward_any_kernel<DT, 1024>, p.parts, 1024, p, s);
 }
 
 }  // namespace
 
-uint32_t norm_backward_parts(uint32_t rows, uint32_t cols) {
-    // as many work-groups as are resident at once, 2048 threads a CU, up to 1024, but two rows each
-    // where there are 512 of those: every range is written, read and added once more
-    const uint32_t resident = kComputeUnits * 2048u / backward_threads(cols);
-    uint32_t parts = resident < 1024u ? resident : 1024u;
-    const uint32_t two = (rows + 1) / 2 < 512u ? 512u : (rows + 1) / 2;
-    if (parts > two) parts = two;
-    return rows < parts ? rows : parts;
-}
+uint32_t norm_backward_parts(uint32_t rows) { return rows < kMostParts ? rows : kMostParts; }
 
 hipError_t launch_quantize(int dtype, bool norm, const Quantize& p, hipStream_t s) {
     if (norm)

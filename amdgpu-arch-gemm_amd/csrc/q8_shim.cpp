@@ -297,7 +297,7 @@ int q8_workspace_size(int call, int dtype, uint32_t m, uint32_t n, uint32_t k, s
     *bytes = 0;
     CHECK(check_type(dtype));
     if (call == Q8_CALL_RMSNORM_BACKWARD) {
-        *bytes = piece((size_t)norm_backward_parts(m, k) * k * sizeof(float));
+        *bytes = piece((size_t)norm_backward_parts(m) * k * sizeof(float));
     } else if (call == Q8_CALL_GEMM) {
         for (int copies = 0; copies < 4; ++copies) {    // the route depends on them
             const size_t need = plan_gemm(m, n, k, copies & 1, copies & 2).at.total;
@@ -398,7 +398,7 @@ int q8_rmsnorm_backward(q8_handle* h, int dtype, const void* dn, uint32_t lddn, 
     OnDevice on(h->device);
     HIP_TRY(on.status());
     NormBackward p = {dn, hidden, gain, rstd, dres, dx, dgain, nullptr, lddn, ldh, lddr, lddx, rows, cols,
-                      norm_backward_parts(rows, cols)};
+                      norm_backward_parts(rows)};
     if (dgain && rows) {
         CHECK(take_workspace(h, (size_t)p.parts * cols * sizeof(float)));
         p.partial = reinterpret_cast<float*>(h->workspace);
