@@ -73,41 +73,48 @@ __device__ __forceinline__ void pack_weights(const PackWeights& p, uint32_t wave
     const uint32_t r = wave_id % tr * 64 + lane % 8 * 8;
     uint32_t c = wave_id / tr * (8 * W) + lane / 8 * W;
     if (r >= p.cp || c >= p.cols) return;
-    const bool narrow = p.cols < W;
-    if (!narrow && c + W > p.cols) c = p.cols - W;
-    uint32_t in[8][W / 4];
+    uint16_t* dst = (uint16_t*)p.dst + r;
+    auto put = [&](uint32_t column, const float (&v)[8]) __attribute__((always_inline)) {
+        const u32x4 w = {pair16<HALF>(v[0], v[1]), pair16<HALF>(v[2], v[3]), pair16<HALF>(v[4], v[5]), pair16<HALF>(v[6], v[7])};
+        uint16_t* d = dst + (uint64_t)column * p.dst_ld;
+        *reinterpret_cast<u32x4*>(d) = w;
+        for (uint32_t q = 1; q < p.terms; ++q) *reinterpret_cast<u32x4*>(d + (uint64_t)q * p.cp) = w;
+    };
     float s[8];
 #pragma unroll
-    for (int k = 0; k < 8; ++k) {
-        const uint32_t row = min(r + k, p.rows - 1);
-        const int8_t* src = p.q + (uint64_t)row * p.ldq + c;
-        if (narrow) {
+    for (int k = 0; k < 8; ++k) s[k] = p.scale ? p.scale[min(r + k, p.rows - 1)] : 1.0f;
 #pragma unroll
-            for (int e = 0; e < W / 4; ++e) in[k][e] = 0;
-            for (uint32_t e = 0; e < p.cols; ++e) in[k][e / 4] |= (uint32_t)(uint8_t)src[e] << (8 * (e % 4));
-        } else if constexpr (W == 16) {
+    for (int k = 0; k < 8; ++k) s[k] = r + k < p.rows ? s[k] * factor : 0.0f;
+    if (p.cols < W) {
+#pragma unroll 1
+        for (uint32_t e = c; e < p.cols; ++e) {
+            float v[8];
+#pragma unroll
+            for (int k = 0; k < 8; ++k) v[k] = (float)p.q[(uint64_t)min(r + k, p.rows - 1) * p.ldq + e] * s[k];
+            put(e, v);
+        }
+        return;
+    }
+    c = min(c, p.cols - W);
+    uint32_t in[8][W / 4];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+        const int8_t* src = p.q + (uint64_t)min(r + k, p.rows - 1) * p.ldq + c;
+        if constexpr (W == 16) {
             const u32x4 w = *reinterpret_cast<const u32x4_at1*>(src);
 #pragma unroll
             for (int e = 0; e < 4; ++e) in[k][e] = w[e];
         } else {
             in[k][0] = *reinterpret_cast<const u32_at1*>(src);
         }
-        s[k] = p.scale ? p.scale[row] : 1.0f;
     }
 #pragma unroll
-    for (int k = 0; k < 8; ++k) s[k] = r + k < p.rows ? s[k] * factor : 0.0f;
-    uint16_t* dst = (uint16_t*)p.dst + (uint64_t)c * p.dst_ld + r;
-#pragma unroll
     for (int e = 0; e < W; ++e) {
-        if (narrow && (uint32_t)e >= p.cols) break;
         float v[8];
         // a scale that is not a number takes its whole row along, zeros too
 #pragma unroll
         for (int k = 0; k < 8; ++k) v[k] = (float)(int8_t)(in[k][e / 4] >> (8 * (e % 4))) * s[k];
-        const u32x4 w = {pair16<HALF>(v[0], v[1]), pair16<HALF>(v[2], v[3]), pair16<HALF>(v[4], v[5]), pair16<HALF>(v[6], v[7])};
-        uint16_t* d = dst + (uint64_t)e * p.dst_ld;
-        *reinterpret_cast<u32x4*>(d) = w;
-        for (uint32_t q = 1; q < p.terms; ++q) *reinterpret_cast<u32x4*>(d + (uint64_t)q * p.cp) = w;
+        put(c + e, v);
     }
 }
 
@@ -126,17 +133,17 @@ __device__ __forceinline__ void three(float x, uint16_t (&b)[3]) {
 
 // Eight 16-bit patterns of a row from column c (0 past `cols`), for FP32 in three terms.
 template <int DT, int TERMS>
-__device__ __forceinline__ void eight(const void* src, uint64_t ld, uint32_t row, uint32_t c, uint32_t cols, const float* scale,
-                                      bool scale_by_row, uint32_t (&out)[TERMS][4]) {
+__device__ __forceinline__ void eight(const void* src, uint64_t ld, uint64_t row, uint32_t c, uint32_t cols, const float* scale,
+                                      uint32_t (&out)[TERMS][4]) {
     typedef typename Type<DT>::T T;
-    const T* line = (const T*)src + (uint64_t)row * ld;
+    const T* line = (const T*)src + row * ld;
     if constexpr (DT == Q8_F32) {
         float v[8];
         load_part<DT>(line, c, cols, v);
         if (scale) {
 #pragma unroll
             for (int e = 0; e < 8; ++e)
-                if (c + e < cols) v[e] *= scale[scale_by_row ? row : c + e];
+                if (c + e < cols) v[e] *= scale[c + e];
         }
         uint16_t b[8][3];
 #pragma unroll
@@ -181,7 +188,7 @@ template <int DT> __device__ __forceinline__ void pack_rows(const PackGradient& 
     const uint32_t c = (uint32_t)(id - row * pieces) * 8;
     if (row >= p.rows) return;
     uint32_t v[TERMS][4] = {};
-    if (c < p.cols) eight<DT, TERMS>(p.src, p.src_ld, (uint32_t)row, c, p.cols, p.scale, false, v);
+    if (c < p.cols) eight<DT, TERMS>(p.src, p.src_ld, row, c, p.cols, p.scale, v);
 #pragma unroll
     for (int q = 0; q < TERMS; ++q)
         *reinterpret_cast<u32x4*>((uint16_t*)p.dst + row * p.dst_ld + (uint64_t)q * p.cp + c) =
@@ -190,37 +197,69 @@ template <int DT> __device__ __forceinline__ void pack_rows(const PackGradient& 
 
 // dst[i][c] from src[c][i]: a wave turns 64 x 64.
 template <int DT> __device__ __forceinline__ void pack_turned(const PackGradient& p, uint32_t wave_id) {
+    typedef typename Type<DT>::T T;
     constexpr int TERMS = DT == Q8_F32 ? 3 : 1;
     const uint32_t tk = (p.cp + 63) / 64;
     const uint32_t lane = threadIdx.x & 63;
     const uint32_t k0 = wave_id % tk * 64 + lane % 8 * 8;
     uint32_t r = wave_id / tk * 64 + lane / 8 * 8;
     if (k0 >= p.cp || r >= p.rows) return;
-    // the last columns with those before them, as pack_weights
-    if (p.rows >= 8) r = min(r, p.rows - 8);
-    uint32_t in[8][TERMS][4];
+    const T* src = (const T*)p.src;
+    uint16_t* dst = (uint16_t*)p.dst + k0;
+    if (p.rows < 8) {
+#pragma unroll 1
+        for (; r < p.rows; ++r) {
+            uint16_t b[8][3] = {};
 #pragma unroll
-    for (int k = 0; k < 8; ++k) eight<DT, TERMS>(p.src, p.src_ld, min(k0 + k, p.cols - 1), r, p.rows, p.scale, true, in[k]);
+            for (int k = 0; k < 8; ++k) {
+                if (k0 + k >= p.cols) continue;
+                const T x = src[(uint64_t)(k0 + k) * p.src_ld + r];
+                if constexpr (DT == Q8_F32) three(p.scale ? x * p.scale[k0 + k] : x, b[k]);
+                else b[k][0] = __builtin_bit_cast(uint16_t, x);
+            }
 #pragma unroll
-    for (int k = 0; k < 8; ++k)
+            for (int q = 0; q < TERMS; ++q)
+                *reinterpret_cast<u32x4*>(dst + (uint64_t)r * p.dst_ld + (uint64_t)q * p.cp) =
+                    u32x4{(uint32_t)b[0][q] | (uint32_t)b[1][q] << 16, (uint32_t)b[2][q] | (uint32_t)b[3][q] << 16,
+                          (uint32_t)b[4][q] | (uint32_t)b[5][q] << 16, (uint32_t)b[6][q] | (uint32_t)b[7][q] << 16};
+        }
+        return;
+    }
+    r = min(r, p.rows - 8);     // as pack_weights
+    typename Type<DT>::Eight in[8];
 #pragma unroll
-        for (int q = 0; q < TERMS; ++q)
+    for (int k = 0; k < 8; ++k) in[k] = Type<DT>::get8(src + (uint64_t)min(k0 + k, p.cols - 1) * p.src_ld + r);
+    if constexpr (DT == Q8_F32) {
+        float s[8];
 #pragma unroll
-            for (int e = 0; e < 4; ++e)
-                if (k0 + k >= p.cols) in[k][q][e] = 0;
+        for (int k = 0; k < 8; ++k) s[k] = p.scale ? p.scale[min(k0 + k, p.cols - 1)] : 1.0f;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-        if (r + e >= p.rows) break;
+        for (int e = 0; e < 8; ++e) {
+            uint16_t b[8][3];
 #pragma unroll
-        for (int q = 0; q < TERMS; ++q) {
+            for (int k = 0; k < 8; ++k) {
+                const float x = e < 4 ? in[k].lo[e % 4] : in[k].hi[e % 4];
+                three(k0 + k < p.cols ? x * s[k] : 0.0f, b[k]);
+            }
+#pragma unroll
+            for (int q = 0; q < 3; ++q)
+                *reinterpret_cast<u32x4*>(dst + (uint64_t)(r + e) * p.dst_ld + (uint64_t)q * p.cp) =
+                    u32x4{(uint32_t)b[0][q] | (uint32_t)b[1][q] << 16, (uint32_t)b[2][q] | (uint32_t)b[3][q] << 16,
+                          (uint32_t)b[4][q] | (uint32_t)b[5][q] << 16, (uint32_t)b[6][q] | (uint32_t)b[7][q] << 16};
+        }
+    } else {
+#pragma unroll
+        for (int k = 0; k < 8; ++k)
+            if (k0 + k >= p.cols) in[k] = u32x4{0, 0, 0, 0};
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
             uint32_t w[4];
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
-                const uint32_t lo = in[2 * k][q][e / 2], hi = in[2 * k + 1][q][e / 2];
+                const uint32_t lo = in[2 * k][e / 2], hi = in[2 * k + 1][e / 2];
                 w[k] = e % 2 ? lo >> 16 | (hi & 0xffff0000u) : (lo & 0xffffu) | hi << 16;
             }
-            *reinterpret_cast<u32x4*>((uint16_t*)p.dst + (uint64_t)(r + e) * p.dst_ld + (uint64_t)q * p.cp + k0) =
-                u32x4{w[0], w[1], w[2], w[3]};
+            *reinterpret_cast<u32x4*>(dst + (uint64_t)(r + e) * p.dst_ld) = u32x4{w[0], w[1], w[2], w[3]};
         }
     }
 }
