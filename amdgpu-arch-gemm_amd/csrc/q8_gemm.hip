@@ -7,14 +7,14 @@
 // finish_kernel adds the sums of K ranges where a product has too few tiles.
 // direct_kernel: few tokens and small products; operands go from memory to the matrix cores.
 //
-// What bounds the large products.  8192^3 in 8-bit integers takes 405 us, 2.7 Pops (a large library
-// product of the same operands 2.35): the card's power, at which an MFMA-only loop on such
-// data reaches 4.0, then the loads.  Without any load the kernel takes 338 us, with all of
-// them out of L2 about 390.  In 16 bits (16384 x 4096 x 4096, BF16) it runs at 1.35 - 1.44 PFLOP/s
-// (library 1.32), 350 us without loads against 400: power alone, but for 12%.
+// What bounds the large products.  8192^3 in 8-bit integers takes 405 - 433 us by card, 2.5 - 2.7 Pops (a
+// large library product 2.35); 16384 x 4096 x 4096 in BF16 400 - 415 us, 1.33 - 1.37 PFLOP/s (library 1.32).
+// The card's power, at which a loop of matrix instructions alone reaches 4.0 Pops and 2.0 PFLOP/s on
+// such data, and the loads' way into LDS: without any load 375 us instead of 430, in BF16
+// 362 instead of 413.  Not memory: with every load from lines that L2 holds the times are the same.
 // Four waves of 128 x 128 rather than eight of 128 x 64: LDS gives 128 bytes a cycle, and eight
 // waves would ask it for 192 KB a K tile beside the 64 KB that arrive, as long as the matrix
-// instructions take (8192^3: 464 us).
+// instructions take (the step from eight to four: 4096^3 74.0 -> 57.5 us, 8192^3 464 -> 453).
 #include "q8_device.hpp"
 #include "q8_internal.hpp"
 #include "q8_plan.hpp"
@@ -64,7 +64,8 @@ __device__ __forceinline__ uint32_t xcd_order(uint32_t id, uint32_t total) {
 }
 // Tiles in groups of six rows of them, column by column within a group: the 32 tiles of
 // 256 x 256 that an XCD works on at a time are then 6 x 5.3 and read the fewest
-// lines (8192^3 in 8-bit integers: six 406 us, four 436, eight 443, sixteen 452).
+// lines.  With `ask` below it matters little: 8192^3 in 8-bit integers takes 426 - 436 us with three to
+// eight, 444 with sixteen; F16 4096 x 4096 x 16384 390 - 396 and 403.
 __device__ __forceinline__ void tile_of(uint32_t z, uint32_t nx, uint32_t ny, uint32_t& tx, uint32_t& ty) {
     constexpr uint32_t GROUP = 6;
     const uint32_t group = z / (GROUP * ny), first = group * GROUP;
@@ -165,8 +166,8 @@ __global__ void __launch_bounds__(256, T == 4 ? 2 : 1) product_kernel(const Prod
     // A tile's loads have the time of one tile, which L2 keeps and memory does not: a dword of
     // each of its lines is asked for one tile before, into LDS that nobody reads.  The
     // work-groups beside this one on the XCD share its rows of A or of B, so each
-    // asks for a quarter of them (8192^3 in 8-bit integers: 427 -> 415 us, BF16 16384 x 4096 x 4096
-    // 408 -> 401; asking for all of its lines, or more than a tile ahead, costs more than it gives).
+    // asks for a quarter of them (F16 4096 x 4096 x 16384: 405 -> 393 us, 8192^3 in 8-bit integers
+    // 438 -> 431, BF16 16384 x 4096 x 4096 415 -> 413).
     constexpr uint32_t SHARE = BM / 4;
     const uint32_t pr = (wave < 2 ? ty % 4 : tx % 4) * SHARE + (uint32_t)(wave & 1) * (SHARE / 2) + (uint32_t)lane;
     const uint32_t pp = (uint32_t)lane < SHARE / 2 ? pr * (wave < 2 ? lda : ldb) : NOWHERE;
@@ -199,7 +200,7 @@ __global__ void __launch_bounds__(256, T == 4 ? 2 : 1) product_kernel(const Prod
         else f.a[i - TN] = *reinterpret_cast<const u32x4*>(from + (fa ^ (s * 64)) + (i - TN) * 16 * KB);
     };
     // One step's products, the next step's operands and, in the second step, a tile's loads
-    // between them.
+    // between them, evenly: all at its start make 431 us 461 (8192^3 in 8-bit integers).
     auto multiply = [&](const Step& f, Step& next, uint32_t buf, uint32_t s, auto loads) __attribute__((always_inline)) {
         constexpr int N = TM * TN, GAP = N / (TM + TN) - 1, EVERY = N / (2 * LOADS);
 #pragma unroll
