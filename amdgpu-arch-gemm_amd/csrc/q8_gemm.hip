@@ -23,7 +23,6 @@ namespace q8 {
 namespace {
 
 constexpr int BUFFER_RSRC_WORD3 = 0x00020000;
-constexpr int XCDS = 8;
 constexpr uint32_t NOWHERE = 0x80000000u;    // an offset past every descriptor's end: loads give 0
 constexpr int KB = kTileBytes;
 
@@ -56,12 +55,6 @@ template <> struct Atom<E_BF16> {
     }
 };
 
-// Workgroups go round the XCDs one by one: consecutive tiles to one XCD instead, so that
-// its L2 serves their shared rows.
-__device__ __forceinline__ uint32_t xcd_order(uint32_t id, uint32_t total) {
-    const uint32_t x = id % XCDS, q = total / XCDS, r = total % XCDS;
-    return x * q + (x < r ? x : r) + id / XCDS;
-}
 // Tiles in groups of six rows of them, column by column within a group: the 32 tiles of
 // 256 x 256 that an XCD works on at a time are then 6 x 5.3 and read the fewest
 // lines.  With `ask` below it matters little: 8192^3 in 8-bit integers takes 426 - 436 us with three to

@@ -119,4 +119,17 @@ struct PackGradient {
 // gradient: null where it is read as it is.
 Q8_INTERNAL hipError_t launch_pack(int dtype, const PackWeights& weights, const PackGradient* gradient, hipStream_t stream);
 
+// A gradient from operands as they are: d[r][c] = sum over s of a_r,s scale_s q_s,c (turned: a_s,r), of
+// type `out`, Q8_F32 or a's.  cols >= 4; turned: rows >= 8, else sum >= 32; F16: sum <= kFewScales.
+struct Gradient {
+    const void* a;
+    const int8_t* q;
+    const float* scale;
+    void* d;
+    uint64_t lda, ldq, ldd;
+    uint32_t rows, cols, sum;
+    int out, accumulate;
+};
+Q8_INTERNAL hipError_t launch_gradient(int dtype, bool turned, const Gradient& p, hipStream_t stream);
+
 }  // namespace q8

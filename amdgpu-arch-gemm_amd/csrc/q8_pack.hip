@@ -4,6 +4,7 @@
 // into the workspace first.  Each kernel is one pass and bounded by memory.
 #include "q8_device.hpp"
 #include "q8_internal.hpp"
+#include "q8_plan.hpp"
 
 namespace q8 {
 namespace {
@@ -47,14 +48,6 @@ __global__ void __launch_bounds__(256) copy_rows_kernel(const CopyRows p) {
         }
         *reinterpret_cast<u32x4*>(p.dst + row * p.dst_ld + c) = v;
     }
-}
-
-__device__ __forceinline__ uint16_t bits16(float x, bool half) {
-    if (half) return __builtin_bit_cast(uint16_t, (_Float16)x);
-    return __builtin_bit_cast(uint16_t, (__bf16)x);
-}
-template <bool HALF> __device__ __forceinline__ uint32_t pair16(float x, float y) {
-    return HALF ? Type<Q8_F16>::pair(x, y) : Type<Q8_BF16>::pair(x, y);
 }
 
 // Turning needs no LDS: a lane takes eight rows of the source, W values of each, and has eight
@@ -116,19 +109,6 @@ __device__ __forceinline__ void pack_weights(const PackWeights& p, uint32_t wave
         for (int k = 0; k < 8; ++k) v[k] = (float)(int8_t)(in[k][e / 4] >> (8 * (e % 4))) * s[k];
         put(c + e, v);
     }
-}
-
-// x = hi + mid + lo in BF16: both differences are exact, and three terms of 8 bits
-// hold the 24 of FP32.  Infinities and NaN stay in the first term.
-__device__ __forceinline__ void three(float x, uint16_t (&b)[3]) {
-    const uint32_t size = magnitude(x);
-    uint32_t hi = (uint32_t)bits16(x, false) << 16;
-    // finite, but the nearest BF16 is not: the first term is cut off instead
-    if (size >= 0x7f7f8000u && size < 0x7f800000u) hi = __builtin_bit_cast(uint32_t, x) & 0xffff0000u;
-    const float r = size < 0x7f800000u ? x - __builtin_bit_cast(float, hi) : 0.0f;
-    b[0] = (uint16_t)(hi >> 16);
-    b[1] = bits16(r, false);
-    b[2] = bits16(r - __builtin_bit_cast(float, (uint32_t)b[1] << 16), false);
 }
 
 // Eight 16-bit patterns of a row from column c (0 past `cols`), for FP32 in three terms.
@@ -264,35 +244,6 @@ template <int DT> __device__ __forceinline__ void pack_turned(const PackGradient
     }
 }
 
-// Half precision keeps 2^-14 .. 2^15 with all its bits, and the weights' values are
-// q scale: a power of two brings the largest scale to 2^7 .. 2^8 (127 times it still fits),
-// and the product is multiplied by its inverse in 32 bits.  The largest finite scale over a
-// work-group:
-template <int THREADS> __device__ __forceinline__ uint32_t largest(const float* scale, uint32_t count, uint32_t (&red)[THREADS / 64]) {
-    uint32_t top = 0;
-    for (uint32_t i = threadIdx.x; i < count; i += THREADS * 4) {
-        uint32_t a[4];      // four loads at once; the last one again past the end
-#pragma unroll
-        for (int k = 0; k < 4; ++k) a[k] = magnitude(scale[min(i + k * THREADS, count - 1)]);
-#pragma unroll
-        for (int k = 0; k < 4; ++k)
-            if (a[k] < 0x7f800000u) top = top > a[k] ? top : a[k];
-    }
-    float none = 0.0f;
-    wave_sum_max(none, top);
-    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = top;
-    __syncthreads();
-#pragma unroll
-    for (int w = 0; w < THREADS / 64; ++w) top = top > red[w] ? top : red[w];
-    return top;
-}
-// 2^-e and 2^e
-__device__ __forceinline__ void powers(uint32_t top, float& down, float& up) {
-    int e = (int)(top >> 23) - 127 - 7;           // scale in [2^(e + 7), 2^(e + 8))
-    e = e < -126 ? -126 : e > 126 ? 126 : e;      // both powers stay normal
-    down = __builtin_bit_cast(float, (uint32_t)(127 - e) << 23);
-    up = __builtin_bit_cast(float, (uint32_t)(127 + e) << 23);
-}
 __global__ void __launch_bounds__(1024) scale_pair_kernel(const float* scale, uint32_t count, float* pair) {
     __shared__ uint32_t red[16];
     const uint32_t top = largest<1024>(scale, count, red);
@@ -300,15 +251,14 @@ __global__ void __launch_bounds__(1024) scale_pair_kernel(const float* scale, ui
 }
 
 // Both operands of a gradient in one launch: the first work-groups lay out the weights, the
-// others the gradient.  Few scales (KNOWN == false) are looked through by every work-group
-// that needs their largest, which costs less than a launch.
+// others the gradient.  KNOWN: the scales are too many for each work-group to look through, and
+// a kernel has set the pair.
 struct PackBoth {
     PackWeights w;
     PackGradient g;
     uint64_t weight_groups, groups;
     int wide;   // pack_weights' W is 16
 };
-constexpr uint32_t kFewScales = 4096;
 template <int DT, bool TURN, bool KNOWN> __global__ void __launch_bounds__(256) pack_kernel(const PackBoth p) {
     constexpr bool HALF = DT == Q8_F16;
     __shared__ uint32_t red[4];

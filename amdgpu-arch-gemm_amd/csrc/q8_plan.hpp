@@ -14,6 +14,9 @@ constexpr uint32_t kMaxSplits = 16;
 constexpr uint64_t kMaxRowBytes = 1u << 22;
 // Up to so many tokens the weights are streamed once, from rows that start anywhere.
 constexpr uint32_t kFewTokens = 64;
+// So many scales are looked through by every work-group that needs their largest, which costs
+// less than a launch.
+constexpr uint32_t kFewScales = 4096;
 
 struct Tile {
     uint32_t m, n;
@@ -103,6 +106,50 @@ inline bool direct_for_many(uint64_t m, uint64_t n, uint64_t k, double tile_time
     const double rows = t <= kComputeUnits ? 32.0 * (double)t : 48.0 * (double)(div_up(m, 32) * div_up(n, 16));
     const double direct = 3.8 + rows * (double)k / 7e6;     // each work-group's rows, out of L2
     return direct < tile_time + 3.0 * copies + 2.0 * (double)copy_bytes / 3e6;
+}
+
+// The kernel that takes a gradient from operands as they are: rows of a work-group without and
+// with a turn of the 16-bit operand, and 64 columns.
+constexpr uint32_t kGradientRows[2] = {64, 128};
+inline uint64_t gradient_groups(bool turned, uint64_t rows, uint64_t cols) {
+    return div_up(rows, kGradientRows[turned]) * div_up(cols, 64);
+}
+// Its waves, which share the summed index: eight where no work-group waits and each still has
+// two steps (BF16, not turned, 64 x 4224 x 924: 8.3 us, four 9.1; 874 x 128 x 106: 4.7 and 4.2).  Turned FP32
+// operands are three terms of 64 values a lane, and 512 registers: four.
+inline uint32_t gradient_waves(bool turned, bool f32, uint64_t rows, uint64_t cols, uint64_t sum) {
+    return gradient_groups(turned, rows, cols) <= kComputeUnits && sum > 512 && !(turned && f32) ? 8 : 4;
+}
+// Its time in microseconds, fitted to launches back to back: a fixed one and, for each 32 values that a
+// wave takes of the summed index, one; with more work-groups than CUs one for each round of
+// them, of which a short last one (half a round and less) overlaps the one before.  Rows of 16-bit
+// values that start between dwords (odd) are read in more pieces: 4096 x 1024 x 1024 21 us, 3000 x 1003 x 1001 34;
+// turned 18 and, of rows of 999, 31 at 999 x 4097 x 1000.
+inline double gradient_time(bool turned, bool f32, bool odd, uint64_t rows, uint64_t cols, uint64_t sum) {
+    const uint64_t groups = gradient_groups(turned, rows, cols);
+    const uint32_t waves = gradient_waves(turned, f32, rows, cols, sum);
+    const double k = (double)div_up(sum, 32 * waves);
+    const double fixed = turned ? 4.2 : 3.0, pieces = !odd ? 1.0 : turned ? 1.15 : 1.6;
+    if (groups <= kComputeUnits) {
+        constexpr double step[2][2][2] = {{{0.75, 1.2}, {2.2, 3.1}}, {{1.0, 1.65}, {3.2, 3.2}}};
+        return fixed + pieces * step[turned][f32][waves == 8] * k;
+    }
+    const uint64_t slots = turned && f32 ? kComputeUnits : 2 * kComputeUnits, rest = groups % slots;
+    const double rounds = (double)(groups / slots) + (!rest ? 0.0 : rest > slots / 2 ? 1.0 : turned ? 0.7 : 0.4);
+    const double round = turned ? fixed + (f32 ? 3.2 : 1.75) * k : f32 ? 1.2 + 3.0 * k : 1.4 + 1.32 * k;
+    return (turned ? 0.0 : fixed) + pieces * rounds * round;
+}
+// Whether a gradient is taken so, rather than laid out (`packed_bytes` read and written) and multiplied by the
+// kernels above in `tile_time`: it has no more than the kernel's smallest operands, and in F16 the scales
+// are few.  (BF16, turned / not, direct and laid out: 512^3 8.0 and 12.5 us / 6.0 and 12.0, 1024^3 11.1 and 17.6 /
+// 9.0 and 15.8, 2048 x 2048 x 1024 17.3 and 21.9 / 24.8 and 19.0; FP32 512^3 16.5 and 21.1 / 11.1 and 18.1,
+// 300 x 300 x 2000 52 and 27 / 28 and 24.)
+inline bool gradient_direct(bool turned, bool f32, bool f16, bool odd, uint64_t rows, uint64_t cols, uint64_t sum, double tile_time,
+                            uint64_t packed_bytes) {
+    if (cols < 4 || sum < (turned ? 1u : 32u) || (turned && rows < 8) || (f16 && sum > kFewScales)) return false;
+    // 2^32 work-items are one grid's end
+    if (rows > (1u << 22) || gradient_groups(turned, rows, cols) >= (1u << 22)) return false;
+    return 1.05 * gradient_time(turned, f32, odd, rows, cols, sum) < tile_time + 3.0 + (double)packed_bytes / 3e6;
 }
 
 }  // namespace q8

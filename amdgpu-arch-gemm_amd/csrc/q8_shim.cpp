@@ -153,6 +153,7 @@ struct Layout {
 };
 
 struct Grad {
+    bool direct;        // from the operands as they are; else:
     uint64_t cp;        // values of the summed index in a laid-out row
     uint32_t terms;
     uint64_t kb;        // its bytes
@@ -160,8 +161,9 @@ struct Grad {
     ProductPlan plan;
     Layout at;
 };
-// The gradient D (rows x cols) summed over `sum`; copy_a: the 16-bit operand is laid out too.
-int plan_grad(int dtype, uint64_t rows, uint64_t cols, uint64_t sum, bool copy_a, Grad& g) {
+// The gradient D (rows x cols) summed over `sum`; copy_a: the 16-bit operand would be laid out too,
+// turned: it has the summed index from row to row, odd: its rows start between dwords.
+int plan_grad(int dtype, bool turned, bool odd, uint64_t rows, uint64_t cols, uint64_t sum, bool copy_a, Grad& g) {
     g.cp = round_up(sum, 8);
     g.terms = dtype == Q8_F32 ? 3 : 1;
     g.kb = g.cp * g.terms * 2;
@@ -174,6 +176,9 @@ int plan_grad(int dtype, uint64_t rows, uint64_t cols, uint64_t sum, bool copy_a
     if (g.pitch % 4096 == 0) g.pitch += 512;
     g.plan = plan_product(rows, cols, g.kb);
     g.at = Layout();
+    const uint64_t bytes = cols * (sum + g.kb) + (copy_a || dtype == Q8_F32 ? rows * (sum * type_bytes(dtype) + g.kb) : 0);
+    g.direct = gradient_direct(turned, dtype == Q8_F32, dtype == Q8_F16, odd, rows, cols, sum, g.plan.time, bytes);
+    if (g.direct) return SGEMM_OK;
     if (copy_a || dtype == Q8_F32) g.at.add(g.at.a, rows * g.pitch);
     g.at.add(g.at.b, cols * g.pitch);
     if (dtype == Q8_F16) g.at.add(g.at.pair, 8);
@@ -214,6 +219,8 @@ GemmPlan plan_gemm(uint64_t m, uint64_t n, uint64_t k, bool copy_a, bool copy_b)
 bool rows_aligned(const void* p, uint64_t ld_bytes) {
     return (uintptr_t)p % 16 == 0 && ld_bytes % 16 == 0 && ld_bytes <= kMaxRowBytes;
 }
+
+bool odd_rows(const void* p, uint64_t ld_bytes) { return ((uintptr_t)p | ld_bytes) % 4 != 0; }
 
 int check_handle(const q8_handle* h) { return h ? SGEMM_OK : fail(SGEMM_E_INVALID, "the handle is null"); }
 int check_type(int dtype) { return is_type(dtype) ? SGEMM_OK : fail(SGEMM_E_INVALID, "%d is no type", dtype); }
@@ -304,10 +311,12 @@ int q8_workspace_size(int call, int dtype, uint32_t m, uint32_t n, uint32_t k, s
             if (need > *bytes) *bytes = need;
         }
     } else if (call == Q8_CALL_GRAD_INPUT || call == Q8_CALL_GRAD_WEIGHT) {
-        Grad g;
-        if (call == Q8_CALL_GRAD_INPUT) CHECK(plan_grad(dtype, m, k, n, true, g));
-        else CHECK(plan_grad(dtype, n, k, m, true, g));
-        *bytes = g.at.total;
+        for (int i = 0; i < 4; ++i) {   // the route depends on dy's rows
+            Grad g;
+            if (call == Q8_CALL_GRAD_INPUT) CHECK(plan_grad(dtype, false, i & 2, m, k, n, i & 1, g));
+            else CHECK(plan_grad(dtype, true, i & 2, n, k, m, true, g));
+            if (g.at.total > *bytes) *bytes = g.at.total;
+        }
     } else {
         return fail(SGEMM_E_INVALID, "%d is no call with a workspace", call);
     }
@@ -456,13 +465,17 @@ int q8_grad_input(q8_handle* h, int dtype, const void* dy, uint32_t lddy, const 
     // dy's rows hold the summed index: read where they are if they are whole pieces
     const bool copy = dtype == Q8_F32 || n % 8 || !rows_aligned(dy, (uint64_t)lddy * size);
     Grad g;
-    CHECK(plan_grad(dtype, m, k, n, copy, g));
-    CHECK(check_grid(m, k, g.plan));
+    CHECK(plan_grad(dtype, false, odd_rows(dy, (uint64_t)lddy * size), m, k, n, copy, g));
+    if (!g.direct) CHECK(check_grid(m, k, g.plan));
     for (const Span& s : in) CHECK(check(s));
     CHECK(check(out));
     for (const Span& s : in) CHECK(check_apart(out, s));
     OnDevice on(h->device);
     HIP_TRY(on.status());
+    if (g.direct) {
+        const Gradient p = {dy, qw, sw, dx, lddy, ldw, lddx, m, k, n, dtype, 0};
+        return launched(launch_gradient(dtype, false, p, h->stream), "launch of the input's gradient failed");
+    }
     CHECK(take_workspace(h, g.at.total));
     const Element e = dtype == Q8_F16 ? E_F16 : E_BF16;
     float* pair = dtype == Q8_F16 ? reinterpret_cast<float*>(h->workspace + g.at.pair) : nullptr;
@@ -498,13 +511,17 @@ int q8_grad_weight(q8_handle* h, int dtype, const void* dy, uint32_t lddy, const
     const Span in[] = {{"dy", dy, m, n, lddy, size}, {"qx", qx, m, k, ldx, 1}, vec("sx", sx, m, 4)};
     const Span out{"dw", dw, n, k, lddw, type_bytes(out_dtype)};
     Grad g;
-    CHECK(plan_grad(dtype, n, k, m, true, g));
-    CHECK(check_grid(n, k, g.plan));
+    CHECK(plan_grad(dtype, true, odd_rows(dy, (uint64_t)lddy * size), n, k, m, true, g));
+    if (!g.direct) CHECK(check_grid(n, k, g.plan));
     for (const Span& s : in) CHECK(check(s));
     CHECK(check(out));
     for (const Span& s : in) CHECK(check_apart(out, s));
     OnDevice on(h->device);
     HIP_TRY(on.status());
+    if (g.direct) {
+        const Gradient p = {dy, qx, sx, dw, lddy, ldx, lddw, n, k, m, out_dtype, accumulate != 0};
+        return launched(launch_gradient(dtype, true, p, h->stream), "launch of the weights' gradient failed");
+    }
     CHECK(take_workspace(h, g.at.total));
     const Element e = dtype == Q8_F16 ? E_F16 : E_BF16;
     float* pair = dtype == Q8_F16 ? reinterpret_cast<float*>(h->workspace + g.at.pair) : nullptr;

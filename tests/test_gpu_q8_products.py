@@ -184,6 +184,35 @@ def test_gradients_in_k_ranges(ops, dtype):
     assert all(np.array_equal(a, b) for a, b in zip(first, again))
 
 
+# The sizes above are taken from the operands as they are, most of these are laid out: the input's
+# gradient, the weights', or both.
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("m,n,k,pad,shift", [(1301, 1203, 1501, 0, 0), (130, 4100, 133, 0, 0), (4100, 130, 133, 0, 0),
+                                             (2050, 130, 1000, 3, 1), (333, 5000, 129, 8, 8), (9, 30, 6, 0, 0),
+                                             (30, 7, 70, 1, 1)])
+def test_gradients_laid_out(ops, m, n, k, pad, shift, dtype):
+    print(f"gradients {m}x{n}x{k} +{pad} {dtype}", flush=True)
+    t = TYPES[dtype]
+    assert any(Q.workspace_size(c, t, m, n, k) for c in (Q.CALL_GRAD_INPUT, Q.CALL_GRAD_WEIGHT))
+    _gradients(ops, m, n, k, dtype, pad, shift)
+
+
+@pytest.mark.parametrize("dtype,out", [("bf16", "f32"), ("f16", "f32"), ("bf16", "bf16"), ("f16", "f16"), ("f32", "f32")])
+def test_weight_gradients_laid_out_accumulate(ops, dtype, out):
+    _gradients(ops, 4100, 130, 133, dtype, out=out, accumulate=True)
+
+
+# ends of tiles (64 and 128 rows, 64 columns), of the last values of a row that are taken with those
+# before them, of a wave's steps (32) and of four or eight waves' turns
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("m,n,k", [(32, 32, 4), (33, 39, 5), (63, 65, 7), (65, 64, 68), (127, 129, 67), (129, 136, 63), (40, 8, 64),
+                                   (160, 161, 30), (511, 160, 61), (513, 513, 60), (545, 1100, 131)])
+def test_gradients_ends(ops, m, n, k, dtype):
+    print(f"gradients {m}x{n}x{k} {dtype}", flush=True)
+    _gradients(ops, m, n, k, dtype)
+    _gradients(ops, m, n, k, dtype, 5, 3, accumulate=True)
+
+
 def test_gradients_against_differences(ops):
     """The product is linear in its 8-bit operands: a step of one in an operand changes a
     loss by exactly its gradient times the scale."""
@@ -235,6 +264,43 @@ def test_gradients_of_values_that_are_not_numbers(ops):
             assert np.all(np.isfinite(rest))
 
 
+@pytest.mark.parametrize("m,n,k", [(100, 72, 66), (97, 105, 35), (4100, 130, 133), (130, 4100, 133)])
+def test_infinities_anywhere_in_a_sum(ops, m, n, k):
+    """Also in the values before a sum's last ones, which are loaded with them."""
+    rng = np.random.default_rng(16)
+    qx, qw = random_q(rng, m, k), random_q(rng, n, k)
+    qx[qx == 0], qw[qw == 0] = 1, 1
+    one_m, one_n = Q.Array.of(np.ones(m)), Q.Array.of(np.ones(n))
+    for dtype, t in TYPES.items():
+        for back in (1, 9, 20, 31, 33):
+            dy = stored(rng.normal(0, 1, (m, n)), dtype)
+            i, j = m - back, n - back
+            dy[i, j] = np.inf
+            dx, dw = Q.Array(m, k, t), Q.Array(n, k, t)
+            ops.grad_input(t, Q.Array.of(dy, t), Q.Array.of(qw), one_n, dx, m, n, k)
+            ops.grad_weight(t, Q.Array.of(dy, t), Q.Array.of(qx), one_m, t, dw, m, n, k)
+            ops.synchronize()
+            for got, row, q in ((dx.numpy(), i, qw[j]), (dw.numpy(), j, qx[i])):
+                assert np.array_equal(got[row], np.sign(q.astype(np.float64)) * np.inf), (dtype, back)
+                assert np.all(np.isfinite(np.delete(got, row, axis=0)))
+
+
+@pytest.mark.parametrize("m,n,k", [(100, 72, 66), (4100, 130, 133), (130, 4100, 133)])
+def test_scales_that_are_not_numbers_reach_every_sum(ops, m, n, k):
+    rng = np.random.default_rng(17)
+    qx, qw = random_q(rng, m, k), random_q(rng, n, k)
+    qx[m - 2], qw[n - 2] = 0, 0
+    sx, sw = np.ones(m), np.ones(n)
+    sx[m - 2], sw[n - 2] = np.nan, np.nan
+    for dtype, t in TYPES.items():
+        dy = Q.Array.of(stored(rng.normal(0, 1, (m, n)), dtype), t)
+        dx, dw = Q.Array(m, k, t), Q.Array(n, k, t)
+        ops.grad_input(t, dy, Q.Array.of(qw), Q.Array.of(sw), dx, m, n, k)
+        ops.grad_weight(t, dy, Q.Array.of(qx), Q.Array.of(sx), t, dw, m, n, k)
+        ops.synchronize()
+        assert np.all(np.isnan(dx.numpy())) and np.all(np.isnan(dw.numpy()))
+
+
 def test_operands_past_32_bit_offsets(ops):
     """Rows far apart: the last token's start past 2^32 bytes."""
     m, n, k, ld = 130, 20, 64, 1 << 25
@@ -252,10 +318,11 @@ def test_operands_past_32_bit_offsets(ops):
         far.close()
 
 
-def test_captured_calls_replay(ops):
+# both gradients from operands as they are, and the weights' or the input's laid out
+@pytest.mark.parametrize("m,n,k", [(300, 200, 4100), (4100, 200, 300), (300, 4100, 200)])
+def test_captured_calls_replay(ops, m, n, k):
     """A graph of a training step's calls replays with the bits of the eager calls, also
     after the handle's workspace has been replaced by a larger one."""
-    m, n, k = 300, 200, 4100
     rng = np.random.default_rng(9)
     hip = _Hip()
     stream = hip.stream()
@@ -286,7 +353,7 @@ def test_captured_calls_replay(ops):
         hip.begin(stream, 0)
         try:
             with pytest.raises(S.SgemmError) as e:      # nothing is reserved yet
-                o.grad_weight(Q.BF16, dy, qx, sx, Q.BF16, dw, m, n, k, ldx=ldq)
+                o.rmsnorm_backward(Q.BF16, dn, x, g, rstd, None, dx, dg, m, k)
             assert e.value.code == -4 and "q8_reserve" in e.value.message
         finally:
             _ok(hip.lib.hipGraphExecDestroy(hip.end(stream)))

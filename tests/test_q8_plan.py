@@ -60,3 +60,40 @@ def program(tmp_path_factory):
 def test_plans_hold_over_all_sizes(program):
     out = subprocess.run([program], capture_output=True, text=True)
     assert out.returncode == 0 and out.stdout.strip() == "ok", out.stdout + out.stderr
+
+
+GRADIENTS = r"""
+#include "q8_plan.hpp"
+#include <cstdio>
+using namespace q8;
+int main() {
+    const uint64_t sizes[] = {1, 3, 4, 7, 8, 31, 32, 33, 64, 128, 129, 512, 513, 1000, 4096, 4097, 16384, 1000000, 2000000,
+                              1u << 22, 1u << 28, 4294967295u};
+    int direct = 0, eight = 0;
+    for (int turned = 0; turned < 2; ++turned) for (int type = 0; type < 3; ++type)
+        for (uint64_t r : sizes) for (uint64_t c : sizes) for (uint64_t s : sizes) {
+            if (s > 2000000 || !gradient_direct(turned, type == 0, type == 1, false, r, c, s, 1e300, 0)) continue;
+            ++direct;
+            // what the kernel takes for granted
+            bool ok = c >= 4 && (turned ? r >= 8 : s >= 32) && (type != 1 || s <= kFewScales);
+            const uint64_t groups = gradient_groups(turned, r, c), waves = gradient_waves(turned, type == 0, r, c, s);
+            ok = ok && groups * waves * 64 < (1ull << 32) && (waves == 4 || waves == 8);
+            ok = ok && div_up(r, kGradientRows[turned]) * kGradientRows[turned] + 512 < (1ull << 32);
+            ok = ok && div_up(c, 64) * 64 < (1ull << 32) && s + 8 * 64 < (1ull << 32);
+            ok = ok && !(turned && type == 0 && waves == 8);
+            eight += waves == 8;
+            if (!ok) { std::printf("%d %d %llu %llu %llu\n", turned, type, (unsigned long long)r, (unsigned long long)c, (unsigned long long)s); return 1; }
+        }
+    std::puts(direct && eight ? "ok" : "no case");
+}
+"""
+
+
+def test_gradients_from_operands_as_they_are(tmp_path):
+    source = tmp_path / "gradients.cpp"
+    source.write_text(GRADIENTS)
+    subprocess.run(["g++", "-std=c++17", "-O1", "-Wall", "-Werror", "-fsanitize=undefined", "-fno-sanitize-recover=all",
+                    "-I", os.path.join(ROOT, "amdgpu-arch-gemm_amd", "csrc"), str(source), "-o", str(tmp_path / "gradients")],
+                   check=True)
+    out = subprocess.run([str(tmp_path / "gradients")], capture_output=True, text=True)
+    assert out.returncode == 0 and out.stdout.strip() == "ok", out.stdout + out.stderr
