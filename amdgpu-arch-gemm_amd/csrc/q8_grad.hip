@@ -5,7 +5,12 @@
 // eight rows of W values each has W such operands after a turn in registers, so a wave
 // turns what it multiplies, and nothing is laid out in memory first: one launch and no
 // workspace.  That turn is done again by each work-group that reads the values, so it pays for
-// small gradients, where launches and their latency count.
+// small gradients, where launches and their latency count: BF16 512^3 6.0 us (8.0 with the 16-bit operand
+// turned), laid out and multiplied 12.0 (12.5); 1024^3 9.0 (11.1) and 15.8 (17.6).  About 3 us (4 turned) are the
+// launch, the first loads and the join; then each step waits for its loads, 0.75 us (1.0) with one
+// work-group a CU, and 1.3 - 1.75 for both of two, where the loads' number bounds it.  FP32 takes three times
+// the matrix instructions and 700 to 1200 others a step to split 64 values a lane into three terms, which
+// bound it: 512^3 11.1 us (16.5).  Groups in XCD order: 4096 x 1024 x 1024 25 -> 21 us.
 #include "q8_device.hpp"
 #include "q8_internal.hpp"
 #include "q8_plan.hpp"

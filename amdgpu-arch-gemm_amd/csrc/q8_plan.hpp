@@ -143,7 +143,8 @@ inline double gradient_time(bool turned, bool f32, bool odd, uint64_t rows, uint
 // kernels above in `tile_time`: it has no more than the kernel's smallest operands, and in F16 the scales
 // are few.  (BF16, turned / not, direct and laid out: 512^3 8.0 and 12.5 us / 6.0 and 12.0, 1024^3 11.1 and 17.6 /
 // 9.0 and 15.8, 2048 x 2048 x 1024 17.3 and 21.9 / 24.8 and 19.0; FP32 512^3 16.5 and 21.1 / 11.1 and 18.1,
-// 300 x 300 x 2000 52 and 27 / 28 and 24.)
+// 300 x 300 x 2000 52 and 27 / 28 and 24.  Over 60 random sizes that the fit has not seen the choice costs 1.3% more
+// than the better one on average, 29% at most.)
 inline bool gradient_direct(bool turned, bool f32, bool f16, bool odd, uint64_t rows, uint64_t cols, uint64_t sum, double tile_time,
                             uint64_t packed_bytes) {
     if (cols < 4 || sum < (turned ? 1u : 32u) || (turned && rows < 8) || (f16 && sum > kFewScales)) return false;

@@ -89,7 +89,8 @@ class Array(S.DeviceBuffer):
         return out
 
     def numpy(self) -> np.ndarray:
-        """The values on the host (bfloat16 as float32); waits for the device."""
+        """The values on the host (bfloat16 as float32); waits for the device, but for a stream that was
+        made not to wait for it: `synchronize` first."""
         host = np.empty((self.rows, self.ld), {F32: np.float32, F16: np.float16, BF16: np.uint16, "int8": np.int8}[self.kind])
         if host.size:
             S._check("sgemm_memcpy_d2h", S.load_library().sgemm_memcpy_d2h(host.ctypes.data, self.ptr, host.nbytes))
