@@ -318,6 +318,43 @@ def test_operands_past_32_bit_offsets(ops):
         far.close()
 
 
+# taken as they are, and laid out: the weights' with fewer than eight channels, the input's with fewer than four features
+@pytest.mark.parametrize("n,k", [(20, 64), (7, 64), (20, 3)])
+def test_gradient_operands_past_32_bit_offsets(ops, n, k):
+    """Rows far apart: the last ones start past 2^32 bytes."""
+    m, ld = 130, 1 << 25
+    rng = np.random.default_rng(18)
+
+    def far(values, size):
+        buffer = S.DeviceBuffer((len(values) - 1) * ld * size + values.shape[1] * size)
+        for i, row in enumerate(values):
+            row = np.ascontiguousarray(row)
+            S._check("sgemm_memcpy_h2d", S.load_library().sgemm_memcpy_h2d(buffer.ptr + i * ld * size, row.ctypes.data, row.nbytes))
+        return buffer
+
+    q, ones = random_q(rng, m, k), Q.Array.of(np.ones(m))
+    dy = rng.integers(-8, 9, (m, n)).astype(np.float64)        # exact products and sums throughout
+    wq = far(q, 1)
+    dw = Q.Array(n, k, Q.F32)
+    ops.grad_weight(Q.F16, Q.Array.of(dy, Q.F16), wq, ones, Q.F32, dw, m, n, k, ldx=ld)
+    ops.synchronize()
+    assert np.array_equal(dw.numpy(), dy.T @ q)
+    # as many channels as there were tokens: the weights' rows are far apart
+    dx = Q.Array(n, k, Q.F32)
+    ops.grad_input(Q.F32, Q.Array.of(dy.T), wq, ones, dx, n, m, k, ldw=ld)
+    ops.synchronize()
+    assert np.array_equal(dx.numpy(), dy.T @ q)
+    wq.close()
+    wdy = far(dy.astype(np.float16), 2)
+    ops.grad_weight(Q.F16, wdy, Q.Array.of(q), ones, Q.F32, dw, m, n, k, lddy=ld)
+    qw, dx = random_q(rng, n, k), Q.Array(m, k, Q.F16)
+    ops.grad_input(Q.F16, wdy, Q.Array.of(qw), Q.Array.of(np.ones(n)), dx, m, n, k, lddy=ld)
+    ops.synchronize()
+    assert np.array_equal(dw.numpy(), dy.T @ q)
+    assert np.array_equal(dx.numpy().astype(np.float64), stored(dy @ qw, "f16"))
+    wdy.close()
+
+
 # both gradients from operands as they are, and the weights' or the input's laid out
 @pytest.mark.parametrize("m,n,k", [(300, 200, 4100), (4100, 200, 300), (300, 4100, 200)])
 def test_captured_calls_replay(ops, m, n, k):
