@@ -23,6 +23,28 @@ typedef f32x4 f32x4_at4 __attribute__((aligned(4)));
 typedef uint32_t u32_at1 __attribute__((aligned(1)));
 typedef u32x2 u32x2_at1 __attribute__((aligned(1)));
 typedef u32x4 u32x4_at1 __attribute__((aligned(1)));
+typedef u32x4 u32x4_at4 __attribute__((aligned(4)));
+
+// 16 bytes as they are loaded.  From any address: five dwords, those that hold the bytes, and the bytes
+// once they have arrived, of which `at` of the first dword come before them.  No dword is read
+// that holds none of the 16.
+template <bool ODD> struct Raw {
+    typedef u32x4 T;
+    static __device__ __forceinline__ T load(const char* p) { return *reinterpret_cast<const u32x4_at1*>(p); }
+    static __device__ __forceinline__ u32x4 value(const T& v, uint32_t) { return v; }
+};
+template <> struct Raw<true> {
+    struct T { u32x4 w; uint32_t x; };
+    static __device__ __forceinline__ T load(const char* p) {
+        const char* first = (const char*)((uintptr_t)p & ~(uintptr_t)3);
+        const char* last = (const char*)((uintptr_t)(p + 15) & ~(uintptr_t)3);
+        return T{*reinterpret_cast<const u32x4_at4*>(first), *reinterpret_cast<const uint32_t*>(last)};
+    }
+    static __device__ __forceinline__ u32x4 value(const T& v, uint32_t at) {
+        return u32x4{__builtin_amdgcn_alignbyte(v.w[1], v.w[0], at), __builtin_amdgcn_alignbyte(v.w[2], v.w[1], at),
+                     __builtin_amdgcn_alignbyte(v.w[3], v.w[2], at), __builtin_amdgcn_alignbyte(v.x, v.w[3], at)};
+    }
+};
 
 template <int DT> struct Type;
 template <> struct Type<Q8_F32> {
@@ -152,18 +174,18 @@ template <bool HALF> __device__ __forceinline__ uint32_t pair16(float x, float y
     return HALF ? Type<Q8_F16>::pair(x, y) : Type<Q8_BF16>::pair(x, y);
 }
 
-// x = hi + mid + lo in BF16: both differences are exact, and three terms of 8 bits
-// hold the 24 of FP32.  Infinities and NaN stay in the first term.
-__device__ __forceinline__ void three(float x, uint16_t (&b)[3]) {
-    const uint32_t size = magnitude(x);
-    uint32_t hi = (uint32_t)bits16(x, false) << 16;
-    // finite, but the nearest BF16 is not: the first term is cut off instead
-    if (size >= 0x7f7f8000u && size < 0x7f800000u) hi = __builtin_bit_cast(uint32_t, x) & 0xffff0000u;
-    const float r = size < 0x7f800000u ? x - __builtin_bit_cast(float, hi) : 0.0f;
-    b[0] = (uint16_t)(hi >> 16);
-    b[1] = bits16(r, false);
-    b[2] = bits16(r - __builtin_bit_cast(float, (uint32_t)b[1] << 16), false);
+// x = hi + mid + lo in BF16, each cut off where the next one goes on: both differences are exact,
+// and three terms of 8 bits hold the 24 of FP32.  Infinities and NaN stay in the first term.
+// The terms are the upper halves of b.
+__device__ __forceinline__ void three(float x, uint32_t (&b)[3]) {
+    x = __builtin_canonicalizef(x);     // a NaN has a bit in the first term
+    b[0] = __builtin_bit_cast(uint32_t, x);
+    const float r = magnitude(x) < 0x7f800000u ? x - __builtin_bit_cast(float, b[0] & 0xffff0000u) : 0.0f;
+    b[1] = __builtin_bit_cast(uint32_t, r);
+    b[2] = __builtin_bit_cast(uint32_t, r - __builtin_bit_cast(float, b[1] & 0xffff0000u));
 }
+// The upper halves of two.
+__device__ __forceinline__ uint32_t uppers(uint32_t lo, uint32_t hi) { return __builtin_amdgcn_perm(hi, lo, 0x07060302u); }
 
 // Half precision keeps 2^-14 .. 2^15 with all its bits, and the weights' values are
 // q scale: a power of two brings the largest scale to 2^7 .. 2^8 (127 times it still fits),

@@ -150,7 +150,7 @@ __global__ void __launch_bounds__(WAVES * 64, DT == Q8_F32 && TURN ? 1 : 2) grad
         for (int i = 0; i < MT; ++i) {
             u32x4 w[TERMS];
             if constexpr (DT == Q8_F32) {
-                uint16_t h[8][3];
+                uint32_t h[8][3];
 #pragma unroll
                 for (int k = 0; k < 8; ++k) {
                     const Eight& from = v.a[TURN ? k : i];
@@ -160,7 +160,7 @@ __global__ void __launch_bounds__(WAVES * 64, DT == Q8_F32 && TURN ? 1 : 2) grad
 #pragma unroll
                 for (int t = 0; t < TERMS; ++t)
 #pragma unroll
-                    for (int k = 0; k < 4; ++k) w[t][k] = (uint32_t)h[2 * k][t] | (uint32_t)h[2 * k + 1][t] << 16;
+                    for (int k = 0; k < 4; ++k) w[t][k] = uppers(h[2 * k][t], h[2 * k + 1][t]);
             } else if constexpr (TURN) {
 #pragma unroll
                 for (int k = 0; k < 4; ++k)

@@ -127,13 +127,13 @@ __device__ __forceinline__ void eight(const void* src, uint64_t ld, uint64_t row
             for (int e = 0; e < 8; ++e)
                 if (c + e < cols) v[e] *= scale[c + e];
         }
-        uint16_t b[8][3];
+        uint32_t b[8][3];
 #pragma unroll
         for (int e = 0; e < 8; ++e) three(v[e], b[e]);
 #pragma unroll
         for (int q = 0; q < TERMS; ++q)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) out[q][e] = (uint32_t)b[2 * e][q] | (uint32_t)b[2 * e + 1][q] << 16;
+            for (int e = 0; e < 4; ++e) out[q][e] = uppers(b[2 * e][q], b[2 * e + 1][q]);
     } else {
         if (cols >= 8) {
             // a last piece with the values before it, moved down
@@ -191,19 +191,18 @@ template <int DT> __device__ __forceinline__ void pack_turned(const PackGradient
     if (p.rows < 8) {
 #pragma unroll 1
         for (; r < p.rows; ++r) {
-            uint16_t b[8][3] = {};
+            uint32_t b[8][3] = {};
 #pragma unroll
             for (int k = 0; k < 8; ++k) {
                 if (k0 + k >= p.cols) continue;
                 const T x = src[(uint64_t)(k0 + k) * p.src_ld + r];
                 if constexpr (DT == Q8_F32) three(p.scale ? x * p.scale[k0 + k] : x, b[k]);
-                else b[k][0] = __builtin_bit_cast(uint16_t, x);
+                else b[k][0] = (uint32_t)__builtin_bit_cast(uint16_t, x) << 16;
             }
 #pragma unroll
             for (int q = 0; q < TERMS; ++q)
                 *reinterpret_cast<u32x4*>(dst + (uint64_t)r * p.dst_ld + (uint64_t)q * p.cp) =
-                    u32x4{(uint32_t)b[0][q] | (uint32_t)b[1][q] << 16, (uint32_t)b[2][q] | (uint32_t)b[3][q] << 16,
-                          (uint32_t)b[4][q] | (uint32_t)b[5][q] << 16, (uint32_t)b[6][q] | (uint32_t)b[7][q] << 16};
+                    u32x4{uppers(b[0][q], b[1][q]), uppers(b[2][q], b[3][q]), uppers(b[4][q], b[5][q]), uppers(b[6][q], b[7][q])};
         }
         return;
     }
@@ -217,7 +216,7 @@ template <int DT> __device__ __forceinline__ void pack_turned(const PackGradient
         for (int k = 0; k < 8; ++k) s[k] = p.scale ? p.scale[min(k0 + k, p.cols - 1)] : 1.0f;
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-            uint16_t b[8][3];
+            uint32_t b[8][3];
 #pragma unroll
             for (int k = 0; k < 8; ++k) {
                 const float x = e < 4 ? in[k].lo[e % 4] : in[k].hi[e % 4];
@@ -226,8 +225,7 @@ template <int DT> __device__ __forceinline__ void pack_turned(const PackGradient
 #pragma unroll
             for (int q = 0; q < 3; ++q)
                 *reinterpret_cast<u32x4*>(dst + (uint64_t)(r + e) * p.dst_ld + (uint64_t)q * p.cp) =
-                    u32x4{(uint32_t)b[0][q] | (uint32_t)b[1][q] << 16, (uint32_t)b[2][q] | (uint32_t)b[3][q] << 16,
-                          (uint32_t)b[4][q] | (uint32_t)b[5][q] << 16, (uint32_t)b[6][q] | (uint32_t)b[7][q] << 16};
+                    u32x4{uppers(b[0][q], b[1][q]), uppers(b[2][q], b[3][q]), uppers(b[4][q], b[5][q]), uppers(b[6][q], b[7][q])};
         }
     } else {
 #pragma unroll
