@@ -9,8 +9,8 @@
 // turned), laid out and multiplied 12.0 (12.5); 1024^3 9.0 (11.1) and 15.8 (17.6).  About 3 us (4 turned) are the
 // launch, the first loads and the join; then each step waits for its loads, 0.75 us (1.0) with one
 // work-group a CU, and 1.3 - 1.75 for both of two, where the loads' number bounds it.  FP32 takes three times
-// the matrix instructions and 700 to 1200 others a step to split 64 values a lane into three terms, which
-// bound it: 512^3 11.1 us (16.5).  Groups in XCD order: 4096 x 1024 x 1024 25 -> 21 us.
+// the matrix instructions and 400 to 700 others a step to split 32 (64) values a lane into three terms, which
+// bound it: 512^3 8.9 us (13.1).  Groups in XCD order: 4096 x 1024 x 1024 25 -> 21 us.
 #include "q8_device.hpp"
 #include "q8_internal.hpp"
 #include "q8_plan.hpp"
@@ -33,6 +33,10 @@ __device__ __forceinline__ u32x4 zero8(u32x4) { return u32x4{0, 0, 0, 0}; }
 __device__ __forceinline__ Type<Q8_F32>::Eight zero8(const Type<Q8_F32>::Eight&) {
     return {f32x4{0, 0, 0, 0}, f32x4{0, 0, 0, 0}};
 }
+
+// Eight values as they are loaded.
+template <typename EIGHT, bool ODD> struct Piece { typedef EIGHT T; };
+template <typename EIGHT> struct Piece<EIGHT, true> { typedef Raw<true>::T T; };
 
 // Four results of a row; the first `skip` of them are another lane's.
 template <int DT>
@@ -57,7 +61,8 @@ __device__ __forceinline__ void put4(typename Type<DT>::T* y, f32x4 v, uint32_t 
 // turn, a step's loads in flight while the one before is multiplied, and add their sums in LDS.
 // TURN: A has the summed index from row to row too, a lane takes eight values of a row, and a
 // work-group has 128 rows.
-template <int DT, bool TURN, int WAVES>
+// ODD (not turned): rows of 16-bit values that start between dwords, see Raw.
+template <int DT, bool TURN, int WAVES, bool ODD>
 __global__ void __launch_bounds__(WAVES * 64, DT == Q8_F32 && TURN ? 1 : 2) gradient_kernel(const Gradient p) {
     constexpr int MT = kGradientRows[TURN] / 16, NT = 4, TERMS = DT == Q8_F32 ? 3 : 1;
     constexpr bool HALF = DT == Q8_F16;
@@ -81,7 +86,8 @@ __global__ void __launch_bounds__(WAVES * 64, DT == Q8_F32 && TURN ? 1 : 2) grad
 #pragma unroll
     for (int i = 0; i < MT; ++i) rows[i] = min(row0 + i * 16 + fr, p.rows - 1);
     struct Step {
-        Eight a[MT];
+        typename Piece<Eight, ODD>::T a[MT];
+        uint32_t at[ODD ? MT : 1];
         uint32_t q[8];
         float s[8];
     };
@@ -114,14 +120,24 @@ __global__ void __launch_bounds__(WAVES * 64, DT == Q8_F32 && TURN ? 1 : 2) grad
             }
         } else {
 #pragma unroll
-            for (int i = 0; i < MT; ++i) v.a[i] = Type<DT>::get8(a + rows[i] * p.lda + s);
+            for (int i = 0; i < MT; ++i) {
+                const T* from = a + rows[i] * p.lda + s;
+                if constexpr (ODD) {
+                    v.at[i] = whole ? (uint32_t)(uintptr_t)from & 3u : 0u;
+                    if (whole) v.a[i] = Raw<true>::load((const char*)from);
+                    else v.a[i].w = Type<DT>::get8(from);
+                } else {
+                    v.a[i] = Type<DT>::get8(from);
+                }
+            }
             if (!whole) {
 #pragma unroll
                 for (int i = 0; i < MT; ++i)
 #pragma unroll
                     for (int e = 0; e < 8; ++e) {
                         if (s + e >= s0) continue;
-                        if constexpr (DT != Q8_F32) v.a[i][e / 2] &= e % 2 ? 0x0000ffffu : 0xffff0000u;
+                        if constexpr (ODD) v.a[i].w[e / 2] &= e % 2 ? 0x0000ffffu : 0xffff0000u;
+                        else if constexpr (DT != Q8_F32) v.a[i][e / 2] &= e % 2 ? 0x0000ffffu : 0xffff0000u;
                         else if (e < 4) v.a[i].lo[e % 4] = 0.0f;
                         else v.a[i].hi[e % 4] = 0.0f;
                     }
@@ -165,6 +181,8 @@ __global__ void __launch_bounds__(WAVES * 64, DT == Q8_F32 && TURN ? 1 : 2) grad
 #pragma unroll
                 for (int k = 0; k < 4; ++k)
                     w[0][k] = __builtin_amdgcn_perm(v.a[2 * k + 1][i / 2], v.a[2 * k][i / 2], i % 2 ? 0x07060302u : 0x05040100u);
+            } else if constexpr (ODD) {
+                w[0] = Raw<true>::value(v.a[i], v.at[i]);
             } else {
                 w[0] = v.a[i];
             }
@@ -216,17 +234,20 @@ __global__ void __launch_bounds__(WAVES * 64, DT == Q8_F32 && TURN ? 1 : 2) grad
     }
 }
 
-template <int DT, bool TURN, int WAVES> hipError_t launch(const Gradient& p, hipStream_t s) {
+template <int DT, bool TURN, int WAVES, bool ODD> hipError_t launch(const Gradient& p, hipStream_t s) {
     void* args[] = {const_cast<Gradient*>(&p)};
-    return hipLaunchKernel((const void*)&gradient_kernel<DT, TURN, WAVES>, dim3((uint32_t)gradient_groups(TURN, p.rows, p.cols)),
-                           dim3(WAVES * 64), args, 0, s);
+    return hipLaunchKernel((const void*)&gradient_kernel<DT, TURN, WAVES, ODD>,
+                           dim3((uint32_t)gradient_groups(TURN, p.rows, p.cols)), dim3(WAVES * 64), args, 0, s);
 }
 template <int DT> hipError_t gradient_any(bool turned, const Gradient& p, hipStream_t s) {
     const bool eight = gradient_waves(turned, DT == Q8_F32, p.rows, p.cols, p.sum) == 8;
-    if (!turned) return eight ? launch<DT, false, 8>(p, s) : launch<DT, false, 4>(p, s);
-    if constexpr (DT != Q8_F32)
-        if (eight) return launch<DT, true, 8>(p, s);
-    return launch<DT, true, 4>(p, s);
+    if constexpr (DT != Q8_F32) {
+        if (turned) return eight ? launch<DT, true, 8, false>(p, s) : launch<DT, true, 4, false>(p, s);
+        if (((uintptr_t)p.a | p.lda * 2) % 4) return eight ? launch<DT, false, 8, true>(p, s) : launch<DT, false, 4, true>(p, s);
+    } else if (turned) {
+        return launch<DT, true, 4, false>(p, s);
+    }
+    return eight ? launch<DT, false, 8, false>(p, s) : launch<DT, false, 4, false>(p, s);
 }
 
 }  // namespace

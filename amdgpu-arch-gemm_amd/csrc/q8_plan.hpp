@@ -122,29 +122,29 @@ inline uint32_t gradient_waves(bool turned, bool f32, uint64_t rows, uint64_t co
 }
 // Its time in microseconds, fitted to launches back to back: a fixed one and, for each 32 values that a
 // wave takes of the summed index, one; with more work-groups than CUs one for each round of
-// them, of which a short last one (half a round and less) overlaps the one before.  Rows of 16-bit
-// values that start between dwords (odd) are read in more pieces: 4096 x 1024 x 1024 21 us, 3000 x 1003 x 1001 34;
-// turned 18 and, of rows of 999, 31 at 999 x 4097 x 1000.
+// them, of which a short last one (half a round and less) overlaps the one before where a CU has
+// two.  Rows of 16-bit values that start between dwords (odd) take more loads: 1024 x 1024 x 1024 9.0 us, 1024 x
+// 1024 x 1025 10.6 (by loads from where they start 3000 x 1003 x 1001 34 us, so 27).
 inline double gradient_time(bool turned, bool f32, bool odd, uint64_t rows, uint64_t cols, uint64_t sum) {
     const uint64_t groups = gradient_groups(turned, rows, cols);
     const uint32_t waves = gradient_waves(turned, f32, rows, cols, sum);
     const double k = (double)div_up(sum, 32 * waves);
-    const double fixed = turned ? 4.2 : 3.0, pieces = !odd ? 1.0 : turned ? 1.15 : 1.6;
+    const double fixed = turned ? 4.2 : 3.0, pieces = !odd ? 1.0 : turned ? 1.15 : 1.35;
     if (groups <= kComputeUnits) {
-        constexpr double step[2][2][2] = {{{0.75, 1.2}, {2.2, 3.1}}, {{1.0, 1.65}, {3.2, 3.2}}};
+        constexpr double step[2][2][2] = {{{0.75, 1.2}, {1.45, 2.4}}, {{1.0, 1.65}, {2.25, 2.25}}};
         return fixed + pieces * step[turned][f32][waves == 8] * k;
     }
     const uint64_t slots = turned && f32 ? kComputeUnits : 2 * kComputeUnits, rest = groups % slots;
-    const double rounds = (double)(groups / slots) + (!rest ? 0.0 : rest > slots / 2 ? 1.0 : turned ? 0.7 : 0.4);
-    const double round = turned ? fixed + (f32 ? 3.2 : 1.75) * k : f32 ? 1.2 + 3.0 * k : 1.4 + 1.32 * k;
+    const double rounds = (double)(groups / slots) + (!rest ? 0.0 : rest > slots / 2 || (turned && f32) ? 1.0 : turned ? 0.7 : 0.4);
+    const double round = turned ? fixed + (f32 ? 2.25 : 1.75) * k : f32 ? 1.9 + 2.2 * k : 1.4 + 1.32 * k;
     return (turned ? 0.0 : fixed) + pieces * rounds * round;
 }
 // Whether a gradient is taken so, rather than laid out (`packed_bytes` read and written) and multiplied by the
-// kernels above in `tile_time`: it has no more than the kernel's smallest operands, and in F16 the scales
+// kernels above in `tile_time`: it has no fewer values than a lane's loads take, and in F16 the scales
 // are few.  (BF16, turned / not, direct and laid out: 512^3 8.0 and 12.5 us / 6.0 and 12.0, 1024^3 11.1 and 17.6 /
-// 9.0 and 15.8, 2048 x 2048 x 1024 17.3 and 21.9 / 24.8 and 19.0; FP32 512^3 16.5 and 21.1 / 11.1 and 18.1,
-// 300 x 300 x 2000 52 and 27 / 28 and 24.  Over 60 random sizes that the fit has not seen the choice costs 1.3% more
-// than the better one on average, 29% at most.)
+// 9.0 and 15.8, 2048 x 2048 x 1024 17.3 and 21.9 / 24.8 and 19.0; FP32 512^3 13.1 and 20.0 / 8.9 and 17.7,
+// 300 x 300 x 2000 40 and 25 / 22 and 24.  Over 80 random sizes that the fit has not seen the choice costs 0.3% more
+// than the better one on average, 16% at most.)
 inline bool gradient_direct(bool turned, bool f32, bool f16, bool odd, uint64_t rows, uint64_t cols, uint64_t sum, double tile_time,
                             uint64_t packed_bytes) {
     if (cols < 4 || sum < (turned ? 1u : 32u) || (turned && rows < 8) || (f16 && sum > kFewScales)) return false;

@@ -57,6 +57,15 @@ def test_gemm_rows_that_start_anywhere(ops, m, n, k, pad, shift):
     _product(ops, m, n, k, "bf16", pad, shift, bias=True)
 
 
+# each tile of the few-token kernel, from whole dwords and from between them
+@pytest.mark.parametrize("pad,shift", [(0, 0), (1, 1), (2, 0), (0, 3)])
+@pytest.mark.parametrize("m,n,k", [(3, 200, 1300), (2, 70, 8300), (3, 12300, 140), (20, 5000, 140), (20, 12300, 140), (50, 5000, 200),
+                                   (50, 12300, 140), (100, 90, 700), (300, 900, 72)])
+def test_gemm_few_tokens_from_any_byte(ops, m, n, k, pad, shift):
+    print(f"gemm {m}x{n}x{k} +{pad} from {shift}", flush=True)
+    _product(ops, m, n, k, "f16", pad, shift, bias=True)
+
+
 # whole rows of 16 bytes that hold values past the sum, which must not count
 @pytest.mark.parametrize("k", [1, 15, 17, 100, 127, 130, 250, 255])
 def test_gemm_sums_that_end_inside_a_piece(ops, k):
@@ -186,15 +195,23 @@ def test_gradients_in_k_ranges(ops, dtype):
 
 # The sizes above are taken from the operands as they are, most of these are laid out: the input's
 # gradient, the weights', or both.
+LAID_OUT = [(1301, 1203, 1501, 0, 0), (130, 4100, 133, 0, 0), (4100, 130, 133, 0, 0), (2050, 130, 1000, 3, 1),
+            (333, 5000, 129, 8, 8), (9, 30, 6, 0, 0), (30, 7, 70, 1, 1), (2701, 2203, 1301, 0, 0)]
+
+
 @pytest.mark.parametrize("dtype", list(TYPES))
-@pytest.mark.parametrize("m,n,k,pad,shift", [(1301, 1203, 1501, 0, 0), (130, 4100, 133, 0, 0), (4100, 130, 133, 0, 0),
-                                             (2050, 130, 1000, 3, 1), (333, 5000, 129, 8, 8), (9, 30, 6, 0, 0),
-                                             (30, 7, 70, 1, 1)])
+@pytest.mark.parametrize("m,n,k,pad,shift", LAID_OUT)
 def test_gradients_laid_out(ops, m, n, k, pad, shift, dtype):
     print(f"gradients {m}x{n}x{k} +{pad} {dtype}", flush=True)
-    t = TYPES[dtype]
-    assert any(Q.workspace_size(c, t, m, n, k) for c in (Q.CALL_GRAD_INPUT, Q.CALL_GRAD_WEIGHT))
     _gradients(ops, m, n, k, dtype, pad, shift)
+
+
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("call", [Q.CALL_GRAD_INPUT, Q.CALL_GRAD_WEIGHT])
+def test_sizes_reach_both_routes(call, dtype):
+    needs = [Q.workspace_size(call, TYPES[dtype], m, n, k) for m, n, k, _, _ in LAID_OUT]
+    assert sum(need > 0 for need in needs) >= 3
+    assert Q.workspace_size(call, TYPES[dtype], 64, 64, 64) == 0
 
 
 @pytest.mark.parametrize("dtype,out", [("bf16", "f32"), ("f16", "f32"), ("bf16", "bf16"), ("f16", "f16"), ("f32", "f32")])
