@@ -35,6 +35,10 @@ struct ProductPlan {
 
 constexpr uint64_t div_up(uint64_t a, uint64_t b) { return (a + b - 1) / b; }
 
+// The next column, after c < cols, of a thread that takes one of every `step`; `cols` after its last.  (A
+// plain sum of 32 bits passes 2^32 in the widest rows, starts again below `cols` and never ends.)
+constexpr uint32_t next_column(uint32_t c, uint32_t step, uint32_t cols) { return cols - c > step ? c + step : cols; }
+
 // Microseconds of `groups` work-groups of `tiles_k` K tiles each on a kernel, fitted to launches
 // back to back: a K tile's time and a fixed one for each round of work-groups.  The large
 // tiles take 1.47 us a K tile whether one or all CUs have one (4096^3 in 8-bit integers: 59

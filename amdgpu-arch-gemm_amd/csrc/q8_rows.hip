@@ -11,6 +11,7 @@
 // of more than the registers hold, have kernels that go by elements at the end and read twice.
 #include "q8_device.hpp"
 #include "q8_internal.hpp"
+#include "q8_plan.hpp"
 
 namespace q8 {
 namespace {
@@ -194,7 +195,7 @@ __global__ void __launch_bounds__(G < 256 ? 256 : G) quantize_any_kernel(const Q
                 for (int e = 0; e < 8; ++e) v[e] *= g[e];
             }
         };
-        for (uint32_t c = lane * 8; on && c < p.cols; c += G * 8) {
+        for (uint32_t c = lane * 8; on && c < p.cols; c = next_column(c, G * 8, p.cols)) {
             float v[8];
             first(c, v);
             if constexpr (NORM) {
@@ -218,7 +219,7 @@ __global__ void __launch_bounds__(G < 256 ? 256 : G) quantize_any_kernel(const Q
             if (NORM && p.rstd) p.rstd[row] = rstd;
         }
         int8_t* q = p.q + row * p.ldq;
-        for (uint32_t c = lane * 8; on && c < p.cols; c += G * 8) {
+        for (uint32_t c = lane * 8; on && c < p.cols; c = next_column(c, G * 8, p.cols)) {
             float v[8];
             if (hid) load_part<DT>(hid, c, p.cols, v);   // x may be gone: hidden may be x itself
             else first(c, v);
@@ -248,7 +249,7 @@ __global__ void __launch_bounds__(G < 256 ? 256 : G) dequantize_kernel(const Deq
             if (lane < p.cols) Type<DT>::put(y + lane, (float)q[lane] * s);
             continue;
         }
-        for (uint32_t n = lane * 8; n < p.cols; n += G * 8) {
+        for (uint32_t n = lane * 8; n < p.cols; n = next_column(n, G * 8, p.cols)) {
             const uint32_t c = min(n, p.cols - 8);
             float v[8];
             const u32x2 w = *reinterpret_cast<const u32x2_at1*>(q + c);
@@ -363,7 +364,7 @@ template <int DT, int G> __global__ void __launch_bounds__(G) norm_backward_any_
             }
         };
         // the column sums stay in the partial row, each entry its own thread's
-        for (uint32_t c = lane * 8; c < p.cols; c += G * 8) {
+        for (uint32_t c = lane * 8; c < p.cols; c = next_column(c, G * 8, p.cols)) {
             float u[8], xh[8], a[8] = {};
             if (part && row != blockIdx.x) load_part<Q8_F32>(part, c, p.cols, a);
             first(c, u, xh, a);
@@ -372,7 +373,7 @@ template <int DT, int G> __global__ void __launch_bounds__(G) norm_backward_any_
             if (part) store_part<Q8_F32>(part, c, p.cols, a);
         }
         row_sum_max<G, G>(sum, none, redf, redu, set);
-        for (uint32_t c = lane * 8; c < p.cols; c += G * 8) {
+        for (uint32_t c = lane * 8; c < p.cols; c = next_column(c, G * 8, p.cols)) {
             float u[8], xh[8], a[8] = {}, d[8] = {};
             first(c, u, xh, a);
             if (res) load_part<DT>(res, c, p.cols, d);

@@ -1,0 +1,91 @@
+"""The 8-bit operators at the ends of their range."""
+import numpy as np
+import pytest
+
+from shim import q8_shim as Q
+from shim import sgemm_shim as S
+
+pytestmark = pytest.mark.gpu
+
+WIDEST = 2 ** 32 - 1
+
+
+@pytest.fixture(scope="module")
+def ops():
+    with Q.Ops() as o:
+        yield o
+
+
+class Wide:
+    """A long device array, all bytes alike at first."""
+
+    def __init__(self, count, kind, byte):
+        self.kind = kind
+        self.buffer = S.DeviceBuffer(count * np.dtype(kind).itemsize)
+        self.ptr = self.buffer.ptr
+        S._check("sgemm_memset", S.load_library().sgemm_memset(self.ptr, byte, self.buffer.nbytes))
+
+    def _at(self, i):
+        return self.ptr + i * np.dtype(self.kind).itemsize
+
+    def put(self, i, values):
+        v = np.ascontiguousarray(values, dtype=self.kind)
+        S._check("sgemm_memcpy_h2d", S.load_library().sgemm_memcpy_h2d(self._at(i), v.ctypes.data, v.nbytes))
+
+    def get(self, i, count):
+        v = np.empty(count, self.kind)
+        S._check("sgemm_memcpy_d2h", S.load_library().sgemm_memcpy_d2h(v.ctypes.data, self._at(i), v.nbytes))
+        return v
+
+    def close(self):
+        self.buffer.close()
+
+
+@pytest.fixture
+def wide():
+    made = []
+
+    def make(*args):
+        made.append(Wide(*args))
+        return made[-1]
+
+    yield make
+    for w in made:
+        w.close()
+
+
+# columns past 2^31 and the last ones, where a counter of 32 bits passes 2^32
+PLACES = [0, 2 ** 31 - 4, 2 ** 32 - 8200, 2 ** 32 - 2056]
+
+
+def test_widest_row_quantized(ops, wide):
+    x, q, s = wide(WIDEST, np.uint16, 0x3C), wide(WIDEST, np.int8, 0x55), Q.Array(1, 1, Q.F32)
+    small = float(Q.from_bf16(np.array([0x3C3C], np.uint16))[0])
+    x.put(WIDEST - 3, Q.to_bf16(np.array([4 * small, -4 * small, small], np.float32)))
+    ops.quantize(Q.BF16, x, q, s, 1, WIDEST)
+    ops.synchronize()
+    assert abs(s.numpy()[0, 0] * 127 / (4 * small) - 1) <= 2.0 ** -22
+    for at in PLACES:
+        assert np.all(q.get(at, 8) == 32)       # 127 / 4 = 31.75
+    assert np.array_equal(q.get(WIDEST - 5, 5), [32, 32, 127, -127, 32])
+
+
+def test_widest_row_restored(ops, wide):
+    q, y, s = wide(WIDEST, np.int8, 1), wide(WIDEST, np.float16, 0x55), Q.Array.of(np.array([0.5]))
+    q.put(WIDEST - 2, [-3, 5])
+    ops.dequantize(Q.F16, q, s, y, 1, WIDEST)
+    ops.synchronize()
+    for at in PLACES:
+        assert np.all(y.get(at, 8) == 0.5)
+    assert np.array_equal(y.get(WIDEST - 4, 4), [0.5, 0.5, -1.5, 2.5])
+
+
+def test_widest_row_of_the_norm_backward(ops, wide):
+    # dn, hidden and gain may be one and the same: u = v^2, xhat = v, and the mean of u xhat moves dx by 1e-4 of it
+    v, dx, rstd = wide(WIDEST, np.uint16, 0x3C), wide(WIDEST, np.uint16, 0x55), Q.Array.of(np.array([1.0]))
+    x = float(Q.from_bf16(np.array([0x3C3C], np.uint16))[0])
+    ops.rmsnorm_backward(Q.BF16, v, v, v, rstd, None, dx, None, 1, WIDEST)
+    ops.synchronize()
+    for at in PLACES + [WIDEST - 8]:
+        got = Q.from_bf16(dx.get(at, 8))
+        assert np.all(np.abs(got - (x ** 2 - x ** 4)) <= 2.0 ** -7 * x ** 2)
