@@ -89,3 +89,24 @@ def test_widest_row_of_the_norm_backward(ops, wide):
     for at in PLACES + [WIDEST - 8]:
         got = Q.from_bf16(dx.get(at, 8))
         assert np.all(np.abs(got - (x ** 2 - x ** 4)) <= 2.0 ** -7 * x ** 2)
+
+
+@pytest.mark.parametrize("cols", [2 ** 20 * 32 + 40, 2 ** 27 + 5])
+def test_gains_gradient_of_wide_rows(ops, wide, cols):
+    """More columns than the work-groups of a launch sum at once, and than a launch has work-items for; dx in place of dn."""
+    rows = 2
+    dn, hidden, gain = (wide(n * cols, np.float16, b) for n, b in ((rows, 0x3C), (rows, 0x3A), (1, 0x3B)))
+    dgain, rstd = wide(cols, np.float32, 0x55), Q.Array.of(np.array([1.0, 0.5]))
+    d, h, g = (float(np.array([b * 257], np.uint16).view(np.float16)[0]) for b in (0x3C, 0x3A, 0x3B))
+    dn.put(cols - 1, [2 * d])        # the first row's last column
+    ops.rmsnorm_backward(Q.F16, dn, hidden, gain, rstd, None, dn, dgain, rows, cols)
+    ops.synchronize()
+    for at in (0, 31, 2 ** 25 - 8, cols - 50, cols - 9):
+        assert np.allclose(dgain.get(at, 8), d * h * 1.5, rtol=2.0 ** -20, atol=0)
+    assert np.allclose(dgain.get(cols - 1, 1), d * h * 2.5, rtol=2.0 ** -20, atol=0)
+    # u - xhat mean(u xhat): a thread adds up to 131072 like terms in a row, within 131072 x 2^-24 = 0.8% of their sum,
+    # of which xhat takes less than one; and a rounding to 2^-11
+    for row, r in ((0, 1.0), (1, 0.5)):
+        want = r * d * g * (1 - (h * r) ** 2)
+        got = dn.get(row * cols + cols // 2, 8).astype(np.float64)
+        assert np.all(np.abs(got - want) <= 2e-2 * abs(r * d * g)), (got, want)
