@@ -12,6 +12,9 @@ constexpr uint32_t kTileBytes = 128;         // of the summed index, a K tile
 constexpr uint32_t kMaxSplits = 16;
 // A tile's rows are addressed with 32-bit offsets from its first one.
 constexpr uint64_t kMaxRowBytes = 1u << 22;
+// The longest sum of a gradient whose operands are laid out, of 16-bit values in `terms` terms each: a
+// row holds a multiple of eight values.
+constexpr uint64_t most_summed(uint32_t terms) { return kMaxRowBytes / (2 * terms) / 8 * 8; }
 // Up to so many tokens the weights are streamed once, from rows that start anywhere.
 constexpr uint32_t kFewTokens = 64;
 // So many scales are looked through by every work-group that needs their largest, which costs

@@ -167,9 +167,9 @@ int plan_grad(int dtype, bool turned, bool odd, uint64_t rows, uint64_t cols, ui
     g.cp = round_up(sum, 8);
     g.terms = dtype == Q8_F32 ? 3 : 1;
     g.kb = g.cp * g.terms * 2;
-    if (g.kb > kMaxRowBytes)
+    if (sum > most_summed(g.terms))
         return fail(SGEMM_E_SHAPE, "a sum over %llu products is too long: at most %llu", (unsigned long long)sum,
-                    (unsigned long long)(kMaxRowBytes / (2 * g.terms)));
+                    (unsigned long long)most_summed(g.terms));
     // whole lines, and not a multiple of 4096 bytes (F16, 4096 x 4096 x 16384: 396 us as it is, 386 with 512
     // bytes more; 1024 x 1024 x 16384 in four ranges: 46 and 47, but 60 with 128)
     g.pitch = round_up(g.kb, 128);

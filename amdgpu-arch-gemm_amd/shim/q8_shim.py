@@ -18,6 +18,7 @@ from . import sgemm_shim as S
 F32, F16, BF16 = 0, 1, 2
 CALL_RMSNORM_BACKWARD, CALL_GEMM, CALL_GRAD_INPUT, CALL_GRAD_WEIGHT = 0, 1, 2, 3
 MAX_K = 131071
+MAX_SUM, MAX_SUM_F32 = 2097152, 699048    # longest sums of the gradients, with 16-bit types and with F32
 
 _int, _u32, _f32, _vp, _size = ctypes.c_int, ctypes.c_uint32, ctypes.c_float, ctypes.c_void_p, ctypes.c_size_t
 

@@ -65,6 +65,11 @@ enum {
 
 /* Longest sum of q8_gemm: 131071 products of -128 * -128 fit 32 bits. */
 #define Q8_MAX_K 131071u
+/* Longest sums of the gradients (n of q8_grad_input, m of q8_grad_weight), with 16-bit types and with Q8_F32:
+ * an operand's row laid out for the matrix cores ends at 2^22 bytes.  A longer one is refused with SGEMM_E_SHAPE;
+ * q8_grad_weight can add the parts of one with `accumulate`. */
+#define Q8_MAX_SUM 2097152u
+#define Q8_MAX_SUM_F32 699048u
 
 typedef struct q8_handle q8_handle;
 

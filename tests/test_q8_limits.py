@@ -1,6 +1,12 @@
 """Index arithmetic of the 8-bit operators at the ends of their range, on the CPU."""
 import os
+import re
 import subprocess
+
+import pytest
+
+from shim import q8_shim as Q
+from shim import sgemm_shim as S
 
 ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 
@@ -36,3 +42,22 @@ int main() {
     std::puts("ok");
 }
 """)
+
+
+@pytest.mark.parametrize("call", [Q.CALL_GRAD_INPUT, Q.CALL_GRAD_WEIGHT])
+@pytest.mark.parametrize("dtype,most", [(Q.F32, Q.MAX_SUM_F32), (Q.F16, Q.MAX_SUM), (Q.BF16, Q.MAX_SUM)])
+def test_longest_sums_of_the_gradients(call, dtype, most):
+    """The longest sum is taken, the next one refused with a message that says which is the longest."""
+    def size(summed):
+        return Q.workspace_size(call, dtype, *((200, summed, 200) if call == Q.CALL_GRAD_INPUT else (summed, 200, 200)))
+
+    assert size(most) > 0
+    with pytest.raises(S.SgemmError) as e:
+        size(most + 1)
+    assert e.value.code == -4 and f"at most {most}" in e.value.message
+
+
+def test_longest_sums_match_the_header():
+    text = open(os.path.join(ROOT, "include", "q8_shim.h")).read()
+    values = {k: int(v) for k, v in re.findall(r"#define (Q8_MAX_\w+) (\d+)u", text)}
+    assert values == {"Q8_MAX_K": Q.MAX_K, "Q8_MAX_SUM": Q.MAX_SUM, "Q8_MAX_SUM_F32": Q.MAX_SUM_F32}
