@@ -258,4 +258,9 @@ hipError_t launch_gradient(int dtype, bool turned, const Gradient& p, hipStream_
                              : gradient_any<Q8_BF16>(turned, p, s);
 }
 
+hipError_t prepare_gradients() {
+    hipFuncAttributes a;
+    return hipFuncGetAttributes(&a, reinterpret_cast<const void*>(&gradient_kernel<Q8_BF16, false, 4, false>));
+}
+
 }  // namespace q8

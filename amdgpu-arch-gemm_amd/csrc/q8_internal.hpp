@@ -87,7 +87,11 @@ struct Route {
 };
 Q8_INTERNAL hipError_t launch_product(Element e, const Route& r, const Product& p, hipStream_t stream);
 Q8_INTERNAL hipError_t launch_direct(const Product& p, hipStream_t stream);   // E_I8, rows that start anywhere
-Q8_INTERNAL hipError_t prepare_products();   // loads the kernels on the current device
+// Each kernel source is a code object of its own, which its prepare function loads on the current device.
+Q8_INTERNAL hipError_t prepare_products();
+Q8_INTERNAL hipError_t prepare_rows();
+Q8_INTERNAL hipError_t prepare_packing();
+Q8_INTERNAL hipError_t prepare_gradients();
 
 // 8-bit rows to rows of whole 16 bytes: dst[r][0 .. cols) and zeros up to dst_ld.
 Q8_INTERNAL hipError_t launch_copy_rows(const int8_t* src, uint64_t src_ld, int8_t* dst, uint64_t dst_ld, uint32_t rows,

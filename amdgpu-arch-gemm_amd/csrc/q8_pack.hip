@@ -329,4 +329,9 @@ hipError_t launch_pack(int dtype, const PackWeights& w, const PackGradient* g, h
     return dtype == Q8_F32 ? pack_any<Q8_F32>(p, s) : dtype == Q8_F16 ? pack_any<Q8_F16>(p, s) : pack_any<Q8_BF16>(p, s);
 }
 
+hipError_t prepare_packing() {
+    hipFuncAttributes a;
+    return hipFuncGetAttributes(&a, reinterpret_cast<const void*>(&copy_rows_kernel));
+}
+
 }  // namespace q8

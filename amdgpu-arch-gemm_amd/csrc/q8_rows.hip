@@ -504,4 +504,9 @@ hipError_t launch_norm_backward(int dtype, const NormBackward& p, hipStream_t s)
     return hipLaunchKernel(reinterpret_cast<const void*>(&column_sum_kernel), dim3(groups_for(cols, 32)), dim3(1024), args, 0, s);
 }
 
+hipError_t prepare_rows() {
+    hipFuncAttributes a;
+    return hipFuncGetAttributes(&a, reinterpret_cast<const void*>(&column_sum_kernel));
+}
+
 }  // namespace q8

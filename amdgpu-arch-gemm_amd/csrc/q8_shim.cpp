@@ -242,7 +242,11 @@ int q8_open(q8_handle** out) {
     if (!h) return fail(SGEMM_E_INVALID, "out of host memory");
     hipError_t e = hipGetDevice(&h->device);
     if (e == hipSuccess) e = hipStreamCreate(&h->own_stream);
+    // no call loads code: a first one may be under capture, and should not take longer than the next
+    if (e == hipSuccess) e = prepare_rows();
+    if (e == hipSuccess) e = prepare_packing();
     if (e == hipSuccess) e = prepare_products();
+    if (e == hipSuccess) e = prepare_gradients();
     if (e != hipSuccess) {
         if (h->own_stream) (void)hipStreamDestroy(h->own_stream);
         delete h;
