@@ -508,11 +508,9 @@ template <int E, int DT> hipError_t product_any(const Route& r, Product p, hipSt
     p.rows = p.nwgx * t.m;
     p.pitch = p.nwgy * t.n;
     const uint32_t tiles_k = (uint32_t)ceil_div(p.kb, KB);
-    p.tiles_per_split = (uint32_t)ceil_div(tiles_k, r.splits);
+    p.tiles_per_split = (uint32_t)tiles_per_split(p.kb, r.splits);
     p.splits = tiles_k ? (uint32_t)ceil_div(tiles_k, p.tiles_per_split) : 1;    // none is empty
-    // A second round of work-groups finds its lines in memory, and in a deep K they drift apart;
-    // one round of few K tiles is 2% faster unasked.
-    const bool ahead = (uint64_t)p.nwgx * p.nwgy * p.splits > kComputeUnits || p.tiles_per_split > 32;
+    const bool ahead = asks_ahead((uint64_t)p.nwgx * p.nwgy * p.splits, p.tiles_per_split);
     const void* f = r.kind == K_SMALL        ? (const void*)&product_kernel<E, DT, 4, 2, false>
                     : r.kind == K_SMALL_DEEP ? (const void*)&product_kernel<E, DT, 4, 3, false>
                     : ahead                  ? (const void*)&product_kernel<E, DT, 8, 2, true>

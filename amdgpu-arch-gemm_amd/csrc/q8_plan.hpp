@@ -86,6 +86,11 @@ inline ProductPlan plan_product(uint64_t m, uint64_t n, uint64_t kb) {
     return best;
 }
 
+// K tiles of a work-group, and whether it asks L2 for the next ones' lines (256 x 256 tiles): a second round of work-groups
+// finds its lines in memory, and in a deep K they drift apart; one round of few K tiles is 2% faster unasked.
+constexpr uint64_t tiles_per_split(uint64_t kb, uint32_t splits) { return div_up(div_up(kb, kTileBytes), splits); }
+constexpr bool asks_ahead(uint64_t groups, uint64_t tiles) { return groups > kComputeUnits || tiles > 32; }
+
 // The direct kernel's tiles, 16 MT tokens x 16 NT channels a work-group of WAVES waves:
 //   1 x 1, 16 waves  a small product: a work-group a CU (333 x 129 x 517: 4.2 us, 2 x 1 5.2)
 //   1 x 1, 8 waves   up to 16 tokens (16 x 4096 x 4096: 6.9 us; 16 waves 7.2), and 16 waves over
@@ -158,6 +163,75 @@ inline bool gradient_direct(bool turned, bool f32, bool f16, bool odd, uint64_t 
     // 2^32 work-items are one grid's end
     if (rows > (1u << 22) || gradient_groups(turned, rows, cols) >= (1u << 22)) return false;
     return 1.05 * gradient_time(turned, f32, odd, rows, cols, sum) < tile_time + 3.0 + (double)packed_bytes / 3e6;
+}
+
+constexpr uint64_t round_up(uint64_t x, uint64_t to) { return (x + to - 1) / to * to; }
+
+// A call's parts of the workspace, one after the other.
+struct Layout {
+    size_t a = 0, b = 0, pair = 0, partial = 0, total = 0;
+    void add(size_t& at, size_t bytes) {
+        at = total;
+        total += piece(bytes);
+    }
+    static constexpr size_t piece(size_t bytes) { return (bytes + 255) & ~(size_t)255; }
+};
+
+// How an 8-bit product runs: on the direct kernel, or on tiles, of rows that are copied first where copy_a
+// and copy_b say so.
+struct GemmPlan {
+    bool direct = false, copy_a = false, copy_b = false;
+    uint64_t ldc = 0;   // bytes of a copied row
+    ProductPlan plan;
+    Layout at;
+};
+inline GemmPlan plan_gemm(uint64_t m, uint64_t n, uint64_t k, bool copy_a, bool copy_b) {
+    GemmPlan g;
+    g.ldc = round_up(k, 16);
+    g.plan = plan_product(m, n, k);
+    g.direct = m <= kFewTokens || direct_for_many(m, n, k, g.plan.time, (int)copy_a + (int)copy_b,
+                                                  (copy_a ? m * g.ldc : 0) + (copy_b ? n * g.ldc : 0));
+    if (g.direct) return g;
+    g.copy_a = copy_a;
+    g.copy_b = copy_b;
+    if (copy_a) g.at.add(g.at.a, m * g.ldc);
+    if (copy_b) g.at.add(g.at.b, n * g.ldc);
+    if (g.plan.partial_bytes) g.at.add(g.at.partial, g.plan.partial_bytes);
+    return g;
+}
+
+// How the gradient D (rows x cols) summed over `sum` runs.
+struct GradPlan {
+    bool direct = false;    // from the operands as they are; else:
+    uint64_t cp = 0;        // values of the summed index in a laid-out row
+    uint32_t terms = 1;
+    uint64_t kb = 0;        // its bytes
+    uint64_t pitch = 0;     // and those from one row to the next
+    ProductPlan plan;
+    Layout at;
+};
+constexpr uint32_t grad_terms(bool f32) { return f32 ? 3 : 1; }
+// copy_a: the 16-bit operand would be laid out too, turned: it has the summed index from row to row, odd: its
+// rows start between dwords.  sum <= most_summed(terms).
+inline GradPlan plan_grad(bool f32, bool f16, bool turned, bool odd, uint64_t rows, uint64_t cols, uint64_t sum, bool copy_a) {
+    GradPlan g;
+    g.cp = round_up(sum, 8);
+    g.terms = grad_terms(f32);
+    g.kb = g.cp * g.terms * 2;
+    // whole lines, and not a multiple of 4096 bytes (F16, 4096 x 4096 x 16384: 396 us as it is, 386 with 512
+    // bytes more; 1024 x 1024 x 16384 in four ranges: 46 and 47, but 60 with 128)
+    g.pitch = round_up(g.kb, 128);
+    if (g.pitch % 4096 == 0) g.pitch += 512;
+    g.plan = plan_product(rows, cols, g.kb);
+    copy_a = copy_a || f32;
+    const uint64_t bytes = cols * (sum + g.kb) + (copy_a ? rows * (sum * (f32 ? 4 : 2) + g.kb) : 0);
+    g.direct = gradient_direct(turned, f32, f16, odd, rows, cols, sum, g.plan.time, bytes);
+    if (g.direct) return g;
+    if (copy_a) g.at.add(g.at.a, rows * g.pitch);
+    g.at.add(g.at.b, cols * g.pitch);
+    if (f16) g.at.add(g.at.pair, 8);
+    if (g.plan.partial_bytes) g.at.add(g.at.partial, g.plan.partial_bytes);
+    return g;
 }
 
 }  // namespace q8

@@ -140,49 +140,14 @@ int take_workspace(q8_handle* h, size_t bytes) {
     return SGEMM_OK;
 }
 
-uint64_t round_up(uint64_t x, uint64_t to) { return (x + to - 1) / to * to; }
-size_t piece(size_t bytes) { return (bytes + 255) & ~(size_t)255; }
-
-// A call's parts of the workspace, one after the other.
-struct Layout {
-    size_t a = 0, b = 0, pair = 0, partial = 0, total = 0;
-    void add(size_t& at, size_t bytes) {
-        at = total;
-        total += piece(bytes);
-    }
-};
-
-struct Grad {
-    bool direct;        // from the operands as they are; else:
-    uint64_t cp;        // values of the summed index in a laid-out row
-    uint32_t terms;
-    uint64_t kb;        // its bytes
-    uint64_t pitch;     // and those from one row to the next
-    ProductPlan plan;
-    Layout at;
-};
-// The gradient D (rows x cols) summed over `sum`; copy_a: the 16-bit operand would be laid out too,
-// turned: it has the summed index from row to row, odd: its rows start between dwords.
-int plan_grad(int dtype, bool turned, bool odd, uint64_t rows, uint64_t cols, uint64_t sum, bool copy_a, Grad& g) {
-    g.cp = round_up(sum, 8);
-    g.terms = dtype == Q8_F32 ? 3 : 1;
-    g.kb = g.cp * g.terms * 2;
-    if (sum > most_summed(g.terms))
+// As plan_grad, refusing a sum that is too long.
+int plan(int dtype, bool turned, bool odd, uint64_t rows, uint64_t cols, uint64_t sum, bool copy_a, GradPlan& g) {
+    const bool f32 = dtype == Q8_F32;
+    const uint64_t most = most_summed(grad_terms(f32));
+    if (sum > most)
         return fail(SGEMM_E_SHAPE, "a sum over %llu products is too long: at most %llu", (unsigned long long)sum,
-                    (unsigned long long)most_summed(g.terms));
-    // whole lines, and not a multiple of 4096 bytes (F16, 4096 x 4096 x 16384: 396 us as it is, 386 with 512
-    // bytes more; 1024 x 1024 x 16384 in four ranges: 46 and 47, but 60 with 128)
-    g.pitch = round_up(g.kb, 128);
-    if (g.pitch % 4096 == 0) g.pitch += 512;
-    g.plan = plan_product(rows, cols, g.kb);
-    g.at = Layout();
-    const uint64_t bytes = cols * (sum + g.kb) + (copy_a || dtype == Q8_F32 ? rows * (sum * type_bytes(dtype) + g.kb) : 0);
-    g.direct = gradient_direct(turned, dtype == Q8_F32, dtype == Q8_F16, odd, rows, cols, sum, g.plan.time, bytes);
-    if (g.direct) return SGEMM_OK;
-    if (copy_a || dtype == Q8_F32) g.at.add(g.at.a, rows * g.pitch);
-    g.at.add(g.at.b, cols * g.pitch);
-    if (dtype == Q8_F16) g.at.add(g.at.pair, 8);
-    if (g.plan.partial_bytes) g.at.add(g.at.partial, g.plan.partial_bytes);
+                    (unsigned long long)most);
+    g = plan_grad(f32, dtype == Q8_F16, turned, odd, rows, cols, sum, copy_a);
     return SGEMM_OK;
 }
 
@@ -193,27 +158,6 @@ int check_grid(uint64_t m, uint64_t n, const ProductPlan& p) {
         return fail(SGEMM_E_SHAPE, "%llu x %llu outputs are more tiles than a grid holds", (unsigned long long)m,
                     (unsigned long long)n);
     return SGEMM_OK;
-}
-
-struct GemmPlan {
-    bool direct = false, copy_a = false, copy_b = false;
-    uint64_t ldc = 0;   // bytes of a copied row
-    ProductPlan plan;
-    Layout at;
-};
-GemmPlan plan_gemm(uint64_t m, uint64_t n, uint64_t k, bool copy_a, bool copy_b) {
-    GemmPlan g;
-    g.ldc = round_up(k, 16);
-    g.plan = plan_product(m, n, k);
-    g.direct = m <= kFewTokens || direct_for_many(m, n, k, g.plan.time, (int)copy_a + (int)copy_b,
-                                                  (copy_a ? m * g.ldc : 0) + (copy_b ? n * g.ldc : 0));
-    if (g.direct) return g;
-    g.copy_a = copy_a;
-    g.copy_b = copy_b;
-    if (copy_a) g.at.add(g.at.a, m * g.ldc);
-    if (copy_b) g.at.add(g.at.b, n * g.ldc);
-    if (g.plan.partial_bytes) g.at.add(g.at.partial, g.plan.partial_bytes);
-    return g;
 }
 
 bool rows_aligned(const void* p, uint64_t ld_bytes) {
@@ -308,7 +252,7 @@ int q8_workspace_size(int call, int dtype, uint32_t m, uint32_t n, uint32_t k, s
     *bytes = 0;
     CHECK(check_type(dtype));
     if (call == Q8_CALL_RMSNORM_BACKWARD) {
-        *bytes = piece((size_t)norm_backward_parts(m) * k * sizeof(float));
+        *bytes = Layout::piece((size_t)norm_backward_parts(m) * k * sizeof(float));
     } else if (call == Q8_CALL_GEMM) {
         for (int copies = 0; copies < 4; ++copies) {    // the route depends on them
             const size_t need = plan_gemm(m, n, k, copies & 1, copies & 2).at.total;
@@ -316,9 +260,9 @@ int q8_workspace_size(int call, int dtype, uint32_t m, uint32_t n, uint32_t k, s
         }
     } else if (call == Q8_CALL_GRAD_INPUT || call == Q8_CALL_GRAD_WEIGHT) {
         for (int i = 0; i < 4; ++i) {   // the route depends on dy's rows
-            Grad g;
-            if (call == Q8_CALL_GRAD_INPUT) CHECK(plan_grad(dtype, false, i & 2, m, k, n, i & 1, g));
-            else CHECK(plan_grad(dtype, true, i & 2, n, k, m, true, g));
+            GradPlan g;
+            if (call == Q8_CALL_GRAD_INPUT) CHECK(plan(dtype, false, i & 2, m, k, n, i & 1, g));
+            else CHECK(plan(dtype, true, i & 2, n, k, m, true, g));
             if (g.at.total > *bytes) *bytes = g.at.total;
         }
     } else {
@@ -468,8 +412,8 @@ int q8_grad_input(q8_handle* h, int dtype, const void* dy, uint32_t lddy, const 
     const Span out{"dx", dx, m, k, lddx, size};
     // dy's rows hold the summed index: read where they are if they are whole pieces
     const bool copy = dtype == Q8_F32 || n % 8 || !rows_aligned(dy, (uint64_t)lddy * size);
-    Grad g;
-    CHECK(plan_grad(dtype, false, odd_rows(dy, (uint64_t)lddy * size), m, k, n, copy, g));
+    GradPlan g;
+    CHECK(plan(dtype, false, odd_rows(dy, (uint64_t)lddy * size), m, k, n, copy, g));
     if (!g.direct) CHECK(check_grid(m, k, g.plan));
     for (const Span& s : in) CHECK(check(s));
     CHECK(check(out));
@@ -514,8 +458,8 @@ int q8_grad_weight(q8_handle* h, int dtype, const void* dy, uint32_t lddy, const
     const uint32_t size = type_bytes(dtype);
     const Span in[] = {{"dy", dy, m, n, lddy, size}, {"qx", qx, m, k, ldx, 1}, vec("sx", sx, m, 4)};
     const Span out{"dw", dw, n, k, lddw, type_bytes(out_dtype)};
-    Grad g;
-    CHECK(plan_grad(dtype, true, odd_rows(dy, (uint64_t)lddy * size), n, k, m, true, g));
+    GradPlan g;
+    CHECK(plan(dtype, true, odd_rows(dy, (uint64_t)lddy * size), n, k, m, true, g));
     if (!g.direct) CHECK(check_grid(n, k, g.plan));
     for (const Span& s : in) CHECK(check(s));
     CHECK(check(out));

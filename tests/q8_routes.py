@@ -1,0 +1,96 @@
+"""Which kernels the 8-bit operators' products run on, as csrc/q8_plan.hpp decides, and the sizes that tests take
+for each of them."""
+import functools
+import os
+import subprocess
+import tempfile
+
+CSRC = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "amdgpu-arch-gemm_amd", "csrc")
+
+PROGRAM = r"""
+#include "q8_plan.hpp"
+#include <cstdio>
+using namespace q8;
+static void tiles(const ProductPlan& p, uint64_t m, uint64_t n, uint64_t kb) {
+    const Tile& t = kTiles[p.kind];
+    const uint64_t per = tiles_per_split(kb, p.splits), groups = div_up(m, t.m) * div_up(n, t.n) * p.splits;
+    std::printf("%s %s", p.kind == K_LARGE ? asks_ahead(groups, per) ? "large-ahead" : "large" : p.kind == K_SMALL ? "small" : "deep",
+                p.splits > 1 ? "ranges" : "whole");
+}
+int main() {
+    char what[16];
+    unsigned long long m, n, k;
+    int a, b, c, d;
+    // gemm m n k copy_a copy_b - -;  grad rows cols sum f32 f16 turned odd+2*copy
+    while (std::scanf("%15s %llu %llu %llu %d %d %d %d", what, &m, &n, &k, &a, &b, &c, &d) == 8) {
+        if (what[1] == 'e') {
+            const GemmPlan g = plan_gemm(m, n, k, a, b);
+            if (g.direct) std::printf("direct %d", (int)direct_kind(m, n, k));
+            else tiles(g.plan, m, n, k), std::printf(" copies-%d", g.copy_a + 2 * g.copy_b);
+        } else {
+            const GradPlan g = plan_grad(a, b, c, d & 1, m, n, k, d & 2);
+            if (g.direct) std::printf("direct waves-%u", gradient_waves(c, a, m, n, k));
+            else tiles(g.plan, m, n, g.kb), std::printf(" copies-%d", (int)(a || d & 2));
+        }
+        std::puts("");
+    }
+}
+"""
+
+
+@functools.lru_cache(maxsize=1)
+def _program():
+    folder = tempfile.mkdtemp(prefix="q8_routes")
+    source, program = os.path.join(folder, "routes.cpp"), os.path.join(folder, "routes")
+    with open(source, "w") as f:
+        f.write(PROGRAM)
+    subprocess.run(["g++", "-std=c++17", "-O1", "-Wall", "-Werror", "-I", CSRC, source, "-o", program], check=True)
+    return program
+
+
+def _ask(lines):
+    out = subprocess.run([_program()], input="\n".join(" ".join(str(int(x)) if not isinstance(x, str) else x for x in l)
+                                                       for l in lines) + "\n", capture_output=True, text=True, check=True)
+    return [tuple(l.split()) for l in out.stdout.splitlines()]
+
+
+def gemm_route(m, n, k, ld, shift):
+    """The route of an 8-bit product whose operands start `shift` bytes past a multiple of 16, in rows of ld bytes."""
+    copy = shift % 16 != 0 or ld % 16 != 0 or ld > 1 << 22
+    return _ask([("gemm", m, n, k, copy or k % 16 != 0, copy, 0, 0)])[0]
+
+
+def grad_routes(m, n, k, dtype, lddy, shift):
+    """The routes of the input's and the weights' gradients; dy starts `shift` values past a multiple of 16 bytes."""
+    size = 4 if dtype == "f32" else 2
+    odd = (shift | lddy) * size % 4 != 0
+    copy = n % 8 != 0 or shift * size % 16 != 0 or lddy * size % 16 != 0 or lddy * size > 1 << 22
+    kinds = dtype == "f32", dtype == "f16"
+    return _ask([("grad", m, k, n, *kinds, 0, odd + 2 * copy), ("grad", n, k, m, *kinds, 1, odd + 2)])
+
+
+# m, n, k, values between rows (of all operands and the result), bytes (values) that they start after a multiple of 16
+GEMMS = [(4001, 3905, 336, 0, 0), (4000, 3900, 200, 8, 0), (4000, 3901, 203, 2, 3),
+         (3999, 3990, 4301, 0, 0), (8100, 4090, 592, 0, 0), (8000, 4000, 600, 8, 0),
+         (1000, 999, 1008, 0, 0), (1000, 1001, 999, 9, 0), (2000, 1000, 1000, 3, 1),
+         (300, 4000, 2000, 0, 0), (16000, 100, 2005, 11, 0), (1500, 1500, 2050, 3, 5),
+         (1100, 128, 4096, 0, 0), (200, 4100, 4090, 6, 0), (130, 4000, 4000, 0, 1),
+         (1000, 1000, 8192, 0, 0), (1003, 997, 8190, 2, 0), (1000, 1000, 8191, 1, 2), (4300, 1000, 16384, 0, 0)]
+GEMM_ROUTES = {(kind, "whole", copies) for kind in ("large", "large-ahead", "small", "deep")
+               for copies in ("copies-0", "copies-1", "copies-3")}
+GEMM_ROUTES |= {(kind, "ranges", copies) for kind in ("small", "deep") for copies in ("copies-0", "copies-1", "copies-3")}
+GEMM_ROUTES |= {("large-ahead", "ranges", "copies-0")}
+
+GRADIENTS = [(1001, 40, 9003, 0, 0), (7, 1003, 9001, 0, 0), (3001, 5, 9003, 0, 0), (3000, 40, 9001, 0, 0), (5, 3001, 9003, 0, 0),
+             (3990, 200, 3901, 0, 0), (200, 3990, 3901, 2, 1), (1500, 1504, 1501, 0, 0), (1501, 1503, 1505, 1, 1),
+             (1500, 9000, 3001, 0, 0), (9001, 1503, 3001, 0, 0), (1501, 4000, 3001, 0, 0), (3001, 503, 9003, 0, 0),
+             (1000, 40, 4003, 0, 0), (300, 7, 301, 3, 1), (6, 8, 5, 0, 0),
+             (130, 4100, 133, 0, 0), (500, 8000, 501, 0, 0), (4100, 130, 133, 5, 3), (6, 6000, 4001, 0, 0), (4001, 6, 6003, 0, 0), (4001, 6000, 6, 0, 0),
+             (6, 1500, 5, 0, 0), (500, 6, 5, 0, 0), (64, 64, 64, 0, 0), (600, 530, 40, 0, 0), (40, 1000, 70, 0, 0)]
+
+
+def grad_wanted(dtype, turned):
+    """Routes of a gradient, without the copies."""
+    want = {(kind, "whole") for kind in ("large", "large-ahead", "small", "deep")}
+    want |= {(kind, "ranges") for kind in ("large-ahead", "small", "deep")}
+    return want | {("direct", "waves-4")} | (set() if turned and dtype == "f32" else {("direct", "waves-8")})
