@@ -20,3 +20,12 @@ def test_opening_a_handle_loads_every_code_object():
     for name in sources:
         defined = re.findall(r"^hipError_t (prepare_\w+)\(\) {", read(name), re.M)
         assert len(defined) == 1 and defined[0] in called, name
+
+
+def test_widths_of_the_row_tests_are_those_of_the_kernels():
+    from test_gpu_q8_widths import HELD, HELD_BACKWARD
+
+    text = read("q8_rows.hip")
+    for function, held in (("quantize_any", HELD), ("backward_any", HELD_BACKWARD)):
+        body = re.search(r"hipError_t %s\(.*?\n}\n" % function, text, re.S).group()
+        assert [int(n) for n in re.findall(r"pieces <= (\d+)\) return", body)] == held, function
