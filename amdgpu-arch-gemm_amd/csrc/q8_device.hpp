@@ -144,6 +144,21 @@ __device__ __forceinline__ void store_part(typename Type<DT>::T* row, uint32_t c
     }
 }
 
+// v = v sx sw + add for integer sums v.  A sum has 31 bits, so a token's scale from 2^96 on could take it past FP32's
+// range where the channel's brings it back: there the channel's comes first, and what passes the range then
+// is a result that does.
+template <int N>
+__device__ __forceinline__ void finish(float (&v)[N], float sx, const float (&sw)[N], const float (&add)[N]) {
+    const bool last = sx >= 0x1p96f;
+    if (__builtin_expect(__any(last), 0)) {
+#pragma unroll
+        for (int e = 0; e < N; ++e) v[e] = __builtin_fmaf(v[e] * (last ? sw[e] : sx), last ? sx : sw[e], add[e]);
+    } else {
+#pragma unroll
+        for (int e = 0; e < N; ++e) v[e] = __builtin_fmaf(v[e] * sx, sw[e], add[e]);
+    }
+}
+
 // |x| as an integer that orders like it, infinities and then NaN last.
 __device__ __forceinline__ uint32_t magnitude(float x) { return __builtin_bit_cast(uint32_t, x) & 0x7fffffffu; }
 

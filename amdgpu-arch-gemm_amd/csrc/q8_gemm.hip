@@ -307,10 +307,11 @@ __global__ void __launch_bounds__(256, T == 4 ? 2 : 1) product_kernel(const Prod
                 }
                 if (!on || row >= p.m) continue;
                 Out* y = (Out*)p.y + (uint64_t)row * p.ldy;
+                if constexpr (E == E_I8) {
+                    finish(v, sx[i][q], sw[h], bias[h]);
+                } else {
 #pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    v[e] *= E == E_I8 ? sx[i][q] : factor;
-                    if constexpr (E == E_I8) v[e] = __builtin_fmaf(v[e], sw[h][e], bias[h][e]);
+                    for (int e = 0; e < 8; ++e) v[e] *= factor;
                 }
                 if (E != E_I8 && p.accumulate) {
                     float old[8];
@@ -345,19 +346,18 @@ template <int E, int DT> __global__ void __launch_bounds__(256) finish_kernel(co
     float v[8];
 #pragma unroll
     for (int e = 0; e < 4; ++e) { v[e] = out_value(lo[e]); v[4 + e] = out_value(hi[e]); }
-    const float sx = E == E_I8 ? p.sx[row] : E == E_F16 && p.alpha ? p.alpha[1] : 1.0f;
     Out* y = (Out*)p.y + (uint64_t)row * p.ldy;
-    float add[8] = {}, sw[8];
+    float add[8] = {};
     if constexpr (E == E_I8) {
+        float sw[8];
         load_part<Q8_F32>(p.sw, col, p.n, sw);
         if (p.bias) load_part<DT>((const Out*)p.bias, col, p.n, add);
-    } else if (p.accumulate) {
-        load_part<DT>(y, col, p.n, add);
-    }
+        finish(v, p.sx[row], sw, add);
+    } else {
+        const float factor = E == E_F16 && p.alpha ? p.alpha[1] : 1.0f;
+        if (p.accumulate) load_part<DT>(y, col, p.n, add);
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-        v[e] *= sx;
-        v[e] = E == E_I8 ? __builtin_fmaf(v[e], sw[e], add[e]) : v[e] + add[e];
+        for (int e = 0; e < 8; ++e) v[e] = v[e] * factor + add[e];
     }
     store_part<DT>(y, col, p.n, v);
 }
@@ -490,9 +490,11 @@ __global__ void __launch_bounds__(WAVES * 64) direct_kernel(const Product p) {
         const uint32_t row = row0 + (uint32_t)(t / NT * 16 + fr), col = col0 + (uint32_t)(t % NT * 16 + fg * 4);
         if (row >= p.m) continue;
         Out* y = (Out*)p.y + row * p.ldy + col;
+        float r[4] = {(float)v[0], (float)v[1], (float)v[2], (float)v[3]};
+        finish(r, sx, sw, bias);
 #pragma unroll
         for (int e = 0; e < 4; ++e)
-            if (col + e < p.n) Type<DT>::put(y + e, __builtin_fmaf((float)v[e] * sx, sw[e], bias[e]));
+            if (col + e < p.n) Type<DT>::put(y + e, r[e]);
     }
 }
 

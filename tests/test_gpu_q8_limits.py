@@ -2,6 +2,7 @@
 import numpy as np
 import pytest
 
+from q8_reference import random_q
 from shim import q8_shim as Q
 from shim import sgemm_shim as S
 
@@ -110,3 +111,20 @@ def test_gains_gradient_of_wide_rows(ops, wide, cols):
         want = r * d * g * (1 - (h * r) ** 2)
         got = dn.get(row * cols + cols // 2, 8).astype(np.float64)
         assert np.all(np.abs(got - want) <= 2e-2 * abs(r * d * g)), (got, want)
+
+
+# the direct kernel, tiles that finish themselves (128 x 128, 256 x 256), and K ranges
+@pytest.mark.parametrize("m,n,k", [(3, 70, 200), (100, 90, 700), (1000, 999, 1008), (4001, 3905, 336), (1100, 128, 4096)])
+def test_scales_whose_product_is_in_range(ops, m, n, k):
+    """Sum times one scale passes FP32's range, the other scale brings it back; beside them ordinary tokens.  All exact."""
+    rng = np.random.default_rng(48)
+    qx, qw = random_q(rng, m, k), random_q(rng, n, k)
+    sums = qx.astype(np.float64) @ qw.astype(np.float64).T
+    assert 2.0 ** 9 < np.abs(sums).max() < 2.0 ** 24
+    for big, small in ((120, -120), (-120, 120), (97, -100)):
+        sx, sw = np.full(m, 2.0 ** big), np.full(n, 2.0 ** small)
+        sx[::5] = 1.0 if big > 0 else 2.0 ** -118
+        y = Q.Array(m, n, Q.F32)
+        ops.gemm(Q.F32, Q.Array.of(qx), Q.Array.of(sx), Q.Array.of(qw), Q.Array.of(sw), None, y, m, n, k)
+        ops.synchronize()
+        assert np.array_equal(y.numpy(), sums * sx[:, None] * sw)
