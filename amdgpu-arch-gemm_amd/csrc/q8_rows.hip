@@ -388,28 +388,25 @@ template <int DT, int G> __global__ void __launch_bounds__(G) norm_backward_any_
 }
 
 // dgain_j = the parts' sums in part order: 32 columns a work-group, 32 slices of parts that meet in
-// LDS, so that few columns still reach many CUs (512 x 999: 64 columns and 16 slices 6.8 us).  Work-groups of a
-// capped grid (a launch ends at 2^32 work-items, 2^27 columns) take their columns in turn.
+// LDS, so that few columns still reach many CUs (512 x 999: 64 columns and 16 slices 6.8 us).  The grid has two
+// dimensions, as one ends at 2^32 work-items, 2^27 columns.  (A loop over a work-group's columns costs more: its
+// loads wait for one another then, 1000 x 999 with it 12.2 us for 8.7.)
 __global__ void __launch_bounds__(1024) column_sum_kernel(const float* partial, float* dgain, uint32_t parts, uint32_t cols) {
     __shared__ float red[32][33];
-    const uint32_t lane = threadIdx.x % 32, slice = threadIdx.x / 32;
+    const uint32_t lane = threadIdx.x % 32, slice = threadIdx.x / 32, c = (blockIdx.y * gridDim.x + blockIdx.x) * 32 + lane;
     const uint32_t per = (parts + 31) / 32, end = min(parts, (slice + 1) * per);
-    for (uint64_t first = (uint64_t)blockIdx.x * 32; first < cols; first += (uint64_t)gridDim.x * 32) {
-        const uint64_t c = first + lane;
-        if (first != (uint64_t)blockIdx.x * 32) __syncthreads();    // the sums before these have been read
-        float s = 0.0f;
-        if (c < cols) {
+    float s = 0.0f;
+    if (c < cols) {
 #pragma unroll 16
-            for (uint32_t i = slice * per; i < end; ++i) s += partial[(uint64_t)i * cols + c];
-        }
-        red[slice][lane] = s;
-        __syncthreads();
-        if (slice == 0 && c < cols) {
-            s = red[0][lane];
+        for (uint32_t i = slice * per; i < end; ++i) s += partial[(uint64_t)i * cols + c];
+    }
+    red[slice][lane] = s;
+    __syncthreads();
+    if (slice == 0 && c < cols) {
+        s = red[0][lane];
 #pragma unroll
-            for (int i = 1; i < 32; ++i) s += red[i][lane];
-            dgain[c] = s;
-        }
+        for (int i = 1; i < 32; ++i) s += red[i][lane];
+        dgain[c] = s;
     }
 }
 
@@ -501,7 +498,9 @@ hipError_t launch_norm_backward(int dtype, const NormBackward& p, hipStream_t s)
     float* dgain = p.dgain;
     uint32_t parts = p.parts, cols = p.cols;
     void* args[] = {&partial, &dgain, &parts, &cols};
-    return hipLaunchKernel(reinterpret_cast<const void*>(&column_sum_kernel), dim3(groups_for(cols, 32)), dim3(1024), args, 0, s);
+    // at most 2^20 x 2^7 work-groups: no column index passes 32 bits
+    const uint32_t x = groups_for(cols, 32), y = (uint32_t)ceil_div(ceil_div(cols, 32), x);
+    return hipLaunchKernel(reinterpret_cast<const void*>(&column_sum_kernel), dim3(x, y), dim3(1024), args, 0, s);
 }
 
 hipError_t prepare_rows() {
