@@ -103,6 +103,12 @@ def _p(a):
     return None if a is None else a.ptr
 
 
+def _check_sizes(func: str, sizes: int):
+    """`sizes`: all sizes or'ed.  One below 0 or past 32 bits would be cut to another one on its way."""
+    if sizes >> 32:
+        raise ValueError(f"{func}: a size or leading dimension is not in 0 .. 2^32 - 1")
+
+
 def row_bytes(cols: int) -> int:
     """The least leading dimension of 8-bit rows that the products read without a copy."""
     return -(-int(cols) // 16) * 16
@@ -110,6 +116,7 @@ def row_bytes(cols: int) -> int:
 
 def workspace_size(call: int, dtype: int, m: int, n: int, k: int) -> int:
     out = _size()
+    _check_sizes("q8_workspace_size", m | n | k)
     S._check("q8_workspace_size", load_library().q8_workspace_size(call, dtype, m, n, k, ctypes.byref(out)))
     return int(out.value)
 
@@ -125,49 +132,63 @@ class Ops:
         self._lib = lib
 
     def quantize(self, dtype, x, q, scale, rows, cols, ldx=None, ldq=None):
-        rc = self._lib.q8_quantize(self.handle, dtype, _p(x), ldx or cols, _p(q), ldq or cols, _p(scale), rows, cols)
+        ldx, ldq = ldx or cols, ldq or cols
+        _check_sizes("q8_quantize", rows | cols | ldx | ldq)
+        rc = self._lib.q8_quantize(self.handle, dtype, _p(x), ldx, _p(q), ldq, _p(scale), rows, cols)
         if rc:
             S._check("q8_quantize", rc)
 
     def dequantize(self, dtype, q, scale, y, rows, cols, ldq=None, ldy=None):
-        rc = self._lib.q8_dequantize(self.handle, dtype, _p(q), ldq or cols, _p(scale), _p(y), ldy or cols, rows, cols)
+        ldq, ldy = ldq or cols, ldy or cols
+        _check_sizes("q8_dequantize", rows | cols | ldq | ldy)
+        rc = self._lib.q8_dequantize(self.handle, dtype, _p(q), ldq, _p(scale), _p(y), ldy, rows, cols)
         if rc:
             S._check("q8_dequantize", rc)
 
     def rmsnorm(self, dtype, x, residual, gain, hidden, q, scale, rstd, rows, cols, eps=1e-5, ldx=None, ldr=None,
                 ldh=None, ldq=None):
         """hidden = x + residual; its norm in 8 bits (residual, hidden and rstd may be None)."""
-        rc = self._lib.q8_rmsnorm(self.handle, dtype, _p(x), ldx or cols, _p(residual), ldr or cols, _p(gain),
-                                  _p(hidden), ldh or cols, _p(q), ldq or cols, _p(scale), _p(rstd), rows, cols, eps)
+        ldx, ldr, ldh, ldq = ldx or cols, ldr or cols, ldh or cols, ldq or cols
+        _check_sizes("q8_rmsnorm", rows | cols | ldx | ldr | ldh | ldq)
+        rc = self._lib.q8_rmsnorm(self.handle, dtype, _p(x), ldx, _p(residual), ldr, _p(gain),
+                                  _p(hidden), ldh, _p(q), ldq, _p(scale), _p(rstd), rows, cols, eps)
         if rc:
             S._check("q8_rmsnorm", rc)
 
     def rmsnorm_backward(self, dtype, dn, hidden, gain, rstd, dres, dx, dgain, rows, cols, lddn=None, ldh=None,
                          lddr=None, lddx=None):
         """dx and dgain (float32) from dn and, where not None, dres."""
-        rc = self._lib.q8_rmsnorm_backward(self.handle, dtype, _p(dn), lddn or cols, _p(hidden), ldh or cols, _p(gain),
-                                           _p(rstd), _p(dres), lddr or cols, _p(dx), lddx or cols, _p(dgain), rows, cols)
+        lddn, ldh, lddr, lddx = lddn or cols, ldh or cols, lddr or cols, lddx or cols
+        _check_sizes("q8_rmsnorm_backward", rows | cols | lddn | ldh | lddr | lddx)
+        rc = self._lib.q8_rmsnorm_backward(self.handle, dtype, _p(dn), lddn, _p(hidden), ldh, _p(gain),
+                                           _p(rstd), _p(dres), lddr, _p(dx), lddx, _p(dgain), rows, cols)
         if rc:
             S._check("q8_rmsnorm_backward", rc)
 
     def gemm(self, dtype, qx, sx, qw, sw, bias, y, m, n, k, ldx=None, ldw=None, ldy=None):
         """y (m x n) = (qx sx) (qw sw)^T + bias."""
-        rc = self._lib.q8_gemm(self.handle, dtype, _p(qx), ldx or k, _p(sx), _p(qw), ldw or k, _p(sw), _p(bias), _p(y),
-                               ldy or n, m, n, k)
+        ldx, ldw, ldy = ldx or k, ldw or k, ldy or n
+        _check_sizes("q8_gemm", m | n | k | ldx | ldw | ldy)
+        rc = self._lib.q8_gemm(self.handle, dtype, _p(qx), ldx, _p(sx), _p(qw), ldw, _p(sw), _p(bias), _p(y), ldy,
+                               m, n, k)
         if rc:
             S._check("q8_gemm", rc)
 
     def grad_input(self, dtype, dy, qw, sw, dx, m, n, k, lddy=None, ldw=None, lddx=None):
         """dx (m x k) = dy (qw sw)."""
-        rc = self._lib.q8_grad_input(self.handle, dtype, _p(dy), lddy or n, _p(qw), ldw or k, _p(sw), _p(dx), lddx or k,
+        lddy, ldw, lddx = lddy or n, ldw or k, lddx or k
+        _check_sizes("q8_grad_input", m | n | k | lddy | ldw | lddx)
+        rc = self._lib.q8_grad_input(self.handle, dtype, _p(dy), lddy, _p(qw), ldw, _p(sw), _p(dx), lddx,
                                      m, n, k)
         if rc:
             S._check("q8_grad_input", rc)
 
     def grad_weight(self, dtype, dy, qx, sx, out_dtype, dw, m, n, k, lddy=None, ldx=None, lddw=None, accumulate=False):
         """dw (n x k) = dy^T (qx sx), added to what dw holds with `accumulate`."""
-        rc = self._lib.q8_grad_weight(self.handle, dtype, _p(dy), lddy or n, _p(qx), ldx or k, _p(sx), out_dtype, _p(dw),
-                                      lddw or k, m, n, k, int(accumulate))
+        lddy, ldx, lddw = lddy or n, ldx or k, lddw or k
+        _check_sizes("q8_grad_weight", m | n | k | lddy | ldx | lddw)
+        rc = self._lib.q8_grad_weight(self.handle, dtype, _p(dy), lddy, _p(qx), ldx, _p(sx), out_dtype, _p(dw),
+                                      lddw, m, n, k, int(accumulate))
         if rc:
             S._check("q8_grad_weight", rc)
 

@@ -1,4 +1,5 @@
 """Index arithmetic of the 8-bit operators at the ends of their range, on the CPU."""
+import inspect
 import os
 import re
 import subprocess
@@ -61,3 +62,30 @@ def test_longest_sums_match_the_header():
     text = open(os.path.join(ROOT, "include", "q8_shim.h")).read()
     values = {k: int(v) for k, v in re.findall(r"#define (Q8_MAX_\w+) (\d+)u", text)}
     assert values == {"Q8_MAX_K": Q.MAX_K, "Q8_MAX_SUM": Q.MAX_SUM, "Q8_MAX_SUM_F32": Q.MAX_SUM_F32}
+
+
+class _Memory:
+    ptr = 4096
+
+
+@pytest.mark.parametrize("size", [-1, 2 ** 32, 2 ** 32 + 5, -2 ** 40])
+@pytest.mark.parametrize("name", ["quantize", "dequantize", "rmsnorm", "rmsnorm_backward", "gemm", "grad_input", "grad_weight"])
+def test_sizes_past_32_bits_reach_no_call(name, size):
+    """They would be cut: 2^32 + 5 rows to five, -1 to 2^32 - 1."""
+    ops = Q.Ops.__new__(Q.Ops)       # without a handle every call that reaches the library is refused there
+    ops.handle, ops._lib = None, Q.load_library()
+    parameters = list(inspect.signature(getattr(Q.Ops, name)).parameters)[1:]
+    sizes = [p for p in parameters if p in ("rows", "cols", "m", "n", "k")]
+    given = {**{p: Q.F32 for p in parameters if p.endswith("dtype")}, **{p: 8 for p in sizes}}
+    given.update({p: _Memory() for p in parameters if p not in given and not p.startswith("ld") and p not in ("eps", "accumulate")})
+    with pytest.raises(S.SgemmError):
+        getattr(ops, name)(**given)
+    for p in sizes + [p for p in parameters if p.startswith("ld")]:
+        with pytest.raises(ValueError, match="q8_" + name):
+            getattr(ops, name)(**{**given, p: size})
+
+
+def test_workspace_of_sizes_past_32_bits():
+    for bad in ((-1, 8, 8), (8, 2 ** 32, 8), (8, 8, 2 ** 33 + 1)):
+        with pytest.raises(ValueError):
+            Q.workspace_size(Q.CALL_GEMM, Q.F32, *bad)
