@@ -5,6 +5,7 @@
 #include "sgemm_internal.hpp"
 
 #include <cstdarg>
+#include <cstdint>
 #include <cstdio>
 #include <new>
 
@@ -115,7 +116,9 @@ int grow(q8_handle* h, size_t bytes) {
     if (capturing(h->stream))
         return fail(SGEMM_E_SHAPE, "a workspace of %zu bytes is needed and %zu are there: under graph capture it cannot grow "
                                    "(q8_reserve beforehand)", bytes, h->workspace_bytes);
-    const size_t want = (bytes + ((size_t)2 << 20) - 1) & ~(((size_t)2 << 20) - 1);
+    constexpr size_t kStep = (size_t)2 << 20;
+    if (bytes > SIZE_MAX - kStep) return hip_fail(hipErrorOutOfMemory, "workspace");    // rounded up it would pass 0
+    const size_t want = (bytes + kStep - 1) / kStep * kStep;
     HIP_TRY(hipStreamSynchronize(h->stream));
     if (h->workspace && h->captured) {
         // a captured call may be replayed: its workspace stays until the handle goes

@@ -128,3 +128,20 @@ def test_scales_whose_product_is_in_range(ops, m, n, k):
         ops.gemm(Q.F32, Q.Array.of(qx), Q.Array.of(sx), Q.Array.of(qw), Q.Array.of(sw), None, y, m, n, k)
         ops.synchronize()
         assert np.array_equal(y.numpy(), sums * sx[:, None] * sw)
+
+
+def test_workspaces_that_cannot_be():
+    """Refused, and the handle works on."""
+    rng = np.random.default_rng(49)
+    m, n, k = 1100, 128, 4096       # K ranges: needs a workspace
+    qx, qw = random_q(rng, m, k), random_q(rng, n, k)
+    y = Q.Array(m, n, Q.F32)
+    with Q.Ops() as o:
+        assert Q.workspace_size(Q.CALL_GEMM, Q.F32, m, n, k) > 0
+        for nbytes in (2 ** 64 - 1, 2 ** 64 - 2 ** 21 + 1, 2 ** 60):
+            with pytest.raises(S.SgemmError) as e:
+                o.reserve(nbytes)
+            assert e.value.code > 0
+            o.gemm(Q.F32, Q.Array.of(qx), Q.Array.of(np.ones(m)), Q.Array.of(qw), Q.Array.of(np.ones(n)), None, y, m, n, k)
+            o.synchronize()
+            assert np.array_equal(y.numpy(), qx.astype(np.float64) @ qw.astype(np.float64).T)
