@@ -91,20 +91,26 @@ inline ProductPlan plan_product(uint64_t m, uint64_t n, uint64_t kb) {
 constexpr uint64_t tiles_per_split(uint64_t kb, uint32_t splits) { return div_up(div_up(kb, kTileBytes), splits); }
 constexpr bool asks_ahead(uint64_t groups, uint64_t tiles) { return groups > kComputeUnits || tiles > 32; }
 
-// The direct kernel's tiles, 16 MT tokens x 16 NT channels a work-group of WAVES waves:
-//   1 x 1, 16 waves  a small product: a work-group a CU (333 x 129 x 517: 4.2 us, 2 x 1 5.2)
-//   1 x 1, 8 waves   up to 16 tokens (16 x 4096 x 4096: 6.9 us; 16 waves 7.2), and 16 waves over
-//                    a deep K of few channels (1 x 4096 x 16384: 14.5 against 16.9)
-//   1 x 4, 8 waves   up to 16 tokens into many channels: the tokens are read a quarter as often
-//                    (16 x 16384 x 4096: 15.8 us, 1 x 1 19.0)
-//   2 x 1, 2 x 4     the same up to 32 tokens (32 x 16384 x 4096: 18.4 us, 2 x 1 26.8)
-//   2 x 2, 4 x 4     and up to 64 (64 x 4096 x 4096: 10.4 us, 2 x 1 14.1, 4 x 1 12.5;
-//                    64 x 16384 x 4096: 25.2 us, 2 x 2 40.8)
+// The direct kernel's tiles, 16 MT tokens x 16 NT channels a work-group of WAVES waves.  Times in us at the sizes named, with
+// 400 MB of weights and more in turn, as a model's layers follow one another; weights that the last-level cache
+// holds favour other tiles in places (1 x 4 at 1 x 12288 x 4096 by 5%, 16 waves at 1 x 4096 x 16384 by 11%).
+//   1 x 1, 8 waves   up to 16 tokens (16 x 4096 x 4096 6.5, one token 5.6); 16 waves gain 4% at most and cost
+//                    up to 14% (1 x 4096 x 10240 10.0 against 9.8, x 12288 13.0 against 11.3)
+//   1 x 4, 8 waves   the same into many channels: four times the tokens' operands for a work-group's weights, a quarter of the
+//                    work-groups, so it pays where the tokens weigh and where K is short.  16 x 16384 x 4096 19.3
+//                    against 21.2, x 12288 16.4 and 16.9, x 11264 15.7 and 15.9; 1 x 12288 x 1024 5.6 and
+//                    6.0, x 2048 7.8 and 8.1, x 3000 18.9 and 15.5, x 8192 27.2 and 19.1; x 4096 of 8, 12 and 16 tokens into 16384
+//                    18.3 and 18.1, 18.9 and 19.7, 19.3 and 21.2
+//   1 x 1, 16 waves  a small product of more tokens: a work-group a CU (333 x 129 x 517: 4.2, 2 x 1 5.2)
+//   2 x 1, 2 x 4     up to 32 tokens.  2 x 4 once 2 x 1 has more than two work-groups a CU: 32 x 8704 x 4096 17.3 against
+//                    20.4, x 16384 22.2 and 29.5, but x 8192 17.0 and 15.4
+//   2 x 2, 4 x 4     and up to 64, with the same bound: 64 x 8704 x 4096 23.9 against 28.3, x 16384 28.8 and
+//                    42.0, but x 8192 23.5 and 21.5 (64 x 4096 x 4096: 2 x 1 14.1, 4 x 1 12.5, 2 x 2 10.4)
 enum Direct { D_1x1_16, D_1x1_8, D_1x4_8, D_2x1_8, D_2x4_8, D_2x2_8, D_4x4_4 };
 inline Direct direct_kind(uint64_t m, uint64_t n, uint64_t k) {
-    const bool wide = n >= 12288;
-    if (m <= 16) return wide ? D_1x4_8 : n <= 4096 && k > 8192 ? D_1x1_16 : D_1x1_8;
+    if (m <= 16) return n >= 12288 && (m >= 12 || k <= 2048) ? D_1x4_8 : D_1x1_8;
     if (div_up(m, 16) * div_up(n, 16) <= kComputeUnits) return D_1x1_16;
+    const bool wide = n > 2 * kComputeUnits * 16;
     if (m <= 32) return wide ? D_2x4_8 : D_2x1_8;
     if (m <= kFewTokens) return wide ? D_4x4_4 : D_2x2_8;
     return D_2x1_8;

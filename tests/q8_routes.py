@@ -94,3 +94,14 @@ def grad_wanted(dtype, turned):
     want = {(kind, "whole") for kind in ("large", "large-ahead", "small", "deep")}
     want |= {(kind, "ranges") for kind in ("large-ahead", "small", "deep")}
     return want | {("direct", "waves-4")} | (set() if turned and dtype == "f32" else {("direct", "waves-8")})
+
+
+# few tokens and small products: each tile of the kernel that takes operands as they are
+DIRECTS = [(3, 200, 1300), (16, 4100, 140), (1, 12300, 2100), (11, 12300, 2100), (12, 12300, 2100), (3, 12300, 1000), (100, 90, 700),
+           (20, 5000, 140), (20, 8200, 140), (50, 5000, 200), (50, 8200, 140), (300, 900, 72)]
+DIRECT_TILES = ["1x1, 16 waves", "1x1", "1x4", "2x1", "2x4", "2x2", "4x4"]
+
+
+def direct_tile(m, n, k):
+    route = gemm_route(m, n, k, k, 0)
+    return DIRECT_TILES[int(route[1])] if route[0] == "direct" else None

@@ -8,7 +8,7 @@ import numpy as np
 import pytest
 
 from q8_reference import TINY, TYPES, UNIT, random_q, stored
-from q8_routes import GEMMS, GRADIENTS
+from q8_routes import DIRECTS, GEMMS, GRADIENTS
 from shim import q8_shim as Q
 from shim import sgemm_shim as S
 
@@ -59,9 +59,7 @@ def sample(rng, rows):
     return np.unique(np.concatenate([[0], np.minimum(some, rows - 1), [rows - 1]]))
 
 
-@pytest.mark.parametrize("dtype", list(TYPES))
-@pytest.mark.parametrize("m,n,k,pad,shift", GEMMS)
-def test_product(ops, m, n, k, pad, shift, dtype):
+def _product(ops, m, n, k, pad, shift, dtype):
     print(f"gemm {m}x{n}x{k} +{pad} from {shift} {dtype}", flush=True)
     rng = np.random.default_rng(41)
     qx, qw = (rng.integers(-128, 128, (r, k), dtype=np.int8) for r in (m, n))
@@ -76,6 +74,19 @@ def test_product(ops, m, n, k, pad, shift, dtype):
     want = p + b
     bound = UNIT[dtype] * np.abs(want) + 4 * 2.0 ** -24 * (np.abs(p) + np.abs(b)) + TINY[dtype]
     _compare(y.result(rows), want, bound, dtype)
+
+
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("m,n,k,pad,shift", GEMMS)
+def test_product(ops, m, n, k, pad, shift, dtype):
+    _product(ops, m, n, k, pad, shift, dtype)
+
+
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("pad,shift", [(0, 0), (1, 1), (2, 0), (0, 3)])
+@pytest.mark.parametrize("m,n,k", DIRECTS)
+def test_few_tokens(ops, m, n, k, pad, shift, dtype):
+    _product(ops, m, n, k, pad, shift, dtype)
 
 
 def _compare(got, want, bound, out):
