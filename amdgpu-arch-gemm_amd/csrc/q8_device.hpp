@@ -181,16 +181,13 @@ __device__ __forceinline__ void wave_sum_max(float& f, uint32_t& u) {
     step((uint32_t)__shfl_xor((int)bits(), 32), (uint32_t)__shfl_xor((int)u, 32));
 }
 
-__device__ __forceinline__ uint16_t bits16(float x, bool half) {
-    if (half) return __builtin_bit_cast(uint16_t, (_Float16)x);
-    return __builtin_bit_cast(uint16_t, (__bf16)x);
-}
 template <bool HALF> __device__ __forceinline__ uint32_t pair16(float x, float y) {
     return HALF ? Type<Q8_F16>::pair(x, y) : Type<Q8_BF16>::pair(x, y);
 }
 
 // x = hi + mid + lo in BF16, each cut off where the next one goes on: both differences are exact,
-// and three terms of 8 bits hold the 24 of FP32.  Infinities and NaN stay in the first term.
+// and three terms of 8 bits hold the 24 of FP32, of all x from 2^-110 on (below, the last term's bits pass BF16's
+// smallest step, 2^-133).  Infinities and NaN stay in the first term.
 // The terms are the upper halves of b.
 __device__ __forceinline__ void three(float x, uint32_t (&b)[3]) {
     x = __builtin_canonicalizef(x);     // a NaN has a bit in the first term

@@ -107,7 +107,8 @@ int q8_dequantize(q8_handle* h, int dtype, const int8_t* q, uint32_t ldq, const 
  * in 8 bits: q and scale[rows].  residual may be NULL (hidden = x); hidden and
  * rstd may be NULL where they are not wanted.  hidden may be x or residual
  * itself (same pointer and ld).  The squares are summed in FP32: a row whose
- * sum passes its largest value (4096 values of 2^58) has rstd = 0. */
+ * sum passes its largest value (4096 values of 2^58) has rstd = 0, and with eps = 0 one whose squares vanish (zeros,
+ * or values below 2^-75) has rstd = infinity and scale = NaN.  hidden_ij gain_j is an FP32 value too. */
 int q8_rmsnorm(q8_handle* h, int dtype, const void* x, uint32_t ldx, const void* residual, uint32_t ldr,
                const void* gain, void* hidden, uint32_t ldh, int8_t* q, uint32_t ldq, float* scale, float* rstd,
                uint32_t rows, uint32_t cols, float eps);
@@ -132,8 +133,9 @@ int q8_gemm(q8_handle* h, int dtype, const int8_t* qx, uint32_t ldx, const float
 /* dx_ik = sum_j dy_ij sw_j qw_jk: m tokens, n channels, k features; dy (m x n)
  * and dx (m x k) in `dtype`.  The products run on the 16-bit matrix cores with
  * FP32 sums; sw_j qw_jk is rounded to `dtype` for it, to 2^-8 of it in Q8_BF16, in
- * Q8_F16 to 2^-11 of it or 2^-32 of the largest scale.  Q8_F32 loses nothing: sw_j dy_ij is split
- * into three BF16 terms that hold all its bits. */
+ * Q8_F16 to 2^-11 of it or 2^-32 of the largest scale.  In Q8_F32 sw_j dy_ij is rounded to FP32 and split into
+ * three BF16 terms, which hold all its bits where it is 2^-110 and more, and its steps of 2^-133 below; past FP32's
+ * largest value it is infinite. */
 int q8_grad_input(q8_handle* h, int dtype, const void* dy, uint32_t lddy, const int8_t* qw, uint32_t ldw,
                   const float* sw, void* dx, uint32_t lddx, uint32_t m, uint32_t n, uint32_t k);
 

@@ -145,3 +145,37 @@ def test_workspaces_that_cannot_be():
             o.gemm(Q.F32, Q.Array.of(qx), Q.Array.of(np.ones(m)), Q.Array.of(qw), Q.Array.of(np.ones(n)), None, y, m, n, k)
             o.synchronize()
             assert np.array_equal(y.numpy(), qx.astype(np.float64) @ qw.astype(np.float64).T)
+
+
+# from the operands as they are, and laid out
+@pytest.mark.parametrize("m,n,k", [(64, 64, 64), (130, 4100, 133)])
+@pytest.mark.parametrize("exponent", [-110, -60, 0, 118])
+def test_fp32_gradients_keep_every_bit(ops, m, n, k, exponent):
+    """One product for each result, so all that is rounded is the sum of its three terms: three roundings of 2^-23 at most."""
+    rng = np.random.default_rng(50)
+    dy = rng.uniform(1, 2, (m, n)).astype(np.float32).astype(np.float64) * 2.0 ** exponent
+    qw = np.zeros((n, k), np.int8)
+    qw[rng.integers(0, n, k), np.arange(k)] = rng.integers(1, 128, k)
+    dx = Q.Array(m, k, Q.F32)
+    ops.grad_input(Q.F32, Q.Array.of(dy), Q.Array.of(qw), Q.Array.of(np.ones(n)), dx, m, n, k)
+    ops.synchronize()
+    want = dy @ qw
+    assert np.all(np.abs(dx.numpy() - want) <= 3 * 2.0 ** -23 * want)
+    qx = np.zeros((m, k), np.int8)
+    qx[rng.integers(0, m, k), np.arange(k)] = rng.integers(1, 128, k)
+    dw = Q.Array(n, k, Q.F32)
+    ops.grad_weight(Q.F32, Q.Array.of(dy), Q.Array.of(qx), Q.Array.of(np.ones(m)), Q.F32, dw, m, n, k)
+    ops.synchronize()
+    want = dy.T @ qx
+    assert np.all(np.abs(dw.numpy() - want) <= 3 * 2.0 ** -23 * want)
+
+
+def test_norm_without_eps(ops):
+    """A row of zeros has no norm then; others have theirs."""
+    x = np.ones((3, 64))
+    x[1] = 0
+    q, s, rstd = Q.Array(3, 64, "int8"), Q.Array(1, 3, Q.F32), Q.Array(1, 3, Q.F32)
+    ops.rmsnorm(Q.F32, Q.Array.of(x), None, Q.Array.of(np.ones(64)), None, q, s, rstd, 3, 64, eps=0.0)
+    ops.synchronize()
+    assert np.array_equal(q.numpy(), np.where(x > 0, 127, 0)) and np.array_equal(rstd.numpy()[0], [1, np.inf, 1])
+    assert np.isnan(s.numpy()[0, 1]) and np.all(np.abs(s.numpy()[0, ::2] * 127 - 1) <= 2.0 ** -23)
