@@ -9,8 +9,9 @@
 //
 // What bounds the large products.  8192^3 in 8-bit integers takes 405 - 433 us by card, 2.5 - 2.7 Pops (a
 // large library product 2.35); 16384 x 4096 x 4096 in BF16 400 - 415 us, 1.33 - 1.37 PFLOP/s (library 1.32).
-// The card's power, at which a loop of matrix instructions alone reaches 4.0 Pops and 2.0 PFLOP/s on
-// such data, and the loads' way into LDS: without any load 375 us instead of 430, in BF16
+// The card's power (a loop of matrix instructions alone reaches 4.0 Pops and 2.0 PFLOP/s on such data;
+// here the clock falls from 2.4 to 1.8 and 1.9 GHz, and the matrix instructions are busy 64% and 66 - 72% of the cycles),
+// and the loads' way into LDS: without any load 375 us instead of 430, in BF16
 // 362 instead of 413.  Not memory: with every load from lines that L2 holds the times are the same.
 // Four waves of 128 x 128 rather than eight of 128 x 64: LDS gives 128 bytes a cycle, and eight
 // waves would ask it for 192 KB a K tile beside the 64 KB that arrive, as long as the matrix
@@ -367,7 +368,7 @@ template <int E, int DT> __global__ void __launch_bounds__(256) finish_kernel(co
 // straight to the matrix cores, from rows that start anywhere, with a run's loads in flight
 // while the one before is multiplied.  The waves' sums meet in LDS.
 // ODD: rows start between dwords.  Loads of 16 bytes from there take more than twice the time (1 x 2551 x
-// 10881: 22.8 us, rows of 10884 10.0), so the dwords around them are read and shifted.
+// 10881: 22.8 us, rows of 10884 9.5), so the dwords around them are read and shifted.
 template <int MT, int NT, int WAVES, int DT, bool ODD>
 __global__ void __launch_bounds__(WAVES * 64) direct_kernel(const Product p) {
     constexpr int RUN = ODD && MT * NT > 1 ? 2 : 4;
