@@ -453,7 +453,9 @@ template <int DT> hipError_t dequantize_any(const Dequantize& p, hipStream_t s) 
 
 // Row ranges that a column's sum is taken over first, one work-group each: two a CU that has 512
 // threads (BF16, 16384 x 4096: 256 / 512 / 1024 ranges 118 / 98 / 116 us, 5.5 TB/s; 16384 x 8192 207 / 194 / 205;
-// 1000 x 999 10.3 / 8.0 / 10.8): each range is written, read and added once more.
+// 1000 x 999 10.3 / 8.0 / 10.8): each range is written, read and added once more.  Threads whose last pieces are empty
+// cost little, so there are no kernels for the widths between (2^27 BF16 values in rows of 4096 5.5 TB/s, 5120 5.3, 6144 5.6,
+// 8192 5.6, 10240 5.2, 12288 5.2, 16384 5.2).
 constexpr uint32_t kMostParts = 512;
 template <int DT> hipError_t backward_any(const NormBackward& p, hipStream_t s) {
     const uint32_t pieces = (uint32_t)ceil_div(p.cols, 8);
