@@ -126,7 +126,7 @@ int q8_rmsnorm_backward(q8_handle* h, int dtype, const void* dn, uint32_t lddn, 
 
 /* y_ij = sx_i sw_j sum_k qx_ik qw_jk + bias_j for m tokens (qx, m x k), n
  * channels (qw, n x k): exact 32-bit integer sums.  y and bias in `dtype`;
- * bias may be NULL.  k at most Q8_MAX_K. */
+ * bias may be NULL.  k at most Q8_MAX_K; n below 2^28 where m is at most 64. */
 int q8_gemm(q8_handle* h, int dtype, const int8_t* qx, uint32_t ldx, const float* sx, const int8_t* qw, uint32_t ldw,
             const float* sw, const void* bias, void* y, uint32_t ldy, uint32_t m, uint32_t n, uint32_t k);
 
