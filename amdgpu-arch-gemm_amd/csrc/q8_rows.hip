@@ -393,7 +393,7 @@ template <int DT, int G> __global__ void __launch_bounds__(G) norm_backward_any_
 // loads wait for one another then, 1000 x 999 with it 12.2 us for 8.7.)
 __global__ void __launch_bounds__(1024) column_sum_kernel(const float* partial, float* dgain, uint32_t parts, uint32_t cols) {
     __shared__ float red[32][33];
-    const uint32_t lane = threadIdx.x % 32, slice = threadIdx.x / 32, c = (blockIdx.y * gridDim.x + blockIdx.x) * 32 + lane;
+    const uint32_t lane = threadIdx.x % 32, slice = threadIdx.x / 32, c = (blockIdx.y * kMostGroups + blockIdx.x) * 32 + lane;
     const uint32_t per = (parts + 31) / 32, end = min(parts, (slice + 1) * per);
     float s = 0.0f;
     if (c < cols) {
@@ -500,7 +500,7 @@ hipError_t launch_norm_backward(int dtype, const NormBackward& p, hipStream_t s)
     float* dgain = p.dgain;
     uint32_t parts = p.parts, cols = p.cols;
     void* args[] = {&partial, &dgain, &parts, &cols};
-    // at most 2^20 x 2^7 work-groups: no column index passes 32 bits
+    // at most kMostGroups x 2^7 work-groups, and kMostGroups of them wherever y is not 1: no column index passes 32 bits
     const uint32_t x = groups_for(cols, 32), y = (uint32_t)ceil_div(ceil_div(cols, 32), x);
     return hipLaunchKernel(reinterpret_cast<const void*>(&column_sum_kernel), dim3(x, y), dim3(1024), args, 0, s);
 }
