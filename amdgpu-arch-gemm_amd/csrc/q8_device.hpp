@@ -181,6 +181,35 @@ __device__ __forceinline__ void wave_sum_max(float& f, uint32_t& u) {
     step((uint32_t)__shfl_xor((int)bits(), 32), (uint32_t)__shfl_xor((int)u, 32));
 }
 
+// q_j = rint(n_j / s), n_j = u_j rstd, s = max|n| / 127 and at least 2^-126.  rstd is a factor of the row,
+// so q_j = rint(u_j 127 / max|u|): the largest |u| gives the scale without a second sum over the row, and
+// the quotient rounds twice, not four times.  It is taken in two factors where one would leave FP32's range:
+// rows below 2^-118, and rows whose scale is the least one.
+struct Scale {
+    float s, f1, f2;
+    bool ok;
+};
+__device__ __forceinline__ Scale scale_of(uint32_t top_bits, float rstd) {
+    Scale r;
+    const float top = __builtin_bit_cast(float, top_bits), most = top * rstd / 127.0f;
+    r.ok = most < __builtin_huge_valf();     // false for infinities and NaN
+    const bool least = !(most > 0x1p-126f), tiny = top < 0x1p-118f;
+    r.s = !r.ok ? __builtin_nanf("") : least ? 0x1p-126f : most;
+    r.f1 = least ? rstd : tiny ? 0x1p60f : 127.0f / top;
+    r.f2 = least ? 0x1p126f : tiny ? 127.0f / (top * 0x1p60f) : 1.0f;
+    return r;
+}
+__device__ __forceinline__ uint32_t to8(float u, const Scale& r) {
+    const float q = __builtin_rintf(u * r.f1 * r.f2);
+    return r.ok ? (uint32_t)(int)__builtin_amdgcn_fmed3f(q, -127.0f, 127.0f) & 0xffu : 0u;
+}
+__device__ __forceinline__ u32x2 bytes8(const float (&u)[8], const Scale& s) {
+    uint32_t q[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) q[e] = to8(u[e], s);
+    return u32x2{q[0] | q[1] << 8 | q[2] << 16 | q[3] << 24, q[4] | q[5] << 8 | q[6] << 16 | q[7] << 24};
+}
+
 template <bool HALF> __device__ __forceinline__ uint32_t pair16(float x, float y) {
     return HALF ? Type<Q8_F16>::pair(x, y) : Type<Q8_BF16>::pair(x, y);
 }

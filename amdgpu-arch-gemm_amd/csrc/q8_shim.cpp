@@ -1,147 +1,14 @@
 // Host side of the 8-bit operators (include/q8_shim.h): handles, argument checks,
 // workspace, and which kernels a call runs on.
-#include "q8_internal.hpp"
+#include "q8_host.hpp"
 #include "q8_plan.hpp"
-#include "sgemm_internal.hpp"
 
-#include <cstdarg>
 #include <cstdint>
-#include <cstdio>
 #include <new>
-
-struct q8_handle {
-    struct Retired {
-        void* memory;
-        Retired* next;
-    };
-    int device = 0;
-    hipStream_t stream = nullptr;
-    hipStream_t own_stream = nullptr;
-    char* workspace = nullptr;
-    size_t workspace_bytes = 0;
-    Retired* retired = nullptr;    // workspaces that captured calls may still use
-    bool captured = false;         // a call that used the workspace was captured
-};
 
 namespace {
 
 using namespace q8;
-
-int fail(int code, const char* fmt, ...) __attribute__((format(printf, 2, 3)));
-int fail(int code, const char* fmt, ...) {
-    char msg[256];
-    va_list ap;
-    va_start(ap, fmt);
-    vsnprintf(msg, sizeof(msg), fmt, ap);
-    va_end(ap);
-    return sgemm_internal::set_error(code, msg);
-}
-int hip_fail(hipError_t e, const char* what) { return fail((int)e, "%s: %s (%d)", what, hipGetErrorString(e), (int)e); }
-int launched(hipError_t e, const char* what) { return e == hipSuccess ? SGEMM_OK : hip_fail(e, what); }
-
-#define HIP_TRY(call)                                      \
-    do {                                                   \
-        const hipError_t e_ = (call);                      \
-        if (e_ != hipSuccess) return hip_fail(e_, #call);  \
-    } while (0)
-#define CHECK(call)                       \
-    do {                                  \
-        const int c_ = (call);            \
-        if (c_ != SGEMM_OK) return c_;    \
-    } while (0)
-
-// The handle's device is current while a call runs.
-class OnDevice {
-public:
-    explicit OnDevice(int device) {
-        if (hipGetDevice(&before_) != hipSuccess) before_ = device;
-        if (before_ != device) status_ = hipSetDevice(device);
-        device_ = device;
-    }
-    ~OnDevice() {
-        if (before_ != device_) (void)hipSetDevice(before_);
-    }
-    hipError_t status() const { return status_; }
-
-private:
-    int before_ = 0, device_ = 0;
-    hipError_t status_ = hipSuccess;
-};
-
-bool capturing(hipStream_t stream) {
-    hipStreamCaptureStatus s = hipStreamCaptureStatusNone;
-    return hipStreamIsCapturing(stream, &s) != hipSuccess || s != hipStreamCaptureStatusNone;
-}
-
-bool is_type(int dtype) { return dtype == Q8_F32 || dtype == Q8_F16 || dtype == Q8_BF16; }
-
-// A matrix argument: rows of cols values at ld, `bytes` each.
-struct Span {
-    const char* name;
-    const void* p;
-    uint64_t rows, cols, ld;
-    uint32_t bytes;
-};
-int check(const Span& s) {
-    if (!s.rows || !s.cols) return SGEMM_OK;
-    if (!s.p) return fail(SGEMM_E_INVALID, "%s is null", s.name);
-    if ((uintptr_t)s.p % s.bytes) return fail(SGEMM_E_INVALID, "%s is not aligned to its %u-byte values", s.name, s.bytes);
-    if (s.ld < s.cols)
-        return fail(SGEMM_E_SHAPE, "%s: leading dimension %llu below its %llu columns", s.name, (unsigned long long)s.ld,
-                    (unsigned long long)s.cols);
-    return SGEMM_OK;
-}
-// Whether two matrices share a byte.  Windows of different columns of one buffer
-// (the same ld) do not.
-bool overlap(const Span& a, const Span& b) {
-    if (!a.p || !b.p || !a.rows || !a.cols || !b.rows || !b.cols) return false;
-    const uintptr_t a0 = (uintptr_t)a.p, b0 = (uintptr_t)b.p;
-    const uint64_t la = a.ld * a.bytes, lb = b.ld * b.bytes;
-    const uint64_t a1 = a0 + (a.rows - 1) * la + a.cols * a.bytes, b1 = b0 + (b.rows - 1) * lb + b.cols * b.bytes;
-    if (a1 <= b0 || b1 <= a0) return false;
-    if (la != lb) return true;
-    const uint64_t d = a0 <= b0 ? (b0 - a0) % la : (la - (a0 - b0) % la) % la;   // b's first column in a's rows
-    return d < a.cols * a.bytes || d + b.cols * b.bytes > la;
-}
-bool same(const Span& a, const Span& b) { return a.p == b.p && a.ld == b.ld && a.bytes == b.bytes; }
-int check_apart(const Span& out, const Span& in, bool in_place = false) {
-    if (in_place && same(out, in)) return SGEMM_OK;
-    if (overlap(out, in)) return fail(SGEMM_E_INVALID, "%s overlaps %s", out.name, in.name);
-    return SGEMM_OK;
-}
-Span vec(const char* name, const void* p, uint64_t count, uint32_t bytes) { return Span{name, p, 1, count, count, bytes}; }
-
-int grow(q8_handle* h, size_t bytes) {
-    if (bytes <= h->workspace_bytes) return SGEMM_OK;
-    if (capturing(h->stream))
-        return fail(SGEMM_E_SHAPE, "a workspace of %zu bytes is needed and %zu are there: under graph capture it cannot grow "
-                                   "(q8_reserve beforehand)", bytes, h->workspace_bytes);
-    constexpr size_t kStep = (size_t)2 << 20;
-    if (bytes > SIZE_MAX - kStep) return hip_fail(hipErrorOutOfMemory, "workspace");    // rounded up it would pass 0
-    const size_t want = (bytes + kStep - 1) / kStep * kStep;
-    HIP_TRY(hipStreamSynchronize(h->stream));
-    if (h->workspace && h->captured) {
-        // a captured call may be replayed: its workspace stays until the handle goes
-        q8_handle::Retired* r = new (std::nothrow) q8_handle::Retired{h->workspace, h->retired};
-        if (!r) return fail(SGEMM_E_SHAPE, "out of host memory");
-        h->retired = r;
-    } else if (h->workspace) {
-        HIP_TRY(hipFree(h->workspace));
-    }
-    h->workspace = nullptr;
-    h->workspace_bytes = 0;
-    void* p = nullptr;
-    HIP_TRY(hipMalloc(&p, want));
-    h->workspace = static_cast<char*>(p);
-    h->workspace_bytes = want;
-    return SGEMM_OK;
-}
-int take_workspace(q8_handle* h, size_t bytes) {
-    if (!bytes) return SGEMM_OK;
-    CHECK(grow(h, bytes));
-    if (!h->captured && capturing(h->stream)) h->captured = true;
-    return SGEMM_OK;
-}
 
 // As plan_grad, refusing a sum that is too long.
 int plan(int dtype, bool turned, bool odd, uint64_t rows, uint64_t cols, uint64_t sum, bool copy_a, GradPlan& g) {
@@ -169,9 +36,6 @@ bool rows_aligned(const void* p, uint64_t ld_bytes) {
 
 bool odd_rows(const void* p, uint64_t ld_bytes) { return ((uintptr_t)p | ld_bytes) % 4 != 0; }
 
-int check_handle(const q8_handle* h) { return h ? SGEMM_OK : fail(SGEMM_E_INVALID, "the handle is null"); }
-int check_type(int dtype) { return is_type(dtype) ? SGEMM_OK : fail(SGEMM_E_INVALID, "%d is no type", dtype); }
-
 void set_common(Product& p, q8_handle* h, const ProductPlan& plan, const Layout& at) {
     p.partial = plan.partial_bytes ? h->workspace + at.partial : nullptr;
 }
@@ -194,6 +58,8 @@ int q8_open(q8_handle** out) {
     if (e == hipSuccess) e = prepare_packing();
     if (e == hipSuccess) e = prepare_products();
     if (e == hipSuccess) e = prepare_gradients();
+    if (e == hipSuccess) e = prepare_cache_rows();
+    if (e == hipSuccess) e = prepare_attention();
     if (e != hipSuccess) {
         if (h->own_stream) (void)hipStreamDestroy(h->own_stream);
         delete h;
