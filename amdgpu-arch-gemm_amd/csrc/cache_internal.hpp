@@ -2,6 +2,7 @@
 // their kernels (cache_rows.hip, cache_attention.hip).  Nothing here is part of the C-ABI.
 #pragma once
 
+#include "cache_plan.hpp"
 #include "q8_cache.h"
 #include "q8_internal.hpp"
 
@@ -60,6 +61,17 @@ struct Attention {
     uint32_t ldq, ldo, heads, group, window;
     float scale;
 };
-Q8_INTERNAL hipError_t launch_attention(int dtype, const Attention& p, hipStream_t stream);
+// One launch of it: the sequences of more than `least` and at most `most` rows (new tokens times the heads that share
+// one of the cache's), in tiles that `slots` are no fewer than, each one's keys in pieces of `piece`.
+struct AttentionArgs {
+    Attention a;
+    Divisor by_group;
+    uint32_t slots, least, most, piece;
+    float* sums;        // pieces x tokens x heads x held dim
+    float* stats;       // pieces x tokens x heads: R, l
+    uint32_t* tickets;  // of each tile: the pieces that are done; 0 before and after a launch
+};
+Q8_INTERNAL hipError_t launch_few(int dtype, const AttentionArgs& g, uint32_t pieces, hipStream_t stream);
+Q8_INTERNAL hipError_t launch_many(int dtype, const AttentionArgs& g, uint32_t pieces, hipStream_t stream);
 
 }  // namespace q8

@@ -1,0 +1,71 @@
+// How an attention over the cache runs: kernels, pieces of the keys, workspace.  Host
+// code without HIP.
+#pragma once
+
+#include <cstddef>
+#include <cstdint>
+
+namespace q8 {
+
+constexpr uint64_t kFewGroups = 1024, kManyGroups = 256;
+// Rows of a tile: tokens of one sequence times the heads that share one of the cache's; keys of a step.
+constexpr uint32_t kFewRows = 16, kFewKeys = 128;
+constexpr uint32_t kManyKeys = 64;
+constexpr uint32_t kFewMost = 32;
+// Tiles whose keys are taken in pieces, at the most: each has a ticket in the handle.
+constexpr uint32_t kTickets = 4096;
+
+constexpr uint64_t up(uint64_t a, uint64_t b) { return (a + b - 1) / b; }
+
+// Values of a head as the kernels hold them.
+constexpr uint32_t held_dim(uint32_t dim) { return dim <= 64 ? 64 : dim <= 128 ? 128 : 256; }
+// Rows of a tile of many: 32 or 64 a wave.
+constexpr uint32_t many_rows(bool f32, uint32_t dim) { return f32 || dim > 128 ? 128 : 256; }
+
+struct AttentionLaunch {
+    uint32_t slots = 0;         // tiles there may be; 0: no launch
+    uint32_t least = 0, most = UINT32_MAX;
+    uint32_t piece = 0;         // keys of a piece
+    uint32_t pieces = 1;        // of the longest sequence
+};
+struct AttentionPlan {
+    AttentionLaunch few, many;
+    size_t bytes = 0;           // workspace: the pieces' sums
+};
+
+inline void cut(AttentionLaunch& l, uint64_t tiles, uint64_t keys, uint64_t step, uint64_t groups) {
+    const uint64_t steps = up(keys ? keys : 1, step);
+    uint64_t most = tiles && tiles <= kTickets ? groups / tiles : 1;
+    if (most < 1) most = 1;
+    const uint64_t each = up(steps, most < steps ? most : steps);
+    l.piece = (uint32_t)(each * step);
+    l.pieces = (uint32_t)up(steps, each);
+}
+
+inline AttentionPlan plan_attention(bool f32, uint64_t tokens, uint64_t seqs, uint64_t keys, uint64_t longest, uint64_t heads,
+                                    uint64_t kv_heads, uint32_t dim) {
+    AttentionPlan p;
+    if (!tokens || !seqs) return p;
+    const uint64_t group = heads / kv_heads, rows = tokens * group, filled = seqs < tokens ? seqs : tokens;
+    if (!longest || longest > tokens) longest = tokens;
+    const bool few = longest * group <= kFewMost || seqs > 1, many = longest * group > kFewMost;
+    if (few) {
+        p.few.slots = (uint32_t)(rows / kFewRows + filled);
+        if (many) {
+            p.few.most = p.many.least = kFewMost;
+            if (p.few.slots > filled * up(kFewMost, kFewRows)) p.few.slots = (uint32_t)(filled * up(kFewMost, kFewRows));
+        }
+        cut(p.few, p.few.slots * kv_heads, keys, kFewKeys, kFewGroups);
+    }
+    if (many) {
+        const uint32_t height = many_rows(f32, dim);
+        const uint64_t own = rows / kFewMost < filled ? rows / kFewMost : filled;      // sequences of more rows than few
+        p.many.slots = (uint32_t)(rows / height + (own ? own : 1));
+        cut(p.many, p.many.slots * kv_heads, keys, kManyKeys, kManyGroups);
+    }
+    const uint64_t pieces = p.few.pieces > p.many.pieces ? p.few.pieces : p.many.pieces;
+    if (pieces > 1) p.bytes = (size_t)pieces * tokens * heads * (held_dim(dim) + 2) * 4;
+    return p;
+}
+
+}  // namespace q8

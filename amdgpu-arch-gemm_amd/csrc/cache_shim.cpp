@@ -34,8 +34,9 @@ int check_cache(const q8_cache* c) {
 int check_batch(const q8_batch* b, const q8_cache* c) {
     if (!b) return fail(SGEMM_E_INVALID, "batch is null");
     if (b->tokens >= (1u << 31) || b->seqs >= (1u << 31)) return fail(SGEMM_E_SHAPE, "batch: tokens and sequences have 31 bits");
-    if ((uint64_t)b->width * c->page_tokens >= (1ull << 31))
-        return fail(SGEMM_E_SHAPE, "batch: %u pages of %u tokens: positions have 31 bits", b->width, c->page_tokens);
+    // kernels look some steps past a sequence's end, still in 31 bits
+    if ((uint64_t)b->width * c->page_tokens >= (1ull << 31) - (1u << 16))
+        return fail(SGEMM_E_SHAPE, "batch: %u pages of %u tokens: positions end at 2^31 - 2^16", b->width, c->page_tokens);
     return SGEMM_OK;
 }
 
@@ -98,10 +99,16 @@ int cache_rows(q8_handle* h, int dtype, const q8_cache* cache, const q8_batch* b
                  : launched(launch_cache_read(dtype, p, h->stream), "launch of the cache's reading failed");
 }
 
-int check_heads(uint32_t heads, const q8_cache* cache) {
-    if (!heads || heads % cache->heads)
-        return fail(SGEMM_E_SHAPE, "%u heads are no multiple of the cache's %u", heads, cache->heads);
-    return check_columns(heads, cache->dim);
+int plan(int dtype, const q8_cache& c, const q8_batch& b, uint32_t heads, AttentionPlan& p) {
+    if (!heads || heads % c.heads) return fail(SGEMM_E_SHAPE, "%u heads are no multiple of the cache's %u", heads, c.heads);
+    CHECK(check_columns(heads, c.dim));
+    if ((uint64_t)b.tokens * heads >= (1ull << 31)) return fail(SGEMM_E_SHAPE, "%u tokens of %u heads: rows have 31 bits", b.tokens, heads);
+    p = plan_attention(dtype == Q8_F32, b.tokens, b.seqs, (uint64_t)b.width * c.page_tokens, b.longest, heads, c.heads, c.dim);
+    // 2^32 work-items are one grid's end
+    for (const AttentionLaunch* l : {&p.few, &p.many})
+        if ((uint64_t)l->slots * c.heads * l->pieces >= (1u << 24))
+            return fail(SGEMM_E_SHAPE, "%u tokens of %u heads are more tiles than a grid holds", b.tokens, heads);
+    return SGEMM_OK;
 }
 
 }  // namespace
@@ -151,7 +158,8 @@ int q8_attention(q8_handle* h, int dtype, const q8_cache* cache, const q8_batch*
     CHECK(check_type(dtype));
     CHECK(check_cache(cache));
     CHECK(check_batch(batch, cache));
-    CHECK(check_heads(heads, cache));
+    AttentionPlan p;
+    CHECK(plan(dtype, *cache, *batch, heads, p));
     if (!(scale >= -3.4e38f && scale <= 3.4e38f)) return fail(SGEMM_E_INVALID, "scale is no number");
     if (!batch->tokens || !batch->seqs) return SGEMM_OK;
     Tensors t;
@@ -172,7 +180,16 @@ int q8_attention(q8_handle* h, int dtype, const q8_cache* cache, const q8_batch*
     OnDevice on(h->device);
     HIP_TRY(on.status());
     const Attention a = {paged(*cache, *batch), q, out, lse, ldq, ldo, heads, heads / cache->heads, window, scale};
-    return launched(launch_attention(dtype, a, h->stream), "launch of the attention failed");
+    CHECK(take_workspace(h, p.bytes));
+    for (const AttentionLaunch* l : {&p.few, &p.many}) {
+        if (!l->slots) continue;
+        const uint64_t rows = (uint64_t)l->pieces * batch->tokens * heads;
+        float* sums = l->pieces > 1 ? reinterpret_cast<float*>(h->workspace) : nullptr;
+        const AttentionArgs g = {a, divisor(a.group), l->slots, l->least, l->most, l->piece,
+                                 sums, sums ? sums + rows * held_dim(cache->dim) : nullptr, h->tickets};
+        CHECK(launched((l == &p.few ? launch_few : launch_many)(dtype, g, l->pieces, h->stream), "launch of the attention failed"));
+    }
+    return SGEMM_OK;
 }
 
 int q8_attention_workspace(int dtype, const q8_cache* cache, const q8_batch* batch, uint32_t heads, size_t* bytes) {
@@ -181,7 +198,10 @@ int q8_attention_workspace(int dtype, const q8_cache* cache, const q8_batch* bat
     CHECK(check_type(dtype));
     CHECK(check_cache(cache));
     CHECK(check_batch(batch, cache));
-    return check_heads(heads, cache);
+    AttentionPlan p;
+    CHECK(plan(dtype, *cache, *batch, heads, p));
+    *bytes = p.bytes;
+    return SGEMM_OK;
 }
 
 }  // extern "C"

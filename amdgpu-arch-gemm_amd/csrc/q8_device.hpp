@@ -9,6 +9,8 @@
 
 namespace q8 {
 
+template <int V> struct Int { static constexpr int value = V; };
+
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef int i32x4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));

@@ -22,6 +22,7 @@ struct q8_handle {
     size_t workspace_bytes = 0;
     Retired* retired = nullptr;    // workspaces that captured calls may still use
     bool captured = false;         // a call that used the workspace was captured
+    uint32_t* tickets = nullptr;   // kTickets zeros of device memory, zeros again after each launch that uses them
 };
 
 namespace q8 {

@@ -16,8 +16,6 @@
 namespace q8 {
 namespace {
 
-template <int V> struct Int { static constexpr int value = V; };
-
 // Work-groups that a launch has at most; they take their rows in turn.
 constexpr uint32_t kMostGroups = 1u << 20;
 

@@ -1,5 +1,6 @@
 // Host side of the 8-bit operators (include/q8_shim.h): handles, argument checks,
 // workspace, and which kernels a call runs on.
+#include "cache_plan.hpp"
 #include "q8_host.hpp"
 #include "q8_plan.hpp"
 
@@ -59,8 +60,13 @@ int q8_open(q8_handle** out) {
     if (e == hipSuccess) e = prepare_products();
     if (e == hipSuccess) e = prepare_gradients();
     if (e == hipSuccess) e = prepare_cache_rows();
-    if (e == hipSuccess) e = prepare_attention();
+    if (e == hipSuccess) e = prepare_few();
+    if (e == hipSuccess) e = prepare_many();
+    if (e == hipSuccess) e = hipMalloc(reinterpret_cast<void**>(&h->tickets), kTickets * sizeof(uint32_t));
+    if (e == hipSuccess) e = hipMemsetAsync(h->tickets, 0, kTickets * sizeof(uint32_t), h->own_stream);
+    if (e == hipSuccess) e = hipStreamSynchronize(h->own_stream);
     if (e != hipSuccess) {
+        if (h->tickets) (void)hipFree(h->tickets);
         if (h->own_stream) (void)hipStreamDestroy(h->own_stream);
         delete h;
         return hip_fail(e, "q8_open");
@@ -81,6 +87,7 @@ void q8_close(q8_handle* h) {
         (void)hipFree(r->memory);
         delete r;
     }
+    if (h->tickets) (void)hipFree(h->tickets);
     if (h->own_stream) (void)hipStreamDestroy(h->own_stream);
     delete h;
 }

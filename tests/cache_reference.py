@@ -85,11 +85,12 @@ class Case:
                 yield b, token, int(self.lengths[b]) - min(int(end), self.tokens) + token
 
     def attention(self, q, scale, window):
-        """out, lse, and per row: the sums of |weight v| and the largest sum of |products| of a score."""
+        """out, lse, and per row: the sums of |weight v|, the largest sum of |products| of a score, and the sums of |v|'s steps
+        times the largest weight of a step (its key's weight times the values' scale)."""
         group = self.heads // self.kv_heads
         q = q.reshape(-1, self.heads, self.dim)
         out, lse = np.zeros(q.shape), np.full(q.shape[:2], -np.inf)
-        spread, products = np.zeros(q.shape), np.zeros(q.shape[:2])
+        spread, products, steps = np.zeros(q.shape), np.zeros(q.shape[:2]), np.zeros(q.shape)
         held = {}
         for b, token, p in self.rows():
             if b not in held:
@@ -98,9 +99,9 @@ class Case:
                 page = self.table[b, at // self.page].astype(np.int64)
                 there = (page >= 0) & (page < self.pages)
                 page = np.where(there, page, 0)
-                held[b] = (there, *(c[page, :, at % self.page, : self.dim].astype(np.float64) * s[page, :, at % self.page].astype(np.float64)[..., None]
+                held[b] = (there, self.sv[page, :, at % self.page].astype(np.float64), *(c[page, :, at % self.page, : self.dim].astype(np.float64) * s[page, :, at % self.page].astype(np.float64)[..., None]
                                     for c, s in ((self.k, self.sk), (self.v, self.sv))))
-            there, k, v = held[b]
+            there, sv, k, v = held[b]
             at = np.arange(len(there))
             seen = there & (at <= p) & ((at > p - window) if window else True)
             if not seen.any():
@@ -114,19 +115,24 @@ class Case:
                 out[token, h] = w @ vv / total
                 lse[token, h] = m + np.log(total)
                 spread[token, h] = w @ np.abs(vv) / total
+                s = sv[seen, h // group]
+                steps[token, h] = (w * s).max() * np.abs(vv / s[:, None]).sum(0) / total
                 products[token, h] = (np.abs(kk) @ np.abs(q[token, h])).max() * abs(scale)
-        return out, lse, spread, products
+        return out, lse, (spread, products, steps)
 
-    def bounds(self, out, lse, spread, products, dtype):
+    def bounds(self, out, lse, sums, dtype):
         """How far out and lse may be off: the scores' products and sums in FP32 (an error of dim + 8 roundings of the
         largest sum of products: the dim - 1 additions, four factors, the exponential's argument and its base), which the
         weights follow to first order, twice, for numerator and sum; exp2 to 2^-22; as many roundings again as keys for the
-        sums; the weights' rounding to 11 bits for 16-bit types (another 2^-23 of a term cut off for F32); the result's rounding.  The second order of these (below 2^-10 of them) is
-        in the factor 1.01."""
+        sums; the weights' rounding to 11 bits for 16-bit types (another 2^-23 of a term cut off for F32); the result's rounding.
+        Half precision's steps are 2^-24 at the least, a weight (times its scale) is off by half of one; the row's largest is 2^6 or
+        more when it is rounded, as R is moved only to bring it there, so the error is 2^-31 of that one.  The second order of
+        these (below 2^-10 of them) is in the factor 1.01."""
+        spread, products, steps = sums
         keys = max([1] + [int(n) for n in self.lengths])
         score = (self.dim + 8) * 2.0 ** -24 * products + 2.0 ** -22 * np.where(np.isfinite(lse), np.abs(lse), 0)
-        sums = (keys + 8) * 2.0 ** -24
+        adds = (keys + 8) * 2.0 ** -24
         weight = 2.0 ** -11 if dtype != "f32" else 2.0 ** -22
-        rel = 1.01 * (2 * score + 2.0 ** -21 + 2 * sums + weight)
-        off = spread * rel[..., None]
-        return off + (np.abs(out) + off) * UNIT[dtype] + TINY[dtype], 1.01 * (score + sums + 2.0 ** -21) + np.where(np.isfinite(lse), np.abs(lse), 0) * 2.0 ** -22
+        rel = 1.01 * (2 * score + 2.0 ** -21 + 2 * adds + weight)
+        off = spread * rel[..., None] + (0 if dtype == "f32" else 1.01 * 2.0 ** -31 * steps)
+        return off + (np.abs(out) + off) * UNIT[dtype] + TINY[dtype], 1.01 * (score + adds + 2.0 ** -21) + np.where(np.isfinite(lse), np.abs(lse), 0) * 2.0 ** -22

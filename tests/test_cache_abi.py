@@ -71,7 +71,7 @@ def test_sizes_that_are_refused():
     workspace(-4, "31 bits", cache=(2 ** 31, 1, 1, 16))
     workspace(-4, "31 bits", batch=(2, 2 ** 31, 4))
     workspace(-4, "31 bits", batch=(2 ** 31, 2, 4))
-    workspace(-4, "31 bits", batch=(2, 2, 2 ** 27))
+    workspace(-4, "positions", batch=(2, 2, 2 ** 27 - 4096))
     workspace(-4, "no multiple", heads=3)
     workspace(-4, "no multiple", heads=0)
     workspace(-4, "2^24", heads=2 ** 18)

@@ -24,8 +24,8 @@ def check(ops, rng, case, dtype, window=0, scale=None, pad=0, shift=0, spread=1.
     wl = Window(1, case.tokens * case.heads, C.F32) if lse else None
     ops.attention(kind, cache, batch, case.heads, wq, wo, wl, scale=scale, window=window, ldq=wq.ld, ldo=wo.ld)
     ops.synchronize()
-    out, want_lse, sums, products = case.attention(q, case.dim ** -0.5 if scale is None else scale, window)
-    off, off_lse = case.bounds(out, want_lse, sums, products, dtype)
+    out, want_lse, sums = case.attention(q, case.dim ** -0.5 if scale is None else scale, window)
+    off, off_lse = case.bounds(out, want_lse, sums, dtype)
     got = wo.values().reshape(case.tokens, case.heads, case.dim)
     mine = np.zeros(case.tokens, bool)
     for _, token, _ in case.rows():
