@@ -178,6 +178,22 @@ template <typename F> hipError_t for_head(int dtype, uint32_t dim, const F& f) {
     return dtype == Q8_F32 ? held(Int<Q8_F32>{}) : dtype == Q8_F16 ? held(Int<Q8_F16>{}) : held(Int<Q8_BF16>{});
 }
 
+// Eight of a row's values from d on, zeros past dim.  (Without branches: of a row's pieces, as many as DP / 8, each would
+// have its own.)
+template <int DT> __device__ __forceinline__ void query(const typename Type<DT>::T* row, uint32_t d, uint32_t dim, float (&v)[8]) {
+    if (dim % 8 == 0) {
+        Type<DT>::load8(row + (d < dim ? d : 0), v);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = d < dim ? v[e] : 0.0f;
+    } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            const float x = Type<DT>::get(row + min(d + e, dim - 1));
+            v[e] = d + e < dim ? x : 0.0f;
+        }
+    }
+}
+
 // Sums of some keys with those of others.
 __device__ __forceinline__ void add_part(float& R, float& l, float (&v)[8], float r, float lr, const float (&o)[8]) {
     const float next = fmaxf(R, r), down = __builtin_amdgcn_exp2f(R - next), part = __builtin_amdgcn_exp2f(r - next);

@@ -141,8 +141,8 @@ template <int DT, int DP> __global__ void __launch_bounds__(64 * kWaves, DP == 2
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
                 const uint32_t d = s * 64 + grp * 16 + h * 8;
-                float v[8] = {};
-                if (mine && d < c.dim) load_part<DT>(row, d, c.dim, v);
+                float v[8];
+                query<DT>(row, d, c.dim, v);
                 terms_of<TERMS, F::QH>(v, q[s][h]);
             }
     }

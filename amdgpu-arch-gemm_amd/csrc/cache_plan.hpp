@@ -19,7 +19,7 @@ constexpr uint64_t up(uint64_t a, uint64_t b) { return (a + b - 1) / b; }
 
 // Values of a head as the kernels hold them.
 constexpr uint32_t held_dim(uint32_t dim) { return dim <= 64 ? 64 : dim <= 128 ? 128 : 256; }
-// Rows of a tile of many: 32 or 64 a wave.
+// Rows of a tile of many: 32 a wave, of eight waves, or of four that have the registers of two each.
 constexpr uint32_t many_rows(bool f32, uint32_t dim) { return f32 || dim > 128 ? 128 : 256; }
 
 struct AttentionLaunch {
