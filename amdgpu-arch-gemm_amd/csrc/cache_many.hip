@@ -29,7 +29,6 @@ template <int DT, int DP> struct Many {
         u32x4 k[2][64 * (DP / 8)];
         u32x4 v[2][DP * 8];
         uint64_t offset[W][64];
-        int last;
     };
 };
 
@@ -254,53 +253,22 @@ template <int DT, int DP> __global__ void __launch_bounds__((Many<DT, DP>::THREA
         if (more && there) store(buffer ^ 1);
     }
 
-    // Rows' results; of pieces their sums, which the work-group that finishes the tile's last piece adds in their order.
     l += __shfl_xor(l, 32);
-    const uint64_t stride = (uint64_t)c.tokens * a.heads, to = at.row * a.heads + at.head;
-    if (pieces > 1) {
-        if (mine) {
-            const uint64_t own = piece * stride + to;
-#pragma unroll
-            for (int d = 0; d < D; ++d)
-#pragma unroll
-                for (int i = 0; i < 16; i += 2)
-                    publish(g.sums + own * DP + d * 32 + (i >> 2) * 8 + half * 4 + (i & 3), o[d][i], o[d][i + 1]);
-            if (half == 0) publish(g.stats + 2 * own, R, l);
-        }
-        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");        // this wave's stores have arrived
-        __syncthreads();
-        if (tid == 0) {
-            uint32_t* ticket = g.tickets + blockIdx.x;
-            shared.last = __hip_atomic_fetch_add(ticket, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == (uint32_t)pieces - 1;
-            if (shared.last) __hip_atomic_store(ticket, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        }
-        __syncthreads();
-        if (!shared.last) return;
-        R = kUnset;
-        l = 0.0f;
+    if (!mine) return;
+    const uint64_t to = at.row * a.heads + at.head;
+    if (pieces > 1) {       // join_kernel's
+        const uint64_t own = (uint64_t)piece * c.tokens * a.heads + to;
 #pragma unroll
         for (int d = 0; d < D; ++d)
 #pragma unroll
-            for (int i = 0; i < 16; ++i) o[d][i] = 0.0f;
-        for (int p = 0; p < pieces; ++p) {
-            const uint64_t own = p * stride + to;
-            float r, lp;
-            published(g.stats + 2 * own, r, lp);
-            const float next = fmaxf(R, r), down = __builtin_amdgcn_exp2f(R - next), part = __builtin_amdgcn_exp2f(r - next);
-            R = next;
-            l = l * down + lp * part;
-#pragma unroll
-            for (int d = 0; d < D; ++d)
-#pragma unroll
-                for (int i = 0; i < 16; i += 2) {
-                    float x, y;
-                    published(g.sums + own * DP + d * 32 + (i >> 2) * 8 + half * 4 + (i & 3), x, y);
-                    o[d][i] = o[d][i] * down + x * part;
-                    o[d][i + 1] = o[d][i + 1] * down + y * part;
-                }
+            for (int i = 0; i < 16; i += 4)
+                *reinterpret_cast<f32x4*>(g.sums + own * DP + d * 32 + i * 2 + half * 4) = f32x4{o[d][i], o[d][i + 1], o[d][i + 2], o[d][i + 3]};
+        if (half == 0) {
+            g.stats[2 * own] = R;
+            g.stats[2 * own + 1] = l;
         }
+        return;
     }
-    if (!mine) return;
     const float part = l == 0.0f ? 0.0f : 1.0f / l;
     T* out = (T*)a.out + at.row * a.ldo + at.head * c.dim;
 #pragma unroll
@@ -313,10 +281,50 @@ template <int DT, int DP> __global__ void __launch_bounds__((Many<DT, DP>::THREA
     if (a.lse && half == 0) a.lse[to] = l == 0.0f ? -__builtin_huge_valf() : (R + __builtin_log2f(l)) * kLn2;
 }
 
+// The pieces' sums of a tile's rows: DP / 8 threads a row, 2048 / DP rows a work-group.  (A work-group of the kernel before
+// that finishes a tile and adds them alone reads for longer than all work-groups together: 64 tokens over 8192 keys,
+// 32 pieces, 195 us.)
+template <int DT, int DP> __global__ void __launch_bounds__(256) join_kernel(const AttentionArgs g) {
+    typedef typename Type<DT>::T T;
+    constexpr int ACROSS = DP / 8;
+    const Attention& a = g.a;
+    const Paged& c = a.at;
+    const uint32_t kv = blockIdx.x % c.heads;
+    Place t;
+    if (!find_tile(g, g.slots - 1 - blockIdx.x / c.heads, 32 * Many<DT, DP>::W, t)) return;
+    const int pieces = pieces_of(t, g.piece), r = blockIdx.y * (256 / ACROSS) + threadIdx.x / ACROSS, d = threadIdx.x % ACROSS * 8;
+    if (pieces <= 1 || r >= t.rows) return;
+    const Row at = row_of(g, t, kv, r);
+    const uint64_t stride = (uint64_t)c.tokens * a.heads, to = at.row * a.heads + at.head;
+    float R = kUnset, l = 0.0f, v[8] = {};
+    constexpr int AHEAD = 4;
+    for (int p = 0; p < pieces; p += AHEAD) {
+        float o[AHEAD][8], rp[AHEAD], lp[AHEAD];
+#pragma unroll
+        for (int i = 0; i < AHEAD; ++i) {
+            const uint64_t from = to + (uint64_t)min(p + i, pieces - 1) * stride;
+            rp[i] = g.stats[2 * from];
+            lp[i] = g.stats[2 * from + 1];
+            Type<Q8_F32>::load8(g.sums + from * DP + d, o[i]);
+        }
+#pragma unroll
+        for (int i = 0; i < AHEAD; ++i)
+            if (p + i < pieces) add_part(R, l, v, rp[i], lp[i], o[i]);
+    }
+    const float part = l == 0.0f ? 0.0f : 1.0f / l;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] *= part;
+    if (d < (int)c.dim) store_part<DT>((T*)a.out + at.row * a.ldo + at.head * c.dim, d, c.dim, v);
+    if (a.lse && d == 0) a.lse[to] = l == 0.0f ? -__builtin_huge_valf() : (R + __builtin_log2f(l)) * kLn2;
+}
+
 template <int DT, int DP> hipError_t run(const AttentionArgs& g, uint32_t pieces, hipStream_t s) {
     void* args[] = {const_cast<AttentionArgs*>(&g)};
-    return hipLaunchKernel(reinterpret_cast<const void*>(&many_kernel<DT, DP>), dim3(g.slots * g.a.at.heads, pieces),
-                           dim3(Many<DT, DP>::THREADS), args, 0, s);
+    typedef Many<DT, DP> F;
+    const uint32_t tiles = g.slots * g.a.at.heads;
+    const hipError_t e = hipLaunchKernel(reinterpret_cast<const void*>(&many_kernel<DT, DP>), dim3(tiles, pieces), dim3(F::THREADS), args, 0, s);
+    if (e != hipSuccess || pieces == 1) return e;
+    return hipLaunchKernel(reinterpret_cast<const void*>(&join_kernel<DT, DP>), dim3(tiles, 32 * F::W * DP / 2048), dim3(256), args, 0, s);
 }
 
 }  // namespace
