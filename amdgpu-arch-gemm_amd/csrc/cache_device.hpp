@@ -14,19 +14,13 @@ __device__ __forceinline__ uint32_t divide(uint32_t n, const Divisor& by) {     
 __device__ __forceinline__ int chunk_begin(const Paged& c, uint32_t b) { return min(max(c.starts[b], 0), (int)c.tokens); }
 __device__ __forceinline__ int chunk_end(const Paged& c, uint32_t b) { return min(max(c.starts[b + 1], 0), (int)c.tokens); }
 
-// The page that holds position p of sequence b, or -1.
-__device__ __forceinline__ int page_at(const Paged& c, uint32_t b, uint32_t index) {
-    if (index >= c.width) return -1;
-    const int page = c.table[(uint64_t)b * c.table_ld + index];
-    return (uint32_t)page < c.pages ? page : -1;
-}
-
 // Row of head 0 for position p of sequence b, or -1 (p may be anything).
 __device__ __forceinline__ int64_t row_at(const Paged& c, uint32_t b, int64_t p) {
     if (p < 0 || p >= 0x7fffffff) return -1;
     const uint32_t index = divide((uint32_t)p, c.page);
-    const int page = page_at(c, b, index);
-    return page < 0 ? -1 : (int64_t)page * c.heads * c.page_tokens + ((uint32_t)p - index * c.page_tokens);
+    if (index >= c.width) return -1;
+    const int page = c.table[(uint64_t)b * c.table_ld + index];
+    return (uint32_t)page >= c.pages ? -1 : (int64_t)page * c.heads * c.page_tokens + ((uint32_t)p - index * c.page_tokens);
 }
 
 }  // namespace q8

@@ -45,7 +45,7 @@ template <int DT, int DP> __global__ void __launch_bounds__(64 * kWaves, DP == 2
     if (!find_tile(g, blockIdx.x / c.heads, 16, t)) return;
     const int pieces = max(1, pieces_of(t, g.piece));
     if ((int)piece >= pieces) return;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, n = lane & 15, grp = lane >> 4;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n = lane & 15, grp = lane >> 4;
     const int begin = t.begin + (int)(piece * g.piece), end = min(t.end, begin + (int)g.piece);
 
     // this lane's row of the scores
@@ -65,16 +65,16 @@ template <int DT, int DP> __global__ void __launch_bounds__(64 * kWaves, DP == 2
     for (int j = 0; j < F::BYTES; ++j) o[j] = f32x4{0, 0, 0, 0};
 
     const int64_t head_rows = (int64_t)kv * c.page_tokens, page_rows = (int64_t)c.heads * c.page_tokens;
-    // page of this lane's key (lane % 32) of the step from key k
-    auto page_of = [&](int k) __attribute__((always_inline)) {
-        const int key = k + (lane & 31);
-        return key < end ? page_at(c, t.b, divide((uint32_t)key, c.page)) : -1;
-    };
+    // What the table says of this lane's key (lane % 32) of the step from key k.  Not looked at before the step's loads: a
+    // wait for it would be one for all loads before it.
+    const int32_t* pages = c.table + (uint64_t)t.b * c.table_ld;
+    auto page_of = [&](int k) __attribute__((always_inline)) { return pages[divide((uint32_t)min(k + (lane & 31), end - 1), c.page)]; };
     // Where the step's keys lie; rows of keys that are not there become those of one that is, and what the padding
     // holds meets zeros of q.
     uint64_t* offset = shared.stage.offset[wave];
     float* factors = shared.stage.scale[wave];
     auto locate = [&](int k, int page, uint32_t& there, float& scale) __attribute__((always_inline)) {
+        page = k + (lane & 31) < end && (uint32_t)kept(page) < c.pages ? page : -1;
         there = (uint32_t)__ballot(page >= 0);
         if (!there) return;
         const uint32_t key = (uint32_t)(k + (lane & 31)), slot = key - divide(key, c.page) * c.page_tokens;

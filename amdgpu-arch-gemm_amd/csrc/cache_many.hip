@@ -25,18 +25,17 @@ template <int DT, int DP> struct Many {
     static constexpr int KEY_UNITS = 64 * (DP / 16), KEY_LOADS = (KEY_UNITS + THREADS / 2 - 1) / (THREADS / 2);   // 16 bytes each
     static constexpr int VALUE_UNITS = 8 * (DP / 4), VALUE_LOADS = (VALUE_UNITS + THREADS / 2 - 1) / (THREADS / 2);  // eight keys of four values
     static constexpr int HELD = KEY_LOADS * 4 > VALUE_LOADS * 8 ? KEY_LOADS * 4 : VALUE_LOADS * 8;
-    struct Shared {
-        u32x4 k[2][64 * (DP / 8)];
-        u32x4 v[2][DP * 8];
-        uint64_t offset[W][64];
-    };
+    // bytes of LDS: keys and values twice
+    static constexpr int KEY_ROW = DP * 2, VALUE_ROW = 128, KEYS = 64 * KEY_ROW, VALUES = DP * VALUE_ROW;
+    static constexpr uint32_t KEY_TURN = DP / 8 < 16 ? 7 : 15;
 };
 
 template <int DT, int DP> __global__ void __launch_bounds__((Many<DT, DP>::THREADS), (Many<DT, DP>::W / 4)) many_kernel(const AttentionArgs g) {
     typedef Many<DT, DP> F;
     typedef typename Type<DT>::T T;
     constexpr int TERMS = F::TERMS, S = DP / 16, D = DP / 32;
-    __shared__ typename F::Shared shared;
+    __shared__ __attribute__((aligned(16))) char lds[2 * (F::KEYS + F::VALUES)];
+    __shared__ uint64_t offsets[F::W][64];
     const Attention& a = g.a;
     const Paged& c = a.at;
     const uint32_t kv = blockIdx.x % c.heads, piece = blockIdx.y;
@@ -45,17 +44,18 @@ template <int DT, int DP> __global__ void __launch_bounds__((Many<DT, DP>::THREA
     if (!find_tile(g, g.slots - 1 - blockIdx.x / c.heads, 32 * F::W, t)) return;
     const int pieces = max(1, pieces_of(t, g.piece));
     if ((int)piece >= pieces) return;
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, n = lane & 31, half = lane >> 5;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), n = lane & 31, half = lane >> 5;
     const int begin = t.begin + (int)(piece * g.piece), end = min(t.end, begin + (int)g.piece);
 
     // this lane's row; those past the tile's are its last
     const bool mine = wave * 32 + n < t.rows;
     const Row at = row_of(g, t, kv, min(wave * 32 + n, t.rows - 1));
     const int position = t.at + ((int)at.row - t.first);
-    const int64_t oldest = a.window ? (int64_t)position - a.window + 1 : INT32_MIN;
+    auto window_of = [&](int p) { return a.window && p - (int64_t)a.window + 1 > INT32_MIN ? (int)(p - (int64_t)a.window + 1) : INT32_MIN; };
+    const int oldest = window_of(position);
     // of this wave's rows: the first's and the last's position (-1: no rows, nothing to compute)
     const int low = __builtin_amdgcn_readlane(position, 0), high = wave * 32 < t.rows ? __builtin_amdgcn_readlane(position, 31) : -1;
-    const int64_t all_from = a.window ? (int64_t)high - a.window + 1 : INT32_MIN, none_to = a.window ? (int64_t)low - a.window + 1 : INT32_MIN;
+    const int all_from = window_of(high), none_to = window_of(low);
 
     u32x4 q[S][TERMS];
     {
@@ -76,10 +76,11 @@ template <int DT, int DP> __global__ void __launch_bounds__((Many<DT, DP>::THREA
         for (int i = 0; i < 16; ++i) o[d][i] = 0.0f;
 
     const int64_t head_rows = (int64_t)kv * c.page_tokens, page_rows = (int64_t)c.heads * c.page_tokens;
-    auto page_of = [&](int k) __attribute__((always_inline)) {
-        return k + lane < end ? page_at(c, t.b, divide((uint32_t)(k + lane), c.page)) : -1;
-    };
-    uint64_t* offset = shared.offset[wave];
+    // What the table says of this lane's key of the step from key k.  Not looked at before the step's loads: a wait for it
+    // would be one for all loads before it.
+    const int32_t* pages = c.table + (uint64_t)t.b * c.table_ld;
+    auto page_of = [&](int k) __attribute__((always_inline)) { return pages[divide((uint32_t)min(k + lane, end - 1), c.page)]; };
+    uint64_t* offset = offsets[wave];
     const bool values = wave < F::W / 2;
     const int worker = values ? tid : tid - F::THREADS / 2;
     uint32_t held[F::HELD];
@@ -87,6 +88,7 @@ template <int DT, int DP> __global__ void __launch_bounds__((Many<DT, DP>::THREA
     // A step's loads; every wave finds all 64 keys for itself.  Rows of keys that are not there become those of one that
     // is; 0: none is.
     auto load = [&](int k, int page) __attribute__((always_inline)) {
+        page = k + lane < end && (uint32_t)kept(page) < c.pages ? page : -1;
         const uint64_t there = __ballot(page >= 0);
         if (!there) return there;
         const uint32_t key = (uint32_t)(k + lane), slot = key - divide(key, c.page) * c.page_tokens;
@@ -132,7 +134,8 @@ template <int DT, int DP> __global__ void __launch_bounds__((Many<DT, DP>::THREA
                 u32x4 r[4];
                 columns<F::VH>(w, r);
 #pragma unroll
-                for (int j = 0; j < 4; ++j) shared.v[to][(d + j) * 8 + (part ^ ((d + j) & 7))] = r[j];
+                for (int j = 0; j < 4; ++j)
+                    *reinterpret_cast<u32x4*>(lds + 2 * F::KEYS + to * F::VALUES + (d + j) * F::VALUE_ROW + (part ^ ((d + j) & 7)) * 16) = r[j];
             }
         } else {
 #pragma unroll
@@ -142,7 +145,8 @@ template <int DT, int DP> __global__ void __launch_bounds__((Many<DT, DP>::THREA
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
                     const u32x2 w0 = four<F::QH>(kept(held[4 * x + 2 * h])), w1 = four<F::QH>(kept(held[4 * x + 2 * h + 1]));
-                    shared.k[to][key_of * (DP / 8) + ((part + h) ^ (key_of & (DP / 8 < 16 ? 7 : 15)))] = u32x4{w0[0], w0[1], w1[0], w1[1]};
+                    *reinterpret_cast<u32x4*>(lds + to * F::KEYS + key_of * F::KEY_ROW + ((part + h) ^ (key_of & F::KEY_TURN)) * 16) =
+                        u32x4{w0[0], w0[1], w1[0], w1[1]};
                 }
             }
         }
@@ -155,20 +159,30 @@ template <int DT, int DP> __global__ void __launch_bounds__((Many<DT, DP>::THREA
         return u32x4{on ? uppers(b[0], b[1]) : 0u, on ? b[2] >> 16 : 0u, 0u, 0u};
     };
     const u32x4 ones = {0x3f803f80u, 0x3f803f80u, 0, 0};
+    // where this lane reads: a place's piece is turned by what the row's number turns, so another piece is an exclusive or away
+    const uint32_t key_at = n * F::KEY_ROW + ((half ^ (n & F::KEY_TURN)) * 16), value_at = 2 * F::KEYS + n * F::VALUE_ROW + ((half ^ (n & 7)) * 16);
     // 32 keys from k, the i-th half of a step's
     auto compute = [&](int from, int i, int k, uint32_t there, float sk_mine, float sv_mine) __attribute__((always_inline)) {
         if (!there || k > high || k + 31 < none_to) return;
         f32x16 score, sk, sv;
 #pragma unroll
         for (int e = 0; e < 16; ++e) score[e] = sk[e] = sv[e] = 0.0f;
-        mfma32<false>(terms_in(sk_mine, i), ones, sk);
-        mfma32<false>(terms_in(sv_mine, i), ones, sv);
+        constexpr int AT_ONCE = S < 8 ? S : 8;
 #pragma unroll
-        for (int s = 0; s < S; ++s) {
-            const int key_of = i * 32 + n;
-            const u32x4 w = shared.k[from][key_of * (DP / 8) + ((2 * s + half) ^ (key_of & (DP / 8 < 16 ? 7 : 15)))];
+        for (int s0 = 0; s0 < S; s0 += AT_ONCE) {
+            u32x4 w[AT_ONCE];
 #pragma unroll
-            for (int m = 0; m < TERMS; ++m) mfma32<F::QH>(w, q[s][m], score);
+            for (int s = 0; s < AT_ONCE; ++s)
+                w[s] = *reinterpret_cast<const u32x4*>(lds + from * F::KEYS + i * 32 * F::KEY_ROW + (key_at ^ ((s0 + s) * 32)));
+            __builtin_amdgcn_sched_barrier(0);
+            if (s0 == 0) {
+                mfma32<false>(terms_in(sk_mine, i), ones, sk);
+                mfma32<false>(terms_in(sv_mine, i), ones, sv);
+            }
+#pragma unroll
+            for (int s = 0; s < AT_ONCE; ++s)
+#pragma unroll
+                for (int m = 0; m < TERMS; ++m) mfma32<F::QH>(w[s], q[s0 + s][m], score);
         }
         const bool whole = there == 0xffffffffu && k + 31 <= low && k >= all_from;
         uint32_t seen = 0xffff;
@@ -220,21 +234,29 @@ template <int DT, int DP> __global__ void __launch_bounds__((Many<DT, DP>::THREA
             const float x[8] = {w[8 * j], w[8 * j + 1], w[8 * j + 2], w[8 * j + 3], w[8 * j + 4], w[8 * j + 5], w[8 * j + 6], w[8 * j + 7]};
             terms_of<TERMS, F::VH>(x, weight[j]);
         }
+        constexpr int D_AT_ONCE = D < 4 ? D : 4;
 #pragma unroll
-        for (int d = 0; d < D; ++d)
+        for (int d0 = 0; d0 < D; d0 += D_AT_ONCE) {
+            u32x4 v[D_AT_ONCE][2];
 #pragma unroll
-            for (int j = 0; j < 2; ++j) {
-                const int row = d * 32 + n;
-                const u32x4 w = shared.v[from][row * 8 + ((i * 4 + j * 2 + half) ^ (row & 7))];
+            for (int d = 0; d < D_AT_ONCE; ++d)
 #pragma unroll
-                for (int m = 0; m < TERMS; ++m) mfma32<F::VH>(w, weight[j][m], o[d]);
-            }
+                for (int j = 0; j < 2; ++j)
+                    v[d][j] = *reinterpret_cast<const u32x4*>(lds + from * F::VALUES + (value_at ^ (i * 64 + j * 32)) + (d0 + d) * 32 * F::VALUE_ROW);
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int j = 0; j < 2; ++j)
+#pragma unroll
+                for (int d = 0; d < D_AT_ONCE; ++d)
+#pragma unroll
+                    for (int m = 0; m < TERMS; ++m) mfma32<F::VH>(v[d][j], weight[j][m], o[d0 + d]);
+        }
     };
 
-    int page = page_of(begin);
+    int page = 0;
     uint64_t there = 0;
     if (begin < end) {
-        there = load(begin, page);
+        there = load(begin, page_of(begin));
         page = page_of(begin + 64);
         if (there) store(0);
     }
