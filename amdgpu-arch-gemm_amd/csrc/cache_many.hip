@@ -27,7 +27,11 @@ template <int DT, int DP> struct Many {
     static constexpr int HELD = KEY_LOADS * 4 > VALUE_LOADS * 8 ? KEY_LOADS * 4 : VALUE_LOADS * 8;
     // bytes of LDS: keys and values twice
     static constexpr int KEY_ROW = DP * 2, VALUE_ROW = 128, KEYS = 64 * KEY_ROW, VALUES = DP * VALUE_ROW;
-    static constexpr uint32_t KEY_TURN = DP / 8 < 16 ? 7 : 15;
+    // What a row turns its pieces by.  Reads of 16 bytes go by 16 lanes a cycle (0-3, 12-15, 20-27 and so on), writes by
+    // eight, over 64 banks: rows of 256 bytes and more need 16 turns, of 128 eight for each of two rows, which bit 4
+    // gives the writes of every fourth row too.
+    static __device__ __forceinline__ uint32_t turn128(uint32_t row) { return ((row >> 1) & 7) ^ ((row >> 4) & 1); }
+    static __device__ __forceinline__ uint32_t key_turn(uint32_t row) { return DP == 64 ? turn128(row) : row & 15; }
 };
 
 template <int DT, int DP> __global__ void __launch_bounds__((Many<DT, DP>::THREADS), (Many<DT, DP>::W / 4)) many_kernel(const AttentionArgs g) {
@@ -135,7 +139,7 @@ template <int DT, int DP> __global__ void __launch_bounds__((Many<DT, DP>::THREA
                 columns<F::VH>(w, r);
 #pragma unroll
                 for (int j = 0; j < 4; ++j)
-                    *reinterpret_cast<u32x4*>(lds + 2 * F::KEYS + to * F::VALUES + (d + j) * F::VALUE_ROW + (part ^ ((d + j) & 7)) * 16) = r[j];
+                    *reinterpret_cast<u32x4*>(lds + 2 * F::KEYS + to * F::VALUES + (d + j) * F::VALUE_ROW + (part ^ F::turn128(d + j)) * 16) = r[j];
             }
         } else {
 #pragma unroll
@@ -145,24 +149,28 @@ template <int DT, int DP> __global__ void __launch_bounds__((Many<DT, DP>::THREA
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
                     const u32x2 w0 = four<F::QH>(kept(held[4 * x + 2 * h])), w1 = four<F::QH>(kept(held[4 * x + 2 * h + 1]));
-                    *reinterpret_cast<u32x4*>(lds + to * F::KEYS + key_of * F::KEY_ROW + ((part + h) ^ (key_of & F::KEY_TURN)) * 16) =
+                    *reinterpret_cast<u32x4*>(lds + to * F::KEYS + key_of * F::KEY_ROW + ((part + h) ^ F::key_turn(key_of)) * 16) =
                         u32x4{w0[0], w0[1], w1[0], w1[1]};
                 }
             }
         }
     };
-    // three terms of a key's scale for the half of the lanes that has the keys of a half step, zeros for the other
-    auto terms_in = [&](float x, int i) __attribute__((always_inline)) {
+    // three terms of this lane's key's scale, and those for the half of the lanes that has the keys of half step i, zeros for the other
+    auto split = [&](float x) __attribute__((always_inline)) {
         uint32_t b[3];
         three(x, b);
+        return u32x2{uppers(b[0], b[1]), b[2] >> 16};
+    };
+    auto terms_in = [&](u32x2 x, int i) __attribute__((always_inline)) {
         const bool on = half == i;
-        return u32x4{on ? uppers(b[0], b[1]) : 0u, on ? b[2] >> 16 : 0u, 0u, 0u};
+        return u32x4{on ? x[0] : 0u, on ? x[1] : 0u, 0u, 0u};
     };
     const u32x4 ones = {0x3f803f80u, 0x3f803f80u, 0, 0};
     // where this lane reads: a place's piece is turned by what the row's number turns, so another piece is an exclusive or away
-    const uint32_t key_at = n * F::KEY_ROW + ((half ^ (n & F::KEY_TURN)) * 16), value_at = 2 * F::KEYS + n * F::VALUE_ROW + ((half ^ (n & 7)) * 16);
+    const uint32_t key_at = n * F::KEY_ROW + ((half ^ F::key_turn(n)) * 16);
+    const uint32_t value_at = 2 * F::KEYS + n * F::VALUE_ROW + ((half ^ F::turn128(n)) * 16);
     // 32 keys from k, the i-th half of a step's
-    auto compute = [&](int from, int i, int k, uint32_t there, float sk_mine, float sv_mine) __attribute__((always_inline)) {
+    auto compute = [&](int from, int i, int k, uint32_t there, u32x2 sk_mine, u32x2 sv_mine) __attribute__((always_inline)) {
         if (!there || k > high || k + 31 < none_to) return;
         f32x16 score, sk, sv;
 #pragma unroll
@@ -253,26 +261,42 @@ template <int DT, int DP> __global__ void __launch_bounds__((Many<DT, DP>::THREA
         }
     };
 
+    // Steps in flight: the one that is computed, the next one in LDS or on its way there, the one after in registers.
+    // Half of the waves store and load before they compute, the others after, so that of the two on a SIMD one has
+    // conversions for the vector unit while the other has products.
+    constexpr int STEP = 64;
+    uint64_t there = 0, there1 = 0, there2 = 0;
+    float sk = 0.0f, sv = 0.0f, sk1 = 0.0f, sv1 = 0.0f;
     int page = 0;
-    uint64_t there = 0;
     if (begin < end) {
         there = load(begin, page_of(begin));
-        page = page_of(begin + 64);
+        sk = k_scale;
+        sv = v_scale;
         if (there) store(0);
+        there1 = load(begin + STEP, page_of(begin + STEP));
+        sk1 = k_scale;
+        sv1 = v_scale;
+        page = page_of(begin + 2 * STEP);
     }
     int buffer = 0;
-    for (int k = begin; k < end; k += 64, buffer ^= 1) {
-        const uint64_t here = there;
-        const float sk = k_scale * factor, sv = v_scale;
+    for (int k = begin; k < end; k += STEP, buffer ^= 1) {
         __syncthreads();        // this step is in LDS, and the one before is done with its half of it
-        const bool more = k + 64 < end;
-        if (more) {
-            there = load(k + 64, page);
-            page = page_of(k + 128);
-        }
-        compute(buffer, 0, k, (uint32_t)here, sk, sv);
-        compute(buffer, 1, k + 32, (uint32_t)(here >> 32), sk, sv);
-        if (more && there) store(buffer ^ 1);
+        auto forward = [&]() __attribute__((always_inline)) {
+            if (there1) store(buffer ^ 1);
+            there2 = load(k + 2 * STEP, page);
+            page = page_of(k + 3 * STEP);
+        };
+        if (!values) forward();
+        const u32x2 ks = split(sk * factor), vs = split(sv);
+        compute(buffer, 0, k, (uint32_t)there, ks, vs);
+        compute(buffer, 1, k + 32, (uint32_t)(there >> 32), ks, vs);
+        if (values) forward();
+        there = there1;
+        there1 = there2;
+        sk = sk1;
+        sv = sv1;
+        sk1 = k_scale;
+        sv1 = v_scale;
     }
 
     l += __shfl_xor(l, 32);
