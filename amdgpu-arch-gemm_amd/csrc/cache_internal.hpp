@@ -70,8 +70,11 @@ struct AttentionArgs {
     float* sums;        // pieces x tokens x heads x held dim
     float* stats;       // pieces x tokens x heads: R, l
     uint32_t* tickets;  // of each tile: the pieces that are done; 0 before and after a launch
+    char* images;       // null: none; image_bytes() for each sequence, head of the cache and 64 keys
+    uint32_t images_each;   // of a sequence and head
 };
 Q8_INTERNAL hipError_t launch_few(int dtype, const AttentionArgs& g, uint32_t pieces, hipStream_t stream);
 Q8_INTERNAL hipError_t launch_many(int dtype, const AttentionArgs& g, uint32_t pieces, hipStream_t stream);
+Q8_INTERNAL hipError_t launch_prompt(int dtype, const AttentionArgs& g, uint32_t pieces, hipStream_t stream);
 
 }  // namespace q8

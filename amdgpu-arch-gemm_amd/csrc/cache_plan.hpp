@@ -22,6 +22,11 @@ constexpr uint32_t held_dim(uint32_t dim) { return dim <= 64 ? 64 : dim <= 128 ?
 // Rows of a tile of many: 32 a wave, of eight waves, or of four that have the registers of two each.
 constexpr uint32_t many_rows(bool f32, uint32_t dim) { return f32 || dim > 128 ? 128 : 256; }
 
+// 64 keys and values as 16-bit values, and their scales.
+constexpr uint32_t image_bytes(uint32_t held) { return 64 * (held * 2 + 16) + held * 144 + 1024; }
+// Images are made beforehand from so many rows a sequence on, if they take no more workspace than this.
+constexpr uint64_t kImageRows = 1024, kMostImageBytes = 1ull << 30;
+
 struct AttentionLaunch {
     uint32_t slots = 0;         // tiles there may be; 0: no launch
     uint32_t least = 0, most = UINT32_MAX;
@@ -30,7 +35,9 @@ struct AttentionLaunch {
 };
 struct AttentionPlan {
     AttentionLaunch few, many;
-    size_t bytes = 0;           // workspace: the pieces' sums
+    uint32_t images = 0;        // of a sequence and head of the cache, for `many`; 0: none
+    size_t image_bytes = 0;     // workspace: images, then the pieces' sums
+    size_t bytes = 0;
 };
 
 inline void cut(AttentionLaunch& l, uint64_t tiles, uint64_t keys, uint64_t step, uint64_t groups) {
@@ -63,8 +70,14 @@ inline AttentionPlan plan_attention(bool f32, uint64_t tokens, uint64_t seqs, ui
         p.many.slots = (uint32_t)(rows / height + (own ? own : 1));
         cut(p.many, p.many.slots * kv_heads, keys, kManyKeys, kManyGroups);
     }
+    const uint64_t each = up(keys, kManyKeys), image = each * kv_heads * seqs * image_bytes(held_dim(dim));
+    if (many && !f32 && dim <= 128 && rows >= kImageRows * seqs && image && image <= kMostImageBytes && each <= kMostImageBytes) {
+        p.images = (uint32_t)each;
+        p.image_bytes = (size_t)image;
+    }
+    p.bytes = p.image_bytes;
     const uint64_t pieces = p.few.pieces > p.many.pieces ? p.few.pieces : p.many.pieces;
-    if (pieces > 1) p.bytes = (size_t)pieces * tokens * heads * (held_dim(dim) + 2) * 4;
+    if (pieces > 1) p.bytes += (size_t)pieces * tokens * heads * (held_dim(dim) + 2) * 4;
     return p;
 }
 

@@ -184,10 +184,11 @@ int q8_attention(q8_handle* h, int dtype, const q8_cache* cache, const q8_batch*
     for (const AttentionLaunch* l : {&p.few, &p.many}) {
         if (!l->slots) continue;
         const uint64_t rows = (uint64_t)l->pieces * batch->tokens * heads;
-        float* sums = l->pieces > 1 ? reinterpret_cast<float*>(h->workspace) : nullptr;
+        float* sums = l->pieces > 1 ? reinterpret_cast<float*>(h->workspace + p.image_bytes) : nullptr;
         const AttentionArgs g = {a, divisor(a.group), l->slots, l->least, l->most, l->piece,
-                                 sums, sums ? sums + rows * held_dim(cache->dim) : nullptr, h->tickets};
-        CHECK(launched((l == &p.few ? launch_few : launch_many)(dtype, g, l->pieces, h->stream), "launch of the attention failed"));
+                                 sums, sums ? sums + rows * held_dim(cache->dim) : nullptr, h->tickets,
+                                 l == &p.many && p.images ? h->workspace : nullptr, p.images};
+        CHECK(launched((l == &p.few ? launch_few : p.images ? launch_prompt : launch_many)(dtype, g, l->pieces, h->stream), "launch of the attention failed"));
     }
     return SGEMM_OK;
 }

@@ -95,6 +95,7 @@ Q8_INTERNAL hipError_t prepare_gradients();
 Q8_INTERNAL hipError_t prepare_cache_rows();
 Q8_INTERNAL hipError_t prepare_few();
 Q8_INTERNAL hipError_t prepare_many();
+Q8_INTERNAL hipError_t prepare_prompt();
 
 // 8-bit rows to rows of whole 16 bytes: dst[r][0 .. cols) and zeros up to dst_ld.
 Q8_INTERNAL hipError_t launch_copy_rows(const int8_t* src, uint64_t src_ld, int8_t* dst, uint64_t dst_ld, uint32_t rows,

@@ -62,6 +62,7 @@ int q8_open(q8_handle** out) {
     if (e == hipSuccess) e = prepare_cache_rows();
     if (e == hipSuccess) e = prepare_few();
     if (e == hipSuccess) e = prepare_many();
+    if (e == hipSuccess) e = prepare_prompt();
     if (e == hipSuccess) e = hipMalloc(reinterpret_cast<void**>(&h->tickets), kTickets * sizeof(uint32_t));
     if (e == hipSuccess) e = hipMemsetAsync(h->tickets, 0, kTickets * sizeof(uint32_t), h->own_stream);
     if (e == hipSuccess) e = hipStreamSynchronize(h->own_stream);

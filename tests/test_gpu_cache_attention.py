@@ -187,3 +187,25 @@ def test_without_lse_and_without_rows(ops):
     ops.attention(C.BF16, cache, none, 4, q, out, lse)
     ops.synchronize()
     assert not out.numpy().any() and np.all(np.isneginf(lse.numpy()))
+
+
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("dim,page,window", [(128, 16, 0), (128, 7, 100), (64, 64, 0), (33, 16, 300), (256, 16, 90)])
+def test_many_rows(ops, dtype, dim, page, window):
+    """Rows from which on the keys are laid out beforehand (dim up to 128); pages that are not there, a whole step of keys among
+    them; nothing of a sequence's; a chunk longer than its sequence."""
+    rng = np.random.default_rng(13)
+    case = Case(rng, [(300, 700), (0, 9), (250, 250), (270, 200)], 16, 2, dim, page, extra_rows=1, front_rows=1, width_more=1)
+    case.table[0, 3] = -1
+    case.table[0, -(-128 // page): -(-330 // page)] = case.pages
+    case.table[3, :] = -1
+    bad = rng.random(case.sk.shape) < 0.5       # behind the sequences
+    used = np.zeros(case.sk.shape, bool)
+    for b, (_, length) in enumerate(case.sequences):
+        for p in range(length):
+            at = case.place(b, p)
+            if at:
+                used[at[0], :, at[1]] = True
+    case.sk[bad & ~used] = np.nan
+    case.sv[bad & ~used] = np.inf
+    check(ops, rng, case, dtype, window=window)
