@@ -7,13 +7,12 @@
 
 namespace q8 {
 
-constexpr uint64_t kFewGroups = 1024, kManyGroups = 256;
 // Rows of a tile: tokens of one sequence times the heads that share one of the cache's; keys of a step.
 constexpr uint32_t kFewRows = 16, kFewKeys = 128;
 constexpr uint32_t kManyKeys = 64;
-constexpr uint32_t kFewMost = 32;
+constexpr uint32_t kFewMost = 64;
 // Tiles whose keys are taken in pieces, at the most: each has a ticket in the handle.
-constexpr uint32_t kTickets = 4096;
+constexpr uint32_t kTickets = 1u << 16;
 
 constexpr uint64_t up(uint64_t a, uint64_t b) { return (a + b - 1) / b; }
 
@@ -40,10 +39,13 @@ struct AttentionPlan {
     size_t bytes = 0;
 };
 
-inline void cut(AttentionLaunch& l, uint64_t tiles, uint64_t keys, uint64_t step, uint64_t groups) {
+// The keys of a sequence in pieces: as many as make `groups` work-groups of `tiles`, and none longer than `longest` keys; at_most so many.
+inline void cut(AttentionLaunch& l, uint64_t tiles, uint64_t keys, uint64_t step, uint64_t groups, uint64_t longest, uint64_t at_most) {
     const uint64_t steps = up(keys ? keys : 1, step);
-    uint64_t most = tiles && tiles <= kTickets ? groups / tiles : 1;
-    if (most < 1) most = 1;
+    uint64_t most = groups / tiles ? groups / tiles : 1;
+    if (most < up(keys, longest)) most = up(keys, longest);
+    if (most > at_most) most = at_most;
+    if (tiles > kTickets) most = 1;
     const uint64_t each = up(steps, most < steps ? most : steps);
     l.piece = (uint32_t)(each * step);
     l.pieces = (uint32_t)up(steps, each);
@@ -62,13 +64,14 @@ inline AttentionPlan plan_attention(bool f32, uint64_t tokens, uint64_t seqs, ui
             p.few.most = p.many.least = kFewMost;
             if (p.few.slots > filled * up(kFewMost, kFewRows)) p.few.slots = (uint32_t)(filled * up(kFewMost, kFewRows));
         }
-        cut(p.few, p.few.slots * kv_heads, keys, kFewKeys, kFewGroups);
+        cut(p.few, p.few.slots * kv_heads, keys, kFewKeys, seqs > 1 ? 1024 : 512, 4096, UINT32_MAX);
     }
     if (many) {
         const uint32_t height = many_rows(f32, dim);
         const uint64_t own = rows / kFewMost < filled ? rows / kFewMost : filled;      // sequences of more rows than few
         p.many.slots = (uint32_t)(rows / height + (own ? own : 1));
-        cut(p.many, p.many.slots * kv_heads, keys, kManyKeys, kManyGroups);
+        const uint64_t each_cu = !f32 && dim <= 64 ? 512 : 256;
+        cut(p.many, (seqs > 1 ? p.many.slots : up(rows, height)) * kv_heads, keys, kManyKeys, seqs > 1 ? 2 * each_cu : each_cu, UINT32_MAX, 16);
     }
     const uint64_t each = up(keys, kManyKeys), image = each * kv_heads * seqs * image_bytes(held_dim(dim));
     if (many && !f32 && dim <= 128 && rows >= kImageRows * seqs && image && image <= kMostImageBytes && each <= kMostImageBytes) {

@@ -29,8 +29,9 @@ __device__ __forceinline__ void angle(int position, float freq, float& c, float&
 
 // A work-group turns the heads of `p.step` tokens: sine and cosine once for each token and pair, into LDS, and then
 // items of eight pairs (or eight values, of neighbours and of those that stay).  An item's values are
-// read and written by one thread, four items' loads before their stores, so y may be x.
-constexpr uint32_t kAngles = 512;
+// read and written by one thread, two items' loads before their stores, so y may be x.  (16384 tokens of 40 heads of 128, BF16: two tokens
+// a work-group and two items at once 68.6 us, 4.9 TB/s; eight and four 79.1.)
+constexpr uint32_t kAngles = 2 * Q8_MAX_DIM / 2;
 struct RotaryPlan {
     Rotary p;
     uint32_t step;              // tokens a work-group
@@ -54,7 +55,7 @@ template <int DT, bool NEIGHBOURS> __global__ void __launch_bounds__(kThreads) r
         }
         __syncthreads();
         const uint32_t count = tokens * p.heads * a.items;
-        constexpr int AT_ONCE = 4;
+        constexpr int AT_ONCE = 2;
         for (uint32_t i0 = threadIdx.x; i0 < count; i0 += kThreads * AT_ONCE) {
             float v[AT_ONCE][2][8];
             uint32_t token[AT_ONCE], item[AT_ONCE], column[AT_ONCE];
@@ -214,7 +215,7 @@ template <int DT> hipError_t rotary_any(const RotaryPlan& a, hipStream_t s) {
 template <int DT, bool WRITE> hipError_t cache_any(const CacheRows& p, hipStream_t s) {
     const Paged& c = p.at;
     // tokens a work-group: as many as leave each CU some work-groups
-    const uint32_t step = c.tokens >= 8192 ? 8 : c.tokens >= 2048 ? 2 : 1;
+    const uint32_t step = c.tokens >= 8192 ? 16 : c.tokens >= 2048 ? 2 : 1;
     const CachePlan a = {p, step, divisor(c.heads)};
     const uint32_t groups = groups_for(c.tokens, step);
     if (c.dim <= 64) return launch(WRITE ? cache_write_kernel<DT, 8> : cache_read_kernel<DT, 8>, groups, a, s);
@@ -228,8 +229,7 @@ hipError_t launch_rotary(int dtype, const Rotary& p, hipStream_t s) {
     const q8_rotation& f = p.form;
     RotaryPlan a = {};
     a.p = p;
-    const uint32_t most = f.pairs ? kAngles / f.pairs : 8;       // 4 and more
-    a.step = p.tokens >= 1024 ? (most < 8 ? most : 8) : 1;
+    a.step = p.tokens >= 1024 ? 2 : 1;
     a.turned = (uint32_t)ceil_div(f.neighbours ? 2 * f.pairs : f.pairs, 8);
     a.items = a.turned + (p.y == p.x ? 0 : (uint32_t)ceil_div(f.dim - 2 * f.pairs, 8));
     if (!a.items) return hipSuccess;
