@@ -160,7 +160,8 @@ int q8_attention(q8_handle* h, int dtype, const q8_cache* cache, const q8_batch*
     CHECK(check_batch(batch, cache));
     AttentionPlan p;
     CHECK(plan(dtype, *cache, *batch, heads, p));
-    if (!(scale >= -3.4e38f && scale <= 3.4e38f)) return fail(SGEMM_E_INVALID, "scale is no number");
+    // times the exponential's base and a key's scale it stays a number
+    if (!(scale >= -0x1p100f && scale <= 0x1p100f)) return fail(SGEMM_E_INVALID, "scale is not in -2^100 .. 2^100");
     if (!batch->tokens || !batch->seqs) return SGEMM_OK;
     Tensors t;
     CHECK(check_tensors(*cache, *batch, t));

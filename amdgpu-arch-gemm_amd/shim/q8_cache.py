@@ -66,7 +66,10 @@ _p, _check_sizes = Q._p, Q._check_sizes
 
 def ints(a) -> S.DeviceBuffer:
     """`a` on the device as int32 (positions, starts, lengths, tables)."""
+    a = np.asarray(a)
     host = np.ascontiguousarray(a, dtype=np.int32)
+    if not np.array_equal(host, a):
+        raise ValueError("ints: a value that int32 does not hold")
     out = S.DeviceBuffer(max(4, host.nbytes))
     if host.size:
         S._check("sgemm_memcpy_h2d", S.load_library().sgemm_memcpy_h2d(out.ptr, host.ctypes.data, host.nbytes))

@@ -92,7 +92,7 @@ int q8_rotary(q8_handle* h, int dtype, const q8_rotation* form, const void* x, u
 /* Keys and values of the chunks' tokens (rows of cache->heads heads) into their
  * pages, as q8_quantize would round each head.  A token whose page is not
  * there, or whose position is below 0, is left out.  If two tokens have one place,
- * either may be there afterwards. */
+ * what it holds afterwards is not defined. */
 int q8_cache_write(q8_handle* h, int dtype, const q8_cache* cache, const q8_batch* batch, const void* k, uint32_t ldk,
                    const void* v, uint32_t ldv);
 
@@ -108,6 +108,7 @@ int q8_cache_read(q8_handle* h, int dtype, const q8_cache* cache, const q8_batch
  * and to no page that is not there:
  *     t_j = scale sum_d q_d k_jd,  out = sum_j exp(t_j) v_j / sum_j exp(t_j)
  *     lse = log sum_j exp(t_j)           (FP32, tokens x heads; may be NULL)
+ * with scale in -2^100 .. 2^100.
  * A row that attends to nothing is 0, its lse -infinity; one of a NaN scale that it sees is NaN.
  * Rows of no chunk are left as they are.  The scores are FP32 values; one below -2^100 counts as
  * not there.  Sums are in FP32; exp(t_j) sv_j is rounded to 11 bits before its product with the
