@@ -1,5 +1,5 @@
 // Interface between the host code of the cache's operators (cache_shim.cpp) and
-// their kernels (cache_rows.hip, cache_attention.hip).  Nothing here is part of the C-ABI.
+// their kernels (cache_rows.hip, cache_few.hip, cache_many.hip, cache_prompt.hip).  Nothing here is part of the C-ABI.
 #pragma once
 
 #include "cache_plan.hpp"

@@ -29,7 +29,7 @@ constexpr uint32_t many_rows(bool f32, uint32_t dim) { return f32 || dim > 128 ?
 constexpr uint32_t image_bytes(uint32_t held) { return 64 * (held * 2 + 16) + held * 144 + 1024; }
 // Images are made beforehand from so many rows a sequence on, if they take no more workspace than this.  Over 8192 keys
 // (bf16, 8 heads of the cache, 4 heads each): 64 tokens (256 rows) 74 us with images and 42 without, 128 tokens 77 and 70;
-// 16 prompts of up to 300 tokens 90 and 69; 256 tokens over 32768 keys 210 and 226; 8192 tokens 628 and 888.
+// 16 prompts of up to 300 tokens 90 and 69; 256 tokens over 32768 keys 210 and 226; 8192 tokens 628 and 719.
 constexpr uint64_t kImageRows = 1024, kMostImageBytes = 1ull << 30;
 
 struct AttentionLaunch {

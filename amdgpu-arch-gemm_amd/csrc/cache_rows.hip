@@ -30,7 +30,7 @@ __device__ __forceinline__ void angle(int position, float freq, float& c, float&
 // A work-group turns the heads of `p.step` tokens: sine and cosine once for each token and pair, into LDS, and then
 // items of eight pairs (or eight values, of neighbours and of those that stay).  An item's values are
 // read and written by one thread, two items' loads before their stores, so y may be x.  (16384 tokens of 40 heads of 128, BF16: two tokens
-// a work-group and two items at once 68.6 us, 4.9 TB/s; eight and four 79.1.)
+// a work-group and two items at once 68.5 us, 4.9 TB/s, a large copy's 5.1; eight and four 79.1.  One token: 3.1 us.)
 constexpr uint32_t kAngles = 2 * Q8_MAX_DIM / 2;
 struct RotaryPlan {
     Rotary p;
@@ -129,7 +129,8 @@ __device__ __forceinline__ void find_places(const Paged& c, uint32_t first, uint
     __syncthreads();
 }
 
-// Keys and values: G threads a head of eight values each, `step` tokens a work-group.
+// Keys and values: G threads a head of eight values each, `step` tokens a work-group.  (16384 tokens of 8 heads of 128, BF16: writing 27.7 us,
+// 3.6 TB/s, as a row's largest value lies between its loads and its stores; reading 18.9, 5.3 TB/s; a large copy 5.1.)
 constexpr uint32_t kMostStep = 16;
 struct CachePlan {
     CacheRows p;
@@ -214,8 +215,9 @@ template <int DT> hipError_t rotary_any(const RotaryPlan& a, hipStream_t s) {
 
 template <int DT, bool WRITE> hipError_t cache_any(const CacheRows& p, hipStream_t s) {
     const Paged& c = p.at;
-    // tokens a work-group: as many as leave each CU some work-groups
-    const uint32_t step = c.tokens >= 8192 ? 16 : c.tokens >= 2048 ? 2 : 1;
+    // Tokens a work-group, as many as leave each CU some work-groups (written and read, 8 heads of 128, us): 16384 tokens BF16 51.5 by 16
+    // and 56.5 by 8; 4096 16.9 by 4, 18.9 by 2, 21.0 by one; 2048 FP32 13.5, 12.4, 14.5; 1239 of 3 heads of 80 9.6 by 4 and 9.0 by one.
+    const uint32_t step = c.tokens >= 8192 ? 16 : c.tokens >= 4096 ? 4 : c.tokens >= 2048 ? 2 : 1;
     const CachePlan a = {p, step, divisor(c.heads)};
     const uint32_t groups = groups_for(c.tokens, step);
     if (c.dim <= 64) return launch(WRITE ? cache_write_kernel<DT, 8> : cache_read_kernel<DT, 8>, groups, a, s);
@@ -229,7 +231,8 @@ hipError_t launch_rotary(int dtype, const Rotary& p, hipStream_t s) {
     const q8_rotation& f = p.form;
     RotaryPlan a = {};
     a.p = p;
-    a.step = p.tokens >= 1024 ? 2 : 1;
+    // 40 heads of 128, BF16: 4096 tokens 15.3 us by two and 17.8 by one, 1024 tokens 7.0 and 6.3
+    a.step = p.tokens >= 2048 ? 2 : 1;
     a.turned = (uint32_t)ceil_div(f.neighbours ? 2 * f.pairs : f.pairs, 8);
     a.items = a.turned + (p.y == p.x ? 0 : (uint32_t)ceil_div(f.dim - 2 * f.pairs, 8));
     if (!a.items) return hipSuccess;
