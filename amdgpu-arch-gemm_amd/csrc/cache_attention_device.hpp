@@ -102,6 +102,9 @@ struct Place {
 __device__ __forceinline__ int pieces_of(const Place& t, uint32_t piece) {
     return (int)(((uint32_t)max(t.end - t.begin, 0) + piece - 1) / piece);
 }
+// The end of the piece that begins at key `begin`: by what is left, since a window's first key and a piece as long as the table
+// may pass 2^31 together.
+__device__ __forceinline__ int piece_end(const Place& t, int begin, uint32_t piece) { return begin + min(t.end - begin, (int)piece); }
 // The tile of slot `slot`, found by every wave for itself: tiles counted over 64 sequences at a time.
 __device__ __forceinline__ bool find_tile(const AttentionArgs& g, uint32_t slot, int height, Place& t) {
     const Paged& c = g.a.at;

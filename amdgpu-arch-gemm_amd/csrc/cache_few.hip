@@ -48,7 +48,7 @@ template <int DT, int DP> __global__ void __launch_bounds__(64 * kWaves, DP == 2
     const int pieces = max(1, pieces_of(t, g.piece));
     if ((int)piece >= pieces) return;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n = lane & 15, grp = lane >> 4;
-    const int begin = t.begin + (int)(piece * g.piece), end = min(t.end, begin + (int)g.piece);
+    const int begin = t.begin + (int)(piece * g.piece), end = piece_end(t, begin, g.piece);
 
     // this lane's row of the scores
     const bool mine = n < t.rows;

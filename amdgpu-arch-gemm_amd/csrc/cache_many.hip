@@ -37,7 +37,7 @@ __global__ void __launch_bounds__((Many<DT, DP>::THREADS), (Many<DT, DP>::W / 4)
     const int pieces = max(1, pieces_of(t, g.piece));
     if ((int)piece >= pieces) return;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), n = lane & 31, half = lane >> 5;
-    const int begin = t.begin + (int)(piece * g.piece), end = min(t.end, begin + (int)g.piece);
+    const int begin = t.begin + (int)(piece * g.piece), end = piece_end(t, begin, g.piece);
 
     // this lane's row; those past the tile's are its last
     const bool mine = wave * 32 + n < t.rows;

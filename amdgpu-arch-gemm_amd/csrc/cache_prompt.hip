@@ -104,7 +104,7 @@ template <int DT, int DP> __global__ void __launch_bounds__(kThreads, 1) prompt_
     const int pieces = max(1, pieces_of(t, g.piece));
     if ((int)piece >= pieces) return;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), n = lane & 31, half = lane >> 5;
-    const int begin = t.begin + (int)(piece * g.piece), end = min(t.end, begin + (int)g.piece);
+    const int begin = t.begin + (int)(piece * g.piece), end = piece_end(t, begin, g.piece);
 
     // Images on their way: a quarter of each by this wave.  begin + 64 * (image's number) is its first key.
     const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)lds;
