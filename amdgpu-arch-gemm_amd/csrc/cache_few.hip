@@ -35,7 +35,7 @@ template <int DT, int DP> struct Few {
     };
 };
 
-template <int DT, int DP> __global__ void __launch_bounds__(64 * kWaves, DP == 256 ? (DT == Q8_F32 ? 1 : 2) : DT == Q8_F32 ? 2 : 3) few_kernel(const AttentionArgs g) {
+template <int DT, int DP> __global__ void __launch_bounds__(64 * kWaves, DP == 256 ? (DT == Q8_F32 ? 1 : 2) : DT == Q8_F32 ? 2 : DP == 64 ? 4 : 3) few_kernel(const AttentionArgs g) {
     typedef Few<DT, DP> F;
     typedef typename Type<DT>::T T;
     constexpr int TERMS = F::TERMS, S = DP / 64, WORDS = F::WORDS;
@@ -199,14 +199,29 @@ template <int DT, int DP> __global__ void __launch_bounds__(64 * kWaves, DP == 2
                     if (!on) { score[e >> 2][e & 3] = -__builtin_huge_valf(); sk[e] = 1.0f; sv[e] = 0.0f; }
                 }
             }
-            float p[8], top = 0.0f;
+            float top, sum;
+            auto weigh = [&]() __attribute__((always_inline)) {
+                float p[8];
 #pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                p[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(score[e >> 2][e & 3], sk[e], -R));
-                w[e] = p[e] * sv[e];
-                top = e ? fmaxf(top, fabsf(w[e])) : fabsf(w[e]);
-            }
-            if (__any(!(top <= kTop))) {
+                for (int e = 0; e < 8; ++e) {
+                    p[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(score[e >> 2][e & 3], sk[e], -R));
+                    w[e] = p[e] * sv[e];
+                }
+                if (!whole) {
+#pragma unroll
+                    for (int e = 0; e < 8; ++e)
+                        if (!(seen >> e & 1)) p[e] = w[e] = 0.0f;
+                }
+                sum = l;
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    sum += p[e];
+                    top = e ? fmaxf(top, fabsf(w[e])) : fabsf(w[e]);
+                }
+            };
+            weigh();
+            // (a product with a scale of 0 may be no number, which fmaxf passes over; the exponential then is infinite)
+            if (__any(!(top <= kTop) || !(sum < __builtin_huge_valf()))) {
                 // R anew, from the row's largest; the four lanes of a row agree
                 float most = kUnset;
 #pragma unroll
@@ -221,19 +236,9 @@ template <int DT, int DP> __global__ void __launch_bounds__(64 * kWaves, DP == 2
                 l *= down;
 #pragma unroll
                 for (int j = 0; j < F::BYTES; ++j) o[j] *= down;
-#pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    p[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(score[e >> 2][e & 3], sk[e], -R));
-                    w[e] = p[e] * sv[e];
-                }
+                weigh();
             }
-            if (!whole) {
-#pragma unroll
-                for (int e = 0; e < 8; ++e)
-                    if (!(seen >> e & 1)) p[e] = w[e] = 0.0f;
-            }
-#pragma unroll
-            for (int e = 0; e < 8; ++e) l += p[e];
+            l = sum;
             u32x4 weight[TERMS];
             terms_of<TERMS, F::VH>(w, weight);
             auto multiply = [&](auto word) __attribute__((always_inline)) {

@@ -158,7 +158,8 @@ __global__ void __launch_bounds__((Many<DT, DP>::THREADS), (Many<DT, DP>::W / 4)
         };
         if (whole) weigh(Int<1>{});
         else weigh(Int<0>{});
-        if (__any(!(top <= kTop))) {
+        // (a product with a scale of 0 may be no number, which fmaxf passes over; the exponential then is infinite)
+        if (__any(!(top <= kTop) || !(l + sum < __builtin_huge_valf()))) {
             float most = kUnset;
             const uint32_t at = kept(scale_at);
 #pragma unroll

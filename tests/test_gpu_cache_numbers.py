@@ -1,0 +1,80 @@
+"""Attention where its arithmetic could leave FP32 or half precision, against float64: value scales of zero and far from one
+another, sums of very different weights, scores of any size."""
+import numpy as np
+import pytest
+
+from cache_reference import Case
+from q8_reference import TYPES, stored
+from shim import q8_cache as C
+from test_gpu_cache_attention import check
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def ops():
+    with C.Ops() as o:
+        yield o
+
+
+class Numbers(Case):
+    """Case, with any value scale, 0 among them."""
+
+    def attention(self, q, scale, window):
+        assert not window
+        group = self.heads // self.kv_heads
+        q = q.reshape(-1, self.heads, self.dim)
+        out, lse = np.zeros(q.shape), np.full(q.shape[:2], -np.inf)
+        spread, products, steps = np.zeros(q.shape), np.zeros(q.shape[:2]), np.zeros(q.shape)
+        self.values = np.zeros(q.shape)         # the sum of the |8-bit values| of the keys that are seen
+        for b, token, p in self.rows():
+            at = np.arange(p + 1)
+            page, slot = self.table[b, at // self.page].astype(np.int64), at % self.page
+            for h in range(self.heads):
+                g = h // group
+                k = self.k[page, g, slot, : self.dim].astype(np.float64) * self.sk[page, g, slot].astype(np.float64)[:, None]
+                v, sv = self.v[page, g, slot, : self.dim].astype(np.float64), self.sv[page, g, slot].astype(np.float64)
+                t = k @ q[token, h] * scale
+                m = t.max()
+                w = np.exp(t - m)
+                total = w.sum()
+                out[token, h] = (w * sv) @ v / total
+                lse[token, h] = m + np.log(total)
+                spread[token, h] = (w * sv) @ np.abs(v) / total
+                self.values[token, h] = np.abs(v).sum(0)
+                steps[token, h] = (w * sv).max() * self.values[token, h] / total
+                products[token, h] = (np.abs(k) @ np.abs(q[token, h])).max() * abs(scale)
+        return out, lse, (spread, products, steps)
+
+    def bounds(self, out, lse, sums, dtype):
+        """Case's, and where values are next to nothing beside the sum of the weights: a weight times its scale is then below
+        2^6 and off by half of half precision's least step, 2^-25, while the sum is 2^106 at the least (the row's reference is
+        2^106 below a weight whose value is that small)."""
+        off, off_lse = super().bounds(out, lse, sums, dtype)
+        return off + 2.0 ** -131 * self.values * (1.0 if dtype != "f32" else 0.0), off_lse
+
+
+# Tiles of few rows, one piece and several; of many; images.
+WAYS = {"few": [(1, 5), (1, 100), (1, 129)], "pieces": [(1, 2000)], "few and many": [(3, 5), (70, 100), (40, 129)], "many": [(90, 700)],
+        "images": [(520, 620)]}
+
+
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("way", list(WAYS))
+def test_value_scales_of_zero(ops, dtype, way):
+    """No values at all; values of some keys only, whose scores are far below and far above the others'."""
+    rng = np.random.default_rng(3)
+    case = Numbers(rng, WAYS[way], 4, 2, 64, 16)
+    held = case.sv.copy()
+    case.sv[:] = 0
+    check(ops, rng, case, dtype)
+    for sign in (0, -1, 1):
+        case.sv = held.copy()
+        none = rng.random(case.sv.shape) < 0.5
+        case.sv[none] = 0
+        q = stored(rng.normal(0, 0.3, (case.tokens, 4 * 64)), dtype)
+        if sign:        # scores of the keys without values are 140 nats below or above the others'
+            case.sk[:] = 0.02
+            case.k[..., 0] = np.where(none, sign * 127, 0)
+            q[:, ::64] = 448
+        check(ops, rng, case, dtype, q=q)
