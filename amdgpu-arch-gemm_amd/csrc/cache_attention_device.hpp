@@ -6,7 +6,9 @@
 //     t_rj = (q_r . k_j) (sk_j scale log2 e),  p_rj = 2^(t_rj - R_r),  l_r = sum p_rj,  O_r = sum (p_rj sv_j) v_j
 // over the 8-bit k_j and v_j, which 16 bits hold exactly.  R_r is no less than the largest t_rj + log2 sv_j by more
 // than a fixed distance, so that p_rj sv_j fits half precision whatever the scales; it moves, and l and O with it, only
-// where a product would pass 2^15.  out = O / l, lse = (R + log2 l) / log2 e.
+// where a product would pass 2^15, or the sum of the p_rj 2^120: those of keys with small values, or none, may be that
+// large.  A scale below 2^-100 counts as that in R, and p_rj are 2^106 at most where R was just set.
+// out = O / l, lse = (R + log2 l) / log2 e.
 //
 // The scores are taken transposed, keys by rows: a lane then has four keys of each 16 for one row, which as they
 // are make the operand of the second product, O^T = V^T P^T, as the order of the keys in its sum is free.
@@ -23,6 +25,10 @@ constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 constexpr float kUnset = -0x1p127f;         // R of a row that has seen no key
 constexpr float kTop = 0x1p15f;             // the largest p sv
 constexpr float kRoom = 6.0f;               // log2 of it where R was just set
+constexpr float kLeastScale = 0x1p-100f;    // of values, as R takes them
+// The largest sum of p of a lane, and how far R moves where it comes near without a p that moves R: a row's lanes and waves
+// may be added, and 2^31 keys' products stay above half precision's least step.
+constexpr float kMostSum = 0x1p120f, kSpare = 8.0f;
 
 // Half precision (H) or BF16, eight values of the summed index a lane.
 template <bool H> __device__ __forceinline__ void mfma16(u32x4 a, u32x4 b, f32x4& c) {
@@ -195,6 +201,31 @@ template <int DT> __device__ __forceinline__ void query(const typename Type<DT>:
             v[e] = d + e < dim ? x : 0.0f;
         }
     }
+}
+
+// What a score and the scales of its key ask of R.
+__device__ __forceinline__ float wanted(float score, float sk, float sv) {
+    return __builtin_fmaf(score, sk, __builtin_amdgcn_logf(fmaxf(fabsf(sv), kLeastScale)));
+}
+// The largest of a row's lanes, which are APART and so on to 64 apart.
+template <int APART> __device__ __forceinline__ float of_row(float x) {
+#pragma unroll
+    for (int m = APART; m < 64; m *= 2) x = fmaxf(x, __shfl_xor(x, m));
+    return x;
+}
+// R anew, the same for a row's lanes: `most` of the lane's keys is wanted, and moves R from `slack` above it on; l is the lane's sum.
+template <int APART> __device__ __forceinline__ float moved(float R, float l, float most, float slack) {
+    most = of_row<APART>(most);
+    const bool full = of_row<APART>(l) > 0.5f * kMostSum;
+    return most > R + slack ? most - kRoom : full ? R + kSpare : R;
+}
+// A piece's sums, so that those of thousands of pieces can be added: the factor for O.
+__device__ __forceinline__ float settle(float& R, float& l) {
+    const bool large = l > 0x1p64f;
+    R += large ? 32.0f : 0.0f;
+    const float down = large ? 0x1p-32f : 1.0f;
+    l *= down;
+    return down;
 }
 
 // Sums of some keys with those of others.

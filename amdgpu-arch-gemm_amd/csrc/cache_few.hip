@@ -221,16 +221,13 @@ template <int DT, int DP> __global__ void __launch_bounds__(64 * kWaves, DP == 2
             };
             weigh();
             // (a product with a scale of 0 may be no number, which fmaxf passes over; the exponential then is infinite)
-            if (__any(!(top <= kTop) || !(sum < __builtin_huge_valf()))) {
+            if (__any(!(top <= kTop) || !(sum <= kMostSum))) {
                 // R anew, from the row's largest; the four lanes of a row agree
                 float most = kUnset;
 #pragma unroll
                 for (int e = 0; e < 8; ++e)
-                    if (seen >> e & 1)
-                        most = fmaxf(most, __builtin_fmaf(score[e >> 2][e & 3], sk[e], __builtin_amdgcn_logf(fmaxf(fabsf(sv[e]), 0x1p-100f))));
-                most = fmaxf(most, __shfl_xor(most, 16));
-                most = fmaxf(most, __shfl_xor(most, 32));
-                const float next = most > R + kRoom ? most - kRoom : R;
+                    if (seen >> e & 1) most = fmaxf(most, wanted(score[e >> 2][e & 3], sk[e], sv[e]));
+                const float next = moved<16>(R, l, most, kRoom);
                 const float down = __builtin_amdgcn_exp2f(R - next);
                 R = next;
                 l *= down;
@@ -303,8 +300,9 @@ template <int DT, int DP> __global__ void __launch_bounds__(64 * kWaves, DP == 2
         if (pieces > 1) {
             const Row at = row_of(g, t, kv, r);
             const uint64_t to = ((uint64_t)piece * c.tokens + at.row) * a.heads + at.head;
+            const float down = settle(most, total);
 #pragma unroll
-            for (int e = 0; e < 8; e += 2) publish(g.sums + to * DP + d + e, v[e], v[e + 1]);
+            for (int e = 0; e < 8; e += 2) publish(g.sums + to * DP + d + e, v[e] * down, v[e + 1] * down);
             if (d == 0) publish(g.stats + 2 * to, most, total);
         } else {
             finish(r, d, most, total, v);

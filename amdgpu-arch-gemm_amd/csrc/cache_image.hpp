@@ -109,11 +109,13 @@ __device__ __forceinline__ void put_row(const AttentionArgs& g, const Row& at, u
     const uint64_t to = at.row * a.heads + at.head;
     if (pieces > 1) {       // join_kernel's
         const uint64_t own = (uint64_t)piece * a.at.tokens * a.heads + to;
+        const float down = settle(R, l);
 #pragma unroll
         for (int d = 0; d < DP / 32; ++d)
 #pragma unroll
             for (int i = 0; i < 16; i += 4)
-                *reinterpret_cast<f32x4*>(g.sums + own * DP + d * 32 + i * 2 + half * 4) = f32x4{o[d][i], o[d][i + 1], o[d][i + 2], o[d][i + 3]};
+                *reinterpret_cast<f32x4*>(g.sums + own * DP + d * 32 + i * 2 + half * 4) =
+                    f32x4{o[d][i] * down, o[d][i + 1] * down, o[d][i + 2] * down, o[d][i + 3] * down};
         if (half == 0) {
             g.stats[2 * own] = R;
             g.stats[2 * own + 1] = l;

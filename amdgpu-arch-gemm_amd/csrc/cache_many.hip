@@ -159,7 +159,7 @@ __global__ void __launch_bounds__((Many<DT, DP>::THREADS), (Many<DT, DP>::W / 4)
         if (whole) weigh(Int<1>{});
         else weigh(Int<0>{});
         // (a product with a scale of 0 may be no number, which fmaxf passes over; the exponential then is infinite)
-        if (__any(!(top <= kTop) || !(l + sum < __builtin_huge_valf()))) {
+        if (__any(!(top <= kTop) || !(l + sum <= kMostSum))) {
             float most = kUnset;
             const uint32_t at = kept(scale_at);
 #pragma unroll
@@ -168,12 +168,10 @@ __global__ void __launch_bounds__((Many<DT, DP>::THREADS), (Many<DT, DP>::W / 4)
                 scales_of(at, e, sk, sv);
 #pragma unroll
                 for (int z = 0; z < 4; ++z) {
-                    const float x = __builtin_fmaf(score[e + z], sk[z], __builtin_amdgcn_logf(fmaxf(fabsf(sv[z]), 0x1p-100f)));
-                    most = seen >> (e + z) & 1 ? fmaxf(most, x) : most;
+                    most = seen >> (e + z) & 1 ? fmaxf(most, wanted(score[e + z], sk[z], sv[z])) : most;
                 }
             }
-            most = fmaxf(most, __shfl_xor(most, 32));
-            const float next = most > R + kRoom ? most - kRoom : R;
+            const float next = moved<32>(R, l, most, kRoom);
             const float down = __builtin_amdgcn_exp2f(R - next);
             R = next;
             l *= down;

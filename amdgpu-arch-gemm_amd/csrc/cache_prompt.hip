@@ -222,7 +222,7 @@ template <int DT, int DP> __global__ void __launch_bounds__(kThreads, 1) prompt_
         read(PRODUCTS - 1);
 #pragma unroll
         for (int y = 0; y < EACH_WEIGHTS; ++y) weigh((PRODUCTS - 1) * EACH_WEIGHTS + y);
-        if (__builtin_expect(__any(too_large(top)), 0)) {
+        if (__builtin_expect(__any(too_large(top) || !(l[B] + sum <= kMostSum)), 0)) {
             uint32_t seen = 0xffff;
             if (edge) {
                 // bits 8 q + 4 half + z, of keys up to this row's position and from its window's first
@@ -239,12 +239,10 @@ template <int DT, int DP> __global__ void __launch_bounds__(kThreads, 1) prompt_
                 read_scales(here, e / 4, ks, vs);
 #pragma unroll
                 for (int z = 0; z < 4; ++z) {
-                    const float x = __builtin_fmaf(score[B][e + z], ks[z], __builtin_amdgcn_logf(fmaxf(fabsf(vs[z]), 0x1p-100f)));
-                    most = seen >> (e + z) & 1 ? fmaxf(most, x) : most;
+                    most = seen >> (e + z) & 1 ? fmaxf(most, wanted(score[B][e + z], ks[z], vs[z])) : most;
                 }
             }
-            most = fmaxf(most, __shfl_xor(most, 32));
-            const float next = most > R[B] + (15.0f - kRoom) ? most - kRoom : R[B];
+            const float next = moved<32>(R[B], l[B], most, 15.0f - kRoom);
             if (__any(next != R[B])) {
                 const float down = __builtin_amdgcn_exp2f(R[B] - next);
                 R[B] = next;

@@ -78,3 +78,62 @@ def test_value_scales_of_zero(ops, dtype, way):
             case.k[..., 0] = np.where(none, sign * 127, 0)
             q[:, ::64] = 448
         check(ops, rng, case, dtype, q=q)
+
+
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("way", list(WAYS))
+@pytest.mark.parametrize("rise", [8.3, 14.0, 15.0, 40.0])
+def test_rows_without_values_and_scores_that_grow(ops, dtype, way, rise):
+    """Keys and values as q8_cache_write stores them: no values up to three quarters of a sequence, the scores there rising by
+    `rise` nats, then values whose scores are the largest, and 14 nats below it."""
+    rng = np.random.default_rng(int(rise))
+    case = Numbers(rng, WAYS[way], 4, 2, 64, 16)
+    cache, batch = case.upload()
+    lengths = case.lengths
+    whole = C.Batch(C.ints(np.concatenate([[0], np.cumsum(lengths)])), batch.memory[1], batch.memory[2], len(lengths), int(lengths.sum()), case.width)
+    for below in (0.0, 14.0):
+        k, v = rng.normal(0, 0.02, (int(lengths.sum()), 2, 64)), rng.normal(0.5, 1, (int(lengths.sum()), 2, 64))
+        at = 0
+        for n in lengths:
+            part = np.arange(n) / max(1, 0.75 * n)
+            k[at:at + n, :, 0] = np.where(part < 1, part * rise, rise - below)[:, None]
+            v[at:at + n][part < 1] = 0
+            at += n
+        ops.cache_write(C.F32, cache, whole, C.Array.of(k.reshape(-1, 128)), C.Array.of(v.reshape(-1, 128)))
+        ops.synchronize()
+        case.k, case.v, case.sk, case.sv = case.download()
+        assert (case.sv == np.float32(2.0 ** -126)).sum() >= 2 * sum(int(0.75 * n) for n in lengths)
+        q = stored(rng.normal(0, 0.3, (case.tokens, 4 * 64)), dtype)
+        q[:, ::64] = 8          # with the scale, dim^-1/2, one score a unit of the first value
+        check(ops, rng, case, dtype, q=q)
+
+
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("sequences", [[(1, 200), (1, 161)] * 130, [(40, 64), (33, 64)], *list(WAYS.values())[1:]],
+                         ids=["one piece", "one piece of many", *list(WAYS)[1:]])
+@pytest.mark.parametrize("where", ["later", "second half"])
+def test_sums_of_lanes_and_pieces(ops, dtype, sequences, where):
+    """No values, and a few scores 14.1 nats, 20.3 bits, above those that come first: exponentials of 2^106 and then 2^126.3, two
+    of which FP32 holds and four not.  They are two of one lane and two of another, in a row's second 32 keys or far behind."""
+    rng = np.random.default_rng(6)
+    case = Numbers(rng, sequences, 4, 2, 64, 16)
+    case.sv[:] = 2.0 ** -126
+    case.v[:] = 0
+    case.k[..., 0] = 0
+    case.sk[:] = 0.001
+    for b, (_, length) in enumerate(case.sequences):
+        for p in range(length):
+            if p % 16 in (0, 4) and (128 <= p < 160 if where == "later" else p % 64 >= 32):
+                page, slot = case.place(b, p)
+                case.k[page, :, slot, 0] = 47
+    q = stored(rng.normal(0, 0.3, (case.tokens, 4 * 64)), dtype)
+    q[:, ::64] = 2400       # 2400 * 47 * 0.001 / 8 = 14.1
+    check(ops, rng, case, dtype, q=q)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("way", list(WAYS))
+@pytest.mark.parametrize("scale", [2.0 ** -115, 2.0 ** -100, 2.0 ** 100])
+def test_values_near_the_ends_of_fp32(ops, dtype, way, scale):
+    rng = np.random.default_rng(5)
+    check(ops, rng, Numbers(rng, WAYS[way], 4, 2, 64, 16, scale=scale), dtype)
