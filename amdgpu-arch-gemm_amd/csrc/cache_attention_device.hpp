@@ -26,6 +26,7 @@ constexpr float kUnset = -0x1p127f;         // R of a row that has seen no key
 constexpr float kTop = 0x1p15f;             // the largest p sv
 constexpr float kRoom = 6.0f;               // log2 of it where R was just set
 constexpr float kLeastScale = 0x1p-100f;    // of values, as R takes them
+constexpr float kWide = 0x1p24f;            // scores that leave R no room for the rest
 // The largest sum of p of a lane, and how far R moves where it comes near without a p that moves R: a row's lanes and waves
 // may be added, and 2^31 keys' products stay above half precision's least step.
 constexpr float kMostSum = 0x1p120f, kSpare = 8.0f;
@@ -203,21 +204,84 @@ template <int DT> __device__ __forceinline__ void query(const typename Type<DT>:
     }
 }
 
-// What a score and the scales of its key ask of R.
-__device__ __forceinline__ float wanted(float score, float sk, float sv) {
-    return __builtin_fmaf(score, sk, __builtin_amdgcn_logf(fmaxf(fabsf(sv), kLeastScale)));
+// R as it moves.  Scores of 2^24 and more leave no room in FP32 for 2^15 beside them: R is then the largest score, as FP32
+// holds it, and `rest` what else belongs to the reference, R + rest.  The kernels' steps know it as -infinity then: every
+// exponential is infinite, or no number, and comes to where R moves, as do those of a row that has seen no key.
+struct Far {
+    float base, rest;           // R and what else
+};
+struct Reference {
+    float R;                    // kUnset: no key seen; -infinity: `far` has it
+    Far far;
+    __device__ __forceinline__ Reference(float r, const Far* kept_far) : R(r), far{r, 0.0f} {
+        if (__builtin_expect(__any(is_far()), 0) && is_far()) far = *kept_far;
+    }
+    __device__ __forceinline__ bool is_far() const { return R == -__builtin_huge_valf(); }
+    __device__ __forceinline__ void keep(Far* kept_far) const {
+        if (__builtin_expect(__any(is_far()), 0) && is_far()) *kept_far = far;
+    }
+};
+// A score rounded, without the operation that follows.
+__device__ __forceinline__ float rounded(float score, float sk) {
+    float t = score * sk;
+    asm("" : "+v"(t));
+    return t;
 }
+__device__ __forceinline__ float exponent(const Reference& r, float score, float sk) {
+    return r.is_far() ? (rounded(score, sk) - r.far.base) - r.far.rest : __builtin_fmaf(score, sk, -r.R);
+}
+__device__ __forceinline__ float log_scale(float sv) { return __builtin_amdgcn_logf(fmaxf(fabsf(sv), kLeastScale)); }
 // The largest of a row's lanes, which are APART and so on to 64 apart.
 template <int APART> __device__ __forceinline__ float of_row(float x) {
 #pragma unroll
     for (int m = APART; m < 64; m *= 2) x = fmaxf(x, __shfl_xor(x, m));
     return x;
 }
-// R anew, the same for a row's lanes: `most` of the lane's keys is wanted, and moves R from `slack` above it on; l is the lane's sum.
-template <int APART> __device__ __forceinline__ float moved(float R, float l, float most, float slack) {
+// The reference anew, the same for a row's lanes; returns the factor for their sums.  `keys` calls what it is given with each of the
+// lane's keys: whether the row sees it, its score, its scales.  The reference moves where one asks for `slack` more
+// than it is; l is the lane's sum.
+template <int APART, typename Keys> __device__ __forceinline__ float moved(Reference& r, float l, float slack, const Keys& keys) {
+    float most = kUnset;
+    keys([&](bool on, float score, float sk, float sv) __attribute__((always_inline)) {
+        most = on ? fmaxf(most, __builtin_fmaf(score, sk, log_scale(sv))) : most;
+    });
     most = of_row<APART>(most);
-    const bool full = of_row<APART>(l) > 0.5f * kMostSum;
-    return most > R + slack ? most - kRoom : full ? R + kSpare : R;
+    bool full = false;
+    if (__builtin_expect(__any(l > 0.5f * kMostSum), 0)) full = of_row<APART>(l) > 0.5f * kMostSum;
+    const float before = r.far.base;
+    const float next = most > before + slack ? most - kRoom : full ? before + kSpare : before;
+    float down = __builtin_amdgcn_exp2f(before - next);
+    const bool wide = r.is_far() || !(fabsf(next) < kWide || next == kUnset);
+    if (__builtin_expect(__any(wide), 0)) {
+        float top = kUnset, want = kUnset;
+        keys([&](bool on, float score, float sk, float) __attribute__((always_inline)) { top = on ? fmaxf(top, rounded(score, sk)) : top; });
+        const float base = fmaxf(before, of_row<APART>(top)), old = (before - base) + r.far.rest;
+        keys([&](bool on, float score, float sk, float sv) __attribute__((always_inline)) {
+            want = on ? fmaxf(want, (rounded(score, sk) - base) + log_scale(sv)) : want;
+        });
+        want = of_row<APART>(want) - kRoom;
+        const float rest = want > old + (slack - kRoom) ? want : full ? old + kSpare : old;
+        if (wide) {
+            down = 1.0f;
+            if (rest > old || base != before) {
+                const bool fits = fabsf(base) < kWide;
+                const Far now = fits ? Far{base + rest, 0.0f} : Far{base, rest};
+                down = __builtin_amdgcn_exp2f((before - now.base) + (r.far.rest - now.rest));
+                r.R = fits ? now.base : -__builtin_huge_valf();
+                r.far = now;
+            }
+            return down;
+        }
+    }
+    r.R = next;
+    return down;
+}
+// Sums whose reference is R alone: the factor for O.  The p then are 2^(t - R), R the largest t or so.
+__device__ __forceinline__ float without_rest(const Reference& r, float& R, float& l) {
+    R = r.far.base;
+    const float up = __builtin_amdgcn_exp2f(r.far.rest);
+    l *= up;
+    return up;
 }
 // A piece's sums, so that those of thousands of pieces can be added: the factor for O.
 __device__ __forceinline__ float settle(float& R, float& l) {

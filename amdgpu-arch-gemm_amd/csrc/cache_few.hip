@@ -40,6 +40,7 @@ template <int DT, int DP> __global__ void __launch_bounds__(64 * kWaves, DP == 2
     typedef typename Type<DT>::T T;
     constexpr int TERMS = F::TERMS, S = DP / 64, WORDS = F::WORDS;
     __shared__ typename F::Shared shared;
+    __shared__ Far fars[kWaves][16];
     const Attention& a = g.a;
     const Paged& c = a.at;
     const uint32_t kv = blockIdx.x % c.heads, piece = blockIdx.y;
@@ -200,11 +201,11 @@ template <int DT, int DP> __global__ void __launch_bounds__(64 * kWaves, DP == 2
                 }
             }
             float top, sum;
-            auto weigh = [&]() __attribute__((always_inline)) {
+            auto weigh = [&](auto exponent_of) __attribute__((always_inline)) {
                 float p[8];
 #pragma unroll
                 for (int e = 0; e < 8; ++e) {
-                    p[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(score[e >> 2][e & 3], sk[e], -R));
+                    p[e] = __builtin_amdgcn_exp2f(exponent_of(score[e >> 2][e & 3], sk[e]));
                     w[e] = p[e] * sv[e];
                 }
                 if (!whole) {
@@ -219,21 +220,27 @@ template <int DT, int DP> __global__ void __launch_bounds__(64 * kWaves, DP == 2
                     top = e ? fmaxf(top, fabsf(w[e])) : fabsf(w[e]);
                 }
             };
-            weigh();
+            auto less_R = [&](float t, float k) __attribute__((always_inline)) { return __builtin_fmaf(t, k, -R); };
+            weigh(less_R);
             // (a product with a scale of 0 may be no number, which fmaxf passes over; the exponential then is infinite)
             if (__any(!(top <= kTop) || !(sum <= kMostSum))) {
-                // R anew, from the row's largest; the four lanes of a row agree
-                float most = kUnset;
+                Reference r(R, &fars[wave][kept((uint32_t)n)]);
+                const float down = moved<16>(r, l, kRoom, [&](auto each) __attribute__((always_inline)) {
+                    const uint32_t mask = kept(seen);
 #pragma unroll
-                for (int e = 0; e < 8; ++e)
-                    if (seen >> e & 1) most = fmaxf(most, wanted(score[e >> 2][e & 3], sk[e], sv[e]));
-                const float next = moved<16>(R, l, most, kRoom);
-                const float down = __builtin_amdgcn_exp2f(R - next);
-                R = next;
+                    for (int e = 0; e < 8; ++e) each(mask >> e & 1, score[e >> 2][e & 3], sk[e], sv[e]);
+                });
+                R = r.R;
+                r.keep(&fars[wave][kept((uint32_t)n)]);
                 l *= down;
 #pragma unroll
                 for (int j = 0; j < F::BYTES; ++j) o[j] *= down;
-                weigh();
+                if (__builtin_expect(__any(r.is_far()), 0)) {
+                    const Reference wide(R, &fars[wave][kept((uint32_t)n)]);
+                    weigh([&](float t, float k) __attribute__((always_inline)) { return exponent(wide, t, k); });
+                } else {
+                    weigh(less_R);
+                }
             }
             l = sum;
             u32x4 weight[TERMS];
@@ -265,6 +272,9 @@ template <int DT, int DP> __global__ void __launch_bounds__(64 * kWaves, DP == 2
     // the waves' sums: each lane has values 8 (4 grp + i) .. of row n (DP 128), and of l what its keys had
     l += __shfl_xor(l, 16);
     l += __shfl_xor(l, 32);
+    const float up = without_rest(Reference(R, &fars[wave][n]), R, l);
+#pragma unroll
+    for (int j = 0; j < F::BYTES; ++j) o[j] *= up;
     __syncthreads();        // every wave is done with its stage
     typename F::Sums& sums = shared.sums;
     if (grp == 0) { sums.r[wave][n] = R; sums.l[wave][n] = l; }

@@ -102,14 +102,15 @@ template <int ROWS> __device__ __forceinline__ bool find_rows(const AttentionArg
 
 // A row's result, or its sums of one of several pieces: a lane has of each 32 values 8 i + 4 half .. + 3, i = 0 .. 3.
 template <int DT, int DP>
-__device__ __forceinline__ void put_row(const AttentionArgs& g, const Row& at, uint32_t piece, int pieces, int half, float R, float l,
+__device__ __forceinline__ void put_row(const AttentionArgs& g, const Row& at, uint32_t piece, int pieces, int half, const Reference& r, float l,
                                         const f32x16 (&o)[DP / 32]) {
     typedef typename Type<DT>::T T;
     const Attention& a = g.a;
     const uint64_t to = at.row * a.heads + at.head;
     if (pieces > 1) {       // join_kernel's
         const uint64_t own = (uint64_t)piece * a.at.tokens * a.heads + to;
-        const float down = settle(R, l);
+        float R;
+        const float up = without_rest(r, R, l), down = settle(R, l) * up;
 #pragma unroll
         for (int d = 0; d < DP / 32; ++d)
 #pragma unroll
@@ -131,7 +132,7 @@ __device__ __forceinline__ void put_row(const AttentionArgs& g, const Row& at, u
             const uint32_t x = d * 32 + (i >> 2) * 8 + half * 4 + (i & 3);
             if (x < a.at.dim) Type<DT>::put(out + x, o[d][i] * part);
         }
-    if (a.lse && half == 0) a.lse[to] = l == 0.0f ? -__builtin_huge_valf() : (R + __builtin_log2f(l)) * kLn2;
+    if (a.lse && half == 0) a.lse[to] = l == 0.0f ? -__builtin_huge_valf() : (r.far.base + (r.far.rest + __builtin_log2f(l))) * kLn2;
 }
 
 // The pieces' sums of a tile's rows: DP / 8 threads a row, 2048 / DP rows a work-group.  (A work-group of the kernel before

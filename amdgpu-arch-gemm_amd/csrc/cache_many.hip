@@ -29,6 +29,7 @@ __global__ void __launch_bounds__((Many<DT, DP>::THREADS), (Many<DT, DP>::W / 4)
     constexpr bool CARRY = IMAGES > 2;
     __shared__ __attribute__((aligned(1024))) char lds[IMAGES * F::BYTES];
     __shared__ uint64_t offsets[F::W][64];
+    __shared__ Far fars[F::W][32];
     const Attention& a = g.a;
     const Paged& c = a.at;
     const uint32_t kv = blockIdx.x % c.heads, piece = blockIdx.y;
@@ -139,7 +140,7 @@ __global__ void __launch_bounds__((Many<DT, DP>::THREADS), (Many<DT, DP>::W / 4)
             seen = (mask & 0xf) | (mask >> 4 & 0xf0) | (mask >> 8 & 0xf00) | (mask >> 12 & 0xf000);
         }
         float w[16], sum = 0.0f, top = 0.0f;
-        auto weigh = [&](auto all) __attribute__((always_inline)) {
+        auto weigh = [&](auto all, auto exponent_of) __attribute__((always_inline)) {
             const uint32_t at = kept(scale_at);
 #pragma unroll
             for (int e = 0; e < 16; e += 4) {
@@ -148,7 +149,7 @@ __global__ void __launch_bounds__((Many<DT, DP>::THREADS), (Many<DT, DP>::W / 4)
 #pragma unroll
                 for (int z = 0; z < 4; ++z) {
                     const bool on = all.value || (seen >> (e + z) & 1);
-                    float p = __builtin_amdgcn_exp2f(__builtin_fmaf(score[e + z], sk[z], -R));
+                    float p = __builtin_amdgcn_exp2f(exponent_of(score[e + z], sk[z]));
                     p = on ? p : 0.0f;
                     w[e + z] = on ? p * sv[z] : 0.0f;
                     sum = e + z ? sum + p : p;
@@ -156,28 +157,34 @@ __global__ void __launch_bounds__((Many<DT, DP>::THREADS), (Many<DT, DP>::W / 4)
                 }
             }
         };
-        if (whole) weigh(Int<1>{});
-        else weigh(Int<0>{});
+        auto less_R = [&](float t, float k) __attribute__((always_inline)) { return __builtin_fmaf(t, k, -R); };
+        if (whole) weigh(Int<1>{}, less_R);
+        else weigh(Int<0>{}, less_R);
         // (a product with a scale of 0 may be no number, which fmaxf passes over; the exponential then is infinite)
         if (__any(!(top <= kTop) || !(l + sum <= kMostSum))) {
-            float most = kUnset;
-            const uint32_t at = kept(scale_at);
+            Reference r(R, &fars[wave][kept((uint32_t)n)]);
+            const float down = moved<32>(r, l, kRoom, [&](auto each) __attribute__((always_inline)) {
+                const uint32_t at = kept(scale_at), mask = kept(seen);
 #pragma unroll
-            for (int e = 0; e < 16; e += 4) {
-                f32x4 sk, sv;
-                scales_of(at, e, sk, sv);
+                for (int e = 0; e < 16; e += 4) {
+                    f32x4 sk, sv;
+                    scales_of(at, e, sk, sv);
 #pragma unroll
-                for (int z = 0; z < 4; ++z) {
-                    most = seen >> (e + z) & 1 ? fmaxf(most, wanted(score[e + z], sk[z], sv[z])) : most;
+                    for (int z = 0; z < 4; ++z) each(mask >> (e + z) & 1, score[e + z], sk[z], sv[z]);
+                    if (e == 4) __builtin_amdgcn_sched_barrier(0);      // half of the scales in registers at a time
                 }
-            }
-            const float next = moved<32>(R, l, most, kRoom);
-            const float down = __builtin_amdgcn_exp2f(R - next);
-            R = next;
+            });
+            R = r.R;
+            r.keep(&fars[wave][kept((uint32_t)n)]);
             l *= down;
 #pragma unroll
             for (int d = 0; d < D; ++d) o[d] *= down;
-            weigh(Int<0>{});
+            if (__builtin_expect(__any(r.is_far()), 0)) {
+                const Reference wide(R, &fars[wave][kept((uint32_t)n)]);
+                weigh(Int<0>{}, [&](float t, float k) __attribute__((always_inline)) { return exponent(wide, t, k); });
+            } else {
+                weigh(Int<0>{}, less_R);
+            }
         }
         l += sum;
 #pragma unroll
@@ -266,7 +273,7 @@ __global__ void __launch_bounds__((Many<DT, DP>::THREADS), (Many<DT, DP>::W / 4)
 
     l += __shfl_xor(l, 32);
     if (!mine) return;
-    put_row<DT, DP>(g, row_of(g, t, kv, (int)kept((uint32_t)in_tile)), piece, pieces, half, R, l, o);
+    put_row<DT, DP>(g, row_of(g, t, kv, (int)kept((uint32_t)in_tile)), piece, pieces, half, Reference(R, &fars[wave][n]), l, o);
 }
 
 template <int DT, int DP> hipError_t run(const AttentionArgs& g, uint32_t pieces, hipStream_t s) {

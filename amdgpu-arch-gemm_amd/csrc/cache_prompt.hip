@@ -96,6 +96,7 @@ template <int DT, int DP> __global__ void __launch_bounds__(kThreads, 1) prompt_
     typedef typename Type<DT>::T T;
     constexpr int S = DP / 16, D = DP / 32, PRODUCTS = S + 2 * D;
     __shared__ __attribute__((aligned(1024))) char lds[kImages * F::BYTES];
+    __shared__ Far fars[kWaves][2][32];
     const Attention& a = g.a;
     const Paged& c = a.at;
     const uint32_t kv = blockIdx.x % c.heads, piece = blockIdx.y;
@@ -232,20 +233,21 @@ template <int DT, int DP> __global__ void __launch_bounds__(kThreads, 1) prompt_
                 seen = (mask & 0xf) | (mask >> 4 & 0xf0) | (mask >> 8 & 0xf00) | (mask >> 12 & 0xf000);
             }
             const uint32_t here = kept(scales);
-            float most = kUnset;
+            Reference r(R[B], &fars[wave][B][kept((uint32_t)n)]);
+            const float down = moved<32>(r, l[B], 15.0f - kRoom, [&](auto each) __attribute__((always_inline)) {
+                const uint32_t mask = kept(seen);
 #pragma unroll
-            for (int e = 0; e < 16; e += 4) {
-                f32x4 ks, vs;
-                read_scales(here, e / 4, ks, vs);
+                for (int e = 0; e < 16; e += 4) {
+                    f32x4 ks, vs;
+                    read_scales(here, e / 4, ks, vs);
 #pragma unroll
-                for (int z = 0; z < 4; ++z) {
-                    most = seen >> (e + z) & 1 ? fmaxf(most, wanted(score[B][e + z], ks[z], vs[z])) : most;
+                    for (int z = 0; z < 4; ++z) each(mask >> (e + z) & 1, score[B][e + z], ks[z], vs[z]);
+                    if (DP == 64 && e == 4) __builtin_amdgcn_sched_barrier(0);      // half of the scales in registers at a time
                 }
-            }
-            const float next = moved<32>(R[B], l[B], most, 15.0f - kRoom);
-            if (__any(next != R[B])) {
-                const float down = __builtin_amdgcn_exp2f(R[B] - next);
-                R[B] = next;
+            });
+            R[B] = r.R;
+            r.keep(&fars[wave][B][kept((uint32_t)n)]);
+            if (__any(down != 1.0f)) {
                 l[B] *= down;
 #pragma unroll
                 for (int d = 0; d < D; ++d) {
@@ -254,21 +256,30 @@ template <int DT, int DP> __global__ void __launch_bounds__(kThreads, 1) prompt_
                     asm volatile("" : "+a"(o[B][d]));
                 }
             }
-            sum = 0.0f;
+            auto again = [&](auto exponent_of) __attribute__((always_inline)) {
+                sum = 0.0f;
 #pragma unroll
-            for (int e = 0; e < 16; e += 4) {
-                f32x4 ks, vs;
-                read_scales(here, e / 4, ks, vs);
+                for (int e = 0; e < 16; e += 4) {
+                    f32x4 ks, vs;
+                    read_scales(here, e / 4, ks, vs);
 #pragma unroll
-                for (int z = 0; z < 4; ++z) {
-                    const bool on = seen >> (e + z) & 1;
-                    p[z] = __builtin_amdgcn_exp2f(__builtin_fmaf(score[B][e + z], ks[z], -R[B]));
-                    p[z] = on ? p[z] : 0.0f;
-                    vs[z] = on ? vs[z] : 0.0f;
-                    sum += p[z];
-                    p[z] *= vs[z];
-                    if (z % 2) weight[B][e / 8][(e + z) / 2 % 4] = halved(p[z - 1], p[z]);
+                    for (int z = 0; z < 4; ++z) {
+                        const bool on = seen >> (e + z) & 1;
+                        p[z] = __builtin_amdgcn_exp2f(exponent_of(score[B][e + z], ks[z]));
+                        p[z] = on ? p[z] : 0.0f;
+                        vs[z] = on ? vs[z] : 0.0f;
+                        sum += p[z];
+                        p[z] *= vs[z];
+                        if (z % 2) weight[B][e / 8][(e + z) / 2 % 4] = halved(p[z - 1], p[z]);
+                    }
+                    if (DP == 64 && e == 4) __builtin_amdgcn_sched_barrier(0);
                 }
+            };
+            if (__builtin_expect(__any(r.is_far()), 0)) {
+                const Reference wide(R[B], &fars[wave][B][kept((uint32_t)n)]);
+                again([&](float t, float k) __attribute__((always_inline)) { return exponent(wide, t, k); });
+            } else {
+                again([&](float t, float k) __attribute__((always_inline)) { return __builtin_fmaf(t, k, -R[B]); });
             }
         }
         l[B] += sum;
@@ -326,7 +337,7 @@ template <int DT, int DP> __global__ void __launch_bounds__(kThreads, 1) prompt_
         const int r = wave * 64 + b * 32 + n;
         if (r >= t.rows) continue;
         const Row at = row_of(g, t, kv, r);
-        put_row<DT, DP>(g, at, piece, pieces, half, R[b], l[b], o[b]);
+        put_row<DT, DP>(g, at, piece, pieces, half, Reference(R[b], &fars[wave][b][n]), l[b], o[b]);
     }
 }
 

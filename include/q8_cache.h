@@ -110,9 +110,10 @@ int q8_cache_read(q8_handle* h, int dtype, const q8_cache* cache, const q8_batch
  *     lse = log sum_j exp(t_j)           (FP32, tokens x heads; may be NULL)
  * with scale in -2^100 .. 2^100.
  * A row that attends to nothing is 0, its lse -infinity; one of a NaN scale that it sees is NaN.
- * Rows of no chunk are left as they are.  The scores are FP32 values; one below -2^100 counts as
- * not there.  Sums are in FP32; exp(t_j) sv_j is rounded to 11 bits before its product with the
- * 8-bit values, in Q8_F32 not at all. */
+ * Rows of no chunk are left as they are.  The scores are FP32 values of any size; one below -2^100 counts
+ * as not there.  Sums are in FP32; exp(t_j) sv_j, sv_j the scale of v_j, is rounded to 11 bits before its product with
+ * the 8-bit values, or to 2^-31 of the row's largest exp(t_i) max(|sv_i|, 2^-100); in Q8_F32 not at all.  An exp(t_j)
+ * below 2^-132 of that largest product counts as 0.  Scales may be 0. */
 int q8_attention(q8_handle* h, int dtype, const q8_cache* cache, const q8_batch* batch, uint32_t heads, const void* q,
                  uint32_t ldq, float scale, uint32_t window, void* out, uint32_t ldo, float* lse);
 

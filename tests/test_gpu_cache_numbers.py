@@ -4,7 +4,7 @@ import numpy as np
 import pytest
 
 from cache_reference import Case
-from q8_reference import TYPES, stored
+from q8_reference import TINY, TYPES, UNIT, stored
 from shim import q8_cache as C
 from test_gpu_cache_attention import check
 
@@ -137,3 +137,61 @@ def test_sums_of_lanes_and_pieces(ops, dtype, sequences, where):
 def test_values_near_the_ends_of_fp32(ops, dtype, way, scale):
     rng = np.random.default_rng(5)
     check(ops, rng, Numbers(rng, WAYS[way], 4, 2, 64, 16, scale=scale), dtype)
+
+
+class Scores(Numbers):
+    """Scores that FP32 holds exactly: q and the keys' scales are powers of two, and a key's first value is all that q meets."""
+
+    def bounds(self, out, lse, sums, dtype):
+        """Keys that a row sees differ by whole steps of the scores, 2^16 nats and more, or not at all: those of the largest score
+        have one weight, the others none, and the scores' roundings, which are the same for equal ones, touch lse only.  So `out` is
+        off by the weights' rounding to 11 bits (FP32: 2^-22), the exponentials' 2^-22 and as many roundings as there are keys in
+        numerator and sum.  Up to 2^24 the reference is off its place by a unit at most, so the row's largest weight is 2^5 or more when it
+        is rounded, and half precision's least step 2^-30 of it.  lse: six factors and terms, each rounded to 2^-24."""
+        keys = max([1] + [int(n) for n in self.lengths])
+        spread, _, steps = sums
+        rel = 1.01 * ((2.0 ** -11 if dtype != "f32" else 2.0 ** -22) + 2.0 ** -21 + 2 * (keys + 8) * 2.0 ** -24)
+        off = spread * rel + (0 if dtype == "f32" else 1.01 * 2.0 ** -30 * steps + 2.0 ** -131 * self.values)
+        return off + (np.abs(out) + off) * UNIT[dtype] + TINY[dtype], 8 * 2.0 ** -24 * np.abs(lse) + (keys + 16) * 2.0 ** -23
+
+
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("way", list(WAYS))
+@pytest.mark.parametrize("step", [2.0 ** 16, 2.0 ** 20, 2.0 ** 25, 2.0 ** 30, 2.0 ** 60, 2.0 ** 90])
+def test_scores_of_any_size(ops, dtype, way, step):
+    """Up to 100 such steps above and below zero, in any order along the keys, rising, falling, and none above zero; value scales that
+    differ by up to 2^69."""
+    rng = np.random.default_rng(9)
+    case = Scores(rng, WAYS[way], 4, 2, 64, 16)
+    case.sk[:] = step
+    case.sv *= np.exp2(rng.integers(-60, 9, case.sv.shape)).astype(np.float32)
+    q = np.zeros((case.tokens, 4 * 64))
+    q[:, ::64] = 8          # with the scale, dim^-1/2, one step of the scores a unit of a key's first value
+    q[:, 64] = -8           # one head sees them the other way round
+    for order in ("any", "rising", "falling", "below"):
+        case.k[..., 0] = rng.integers(-100, 1 if order == "below" else 101, case.k.shape[:3])
+        for b, (_, length) in enumerate(case.sequences):
+            if order in ("rising", "falling"):
+                for p in range(length):
+                    page, slot = case.place(b, p)
+                    case.k[page, :, slot, 0] = (1 if order == "rising" else -1) * (200 * p // length - 100)
+        check(ops, rng, case, dtype, q=q)
+
+
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("way", list(WAYS))
+def test_one_score_a_little_above_large_ones(ops, dtype, way):
+    """Scores of 2^24, all the same, and one key's 2^9 above them: a row is the mean of the values that it sees, or that key's."""
+    rng = np.random.default_rng(10)
+    case = Scores(rng, WAYS[way], 4, 2, 64, 16)
+    case.sk[:] = 2.0 ** 18
+    case.sv[:] = 1 / 64
+    case.k[..., 0] = 64
+    q = np.zeros((case.tokens, 4 * 64))
+    q[:, ::64] = 8
+    case.k[..., 1] = 0
+    for b, (_, length) in enumerate(case.sequences):
+        page, slot = case.place(b, length // 3)
+        case.k[page, :, slot, 1] = 64
+    q[:, 1::64] = 2.0 ** -12         # 2^18 2^-12 64 / 8 = 2^9
+    check(ops, rng, case, dtype, q=q)
