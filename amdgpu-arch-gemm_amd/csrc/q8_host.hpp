@@ -73,6 +73,18 @@ inline bool capturing(hipStream_t stream) {
     return hipStreamIsCapturing(stream, &s) != hipSuccess || s != hipStreamCaptureStatusNone;
 }
 
+// While it lives, this thread's allocations are none of other streams' captures, which they would end.
+class BesideCaptures {
+public:
+    BesideCaptures() { (void)hipThreadExchangeStreamCaptureMode(&mode_); }
+    ~BesideCaptures() { (void)hipThreadExchangeStreamCaptureMode(&mode_); }
+    BesideCaptures(const BesideCaptures&) = delete;
+    BesideCaptures& operator=(const BesideCaptures&) = delete;
+
+private:
+    hipStreamCaptureMode mode_ = hipStreamCaptureModeRelaxed;      // then the thread's own
+};
+
 inline bool is_type(int dtype) { return dtype == Q8_F32 || dtype == Q8_F16 || dtype == Q8_BF16; }
 
 // A matrix argument: rows of cols values at ld, `bytes` each.

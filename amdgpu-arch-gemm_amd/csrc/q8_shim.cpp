@@ -52,6 +52,7 @@ int q8_open(q8_handle** out) {
     if (hipGetDeviceCount(&count) != hipSuccess || count < 1) return fail(SGEMM_E_NO_DEVICE, "no HIP device is visible");
     q8_handle* h = new (std::nothrow) q8_handle;
     if (!h) return fail(SGEMM_E_INVALID, "out of host memory");
+    const BesideCaptures beside;
     hipError_t e = hipGetDevice(&h->device);
     if (e == hipSuccess) e = hipStreamCreate(&h->own_stream);
     // no call loads code: a first one may be under capture, and should not take longer than the next
