@@ -40,8 +40,8 @@ def test_opened_during_a_capture(mode, thread):
             else:
                 opened.append(C.Ops())
         finally:
-            gc.enable()
             exe = hip.end(stream)
+            gc.enable()
         assert len(opened) == 1
         with opened[0] as b:
             b.attention(C.BF16, cache, batch, 4, q, outs[2])
