@@ -15,7 +15,8 @@ constexpr uint32_t kManyKeys = 64;
 constexpr uint32_t kFewMost = 64;
 // Tiles whose keys are taken in pieces, at the most: each has a ticket in the handle.
 constexpr uint32_t kTickets = 1u << 16;
-// Pieces: the grid's second dimension ends at 65535, the grid at 2^32 work-items; and their sums stay small beside a cache.
+// Pieces: the grid's second dimension ends at 65535, the grid at 2^32 work-items (kMostGroups work-groups of 256); and their
+// sums stay small beside a cache.
 constexpr uint64_t kMostPieces = 4096, kMostGroups = (1u << 24) - 1, kMostSumBytes = 1ull << 28;
 
 constexpr uint64_t up(uint64_t a, uint64_t b) { return (a + b - 1) / b; }
@@ -37,6 +38,7 @@ struct AttentionLaunch {
     uint32_t least = 0, most = UINT32_MAX;
     uint32_t piece = 0;         // keys of a piece
     uint32_t pieces = 1;        // of the longest sequence
+    uint64_t most_groups = kMostGroups;
 };
 struct AttentionPlan {
     AttentionLaunch few, many;
@@ -51,7 +53,7 @@ inline void cut(AttentionLaunch& l, uint64_t heads, uint64_t tiles, uint64_t key
                 uint64_t at_most) {
     const uint64_t steps = up(keys ? keys : 1, step);
     uint64_t most = groups / tiles ? groups / tiles : 1;
-    const uint64_t limits[] = {steps, at_most, kMostGroups / (l.slots * heads), l.slots * heads > kTickets ? 1 : kMostPieces};
+    const uint64_t limits[] = {steps, at_most, l.most_groups / (l.slots * heads), l.slots * heads > kTickets ? 1 : kMostPieces};
     if (most < up(keys, longest)) most = up(keys, longest);
     for (uint64_t limit : limits)
         if (most > limit) most = limit ? limit : 1;
@@ -83,6 +85,7 @@ inline AttentionPlan plan_attention(bool f32, uint64_t tokens, uint64_t seqs, ui
         const uint32_t height = many_rows(f32, dim);
         const uint64_t own = rows / kFewMost < filled ? rows / kFewMost : filled;      // sequences of more rows than few
         p.many.slots = (uint32_t)(rows / height + (own ? own : 1));
+        p.many.most_groups = kMostGroups * 128 / height;      // two work-items a row
         // One work-group a CU, two where their registers and images are small; twice that of several sequences, whose tiles
         // end at different times (4 of 512 tokens over up to 8192 keys: 311 us, in 1024 work-groups 346).  FP32, 512 tokens
         // over 2048 keys: 85 us in two pieces, 147 in one; heads of 256, 1024 tokens over 4096: 203 and 381.  A piece costs its

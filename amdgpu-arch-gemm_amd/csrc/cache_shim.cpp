@@ -104,9 +104,8 @@ int plan(int dtype, const q8_cache& c, const q8_batch& b, uint32_t heads, Attent
     CHECK(check_columns(heads, c.dim));
     if ((uint64_t)b.tokens * heads >= (1ull << 31)) return fail(SGEMM_E_SHAPE, "%u tokens of %u heads: rows have 31 bits", b.tokens, heads);
     p = plan_attention(dtype == Q8_F32, b.tokens, b.seqs, (uint64_t)b.width * c.page_tokens, b.longest, heads, c.heads, c.dim);
-    // 2^32 work-items are one grid's end
     for (const AttentionLaunch* l : {&p.few, &p.many})
-        if ((uint64_t)l->slots * c.heads * l->pieces >= (1u << 24))
+        if ((uint64_t)l->slots * c.heads * l->pieces > l->most_groups)
             return fail(SGEMM_E_SHAPE, "%u tokens of %u heads are more tiles than a grid holds", b.tokens, heads);
     return SGEMM_OK;
 }

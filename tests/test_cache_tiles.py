@@ -2,6 +2,11 @@
 import os
 import subprocess
 
+import pytest
+
+from shim import q8_cache as C
+from shim import sgemm_shim as S
+
 ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 CSRC = os.path.join(ROOT, "amdgpu-arch-gemm_amd", "csrc")
 
@@ -82,3 +87,13 @@ def test_every_row_has_a_tile(tmp_path):
                     "-o", str(tmp_path / "tiles")], check=True)
     out = subprocess.run([str(tmp_path / "tiles")], capture_output=True, text=True)
     assert out.returncode == 0 and out.stdout.strip() == "ok 1", out.stdout + out.stderr
+
+
+def test_no_grid_passes_2_to_the_32_work_items():
+    """A tile of many rows has eight waves, 2^23 of them are more than a grid holds: such sizes are refused before a launch."""
+    cache = C.Cache(None, None, None, None, 4, 16, 64, 1)
+    for seqs in (1, 2):
+        C.attention_workspace(C.BF16, cache, C.Batch(None, None, None, seqs, 2 ** 24, 8), 64)
+        with pytest.raises(S.SgemmError) as e:
+            C.attention_workspace(C.BF16, cache, C.Batch(None, None, None, seqs, 2 ** 25 - 1, 8), 64)
+        assert e.value.code == -4 and "grid" in e.value.message
