@@ -8,7 +8,7 @@ namespace {
 // turn from memory to registers, and their sums meet in LDS at the end.  Of a step's keys, lane l has the
 // 16-byte pieces l / 16 of key l % 16 for the scores, and DP / 16 values of eight keys for the second product, those
 // whose weights it has.  DP: values of a head, those past dim are 0 in q and left out at the end.
-// (32 heads of 128 on 8 of the cache: 64 sequences of up to 8192 keys 132 us, 4.7 TB/s; one of 131072 64, 4.3; one of 4096 13, which
+// (32 heads of 128 on 8 of the cache: 64 sequences of up to 8192 keys 134 us, 4.7 TB/s; one of 131072 64, 4.3; one of 4096 13, which
 // is latency: launch and tile 5, pages, keys and products 6, the join of 32 pieces 2.)
 constexpr int kWaves = 4;
 template <int DT, int DP> struct Few {

@@ -11,8 +11,10 @@ template <bool H> __device__ __forceinline__ void mfma32(u32x4 a, u32x4 b, f32x1
 
 // A work-group of W waves has a tile of 32 W rows, 32 a wave, and takes 64 keys a step, whose image it makes itself in LDS: half
 // of the waves load and convert the values, the others the keys, while steps before are computed.  Bounded by the latency of few
-// work-groups' steps (64 tokens of 32 heads of 128 over 8192 keys, BF16: 42 us; 5 chunks of up to 77 over 1501, FP32: 20.5), in FP32
-// and with heads of 256 by spilled registers too (FP32, 512 tokens over 2048 keys: 85 us).
+// work-groups' steps (64 tokens of 32 heads of 128 over 8192 keys, BF16: 41 us; 5 chunks of up to 77 over 1501, FP32: 20.9).  FP32
+// takes three products for one and leaves a SIMD one wave (400 registers; 512 tokens over 2048 keys 84 us, the products alone
+// 38; a prompt of 2048 169 and 86).  Heads of 256 spill registers, FP32 134 and 16-bit types 9 (BF16, 16 heads, 1024 tokens over
+// 4096 keys: 173 us, the products 50).
 template <int DT, int DP> struct Many : Image<DT, DP> {
     static constexpr int TERMS = DT == Q8_F32 ? 3 : 1, W = (int)many_rows(DT == Q8_F32, DP) / 32, THREADS = 64 * W;
 };

@@ -30,7 +30,8 @@ constexpr uint32_t many_rows(bool f32, uint32_t dim) { return f32 || dim > 128 ?
 constexpr uint32_t image_bytes(uint32_t held) { return 64 * (held * 2 + 16) + held * 144 + 1024; }
 // Images are made beforehand from so many rows a sequence on, if they take no more workspace than this.  Over 8192 keys
 // (bf16, 8 heads of the cache, 4 heads each): 64 tokens (256 rows) 74 us with images and 42 without, 128 tokens 77 and 70;
-// 16 prompts of up to 300 tokens 90 and 69; 256 tokens over 32768 keys 210 and 226; 8192 tokens 628 and 719.
+// 16 prompts of up to 300 tokens 90 and 69; 256 tokens over 32768 keys 210 and 226; 8192 tokens 628 and 719.  Their workspace, too, is
+// by the table's width: 16 prompts of 2048 take 1053 us, and with a table for 32768 positions, without images, 1109.
 constexpr uint64_t kImageRows = 1024, kMostImageBytes = 1ull << 30;
 
 struct AttentionLaunch {
@@ -48,7 +49,9 @@ struct AttentionPlan {
 };
 
 // The keys of a sequence in pieces: as many as make `groups` work-groups of `tiles`, and none longer than `longest` keys; at
-// most `at_most`, and no more than a grid of the slots and the `heads` of the cache can hold.
+// most `at_most`, and no more than a grid of the slots and the `heads` of the cache can hold.  `keys` is the table's width, as
+// the host does not know the lengths, so a table far wider than they are makes pieces too long (a token over 4096 keys takes
+// 13.5 us with a table for 4096 or 32768 positions and 28 with one for 131072; 8 such sequences 21, 46 and 61).
 inline void cut(AttentionLaunch& l, uint64_t heads, uint64_t tiles, uint64_t keys, uint64_t step, uint64_t groups, uint64_t longest,
                 uint64_t at_most) {
     const uint64_t steps = up(keys ? keys : 1, step);
@@ -88,7 +91,7 @@ inline AttentionPlan plan_attention(bool f32, uint64_t tokens, uint64_t seqs, ui
         p.many.most_groups = kMostGroups * 128 / height;      // two work-items a row
         // One work-group a CU, two where their registers and images are small; twice that of several sequences, whose tiles
         // end at different times (4 of 512 tokens over up to 8192 keys: 311 us, in 1024 work-groups 346).  FP32, 512 tokens
-        // over 2048 keys: 85 us in two pieces, 147 in one; heads of 256, 1024 tokens over 4096: 203 and 381.  A piece costs its
+        // over 2048 keys: 85 us in two pieces, 147 in one.  A piece costs its
         // sums' way through memory: 64 tokens over 8192 keys take 42 us in 16 pieces, 54 in 32.
         const uint64_t each_cu = !f32 && dim <= 64 ? 512 : 256;
         cut(p.many, kv_heads, (seqs > 1 ? p.many.slots : up(rows, height)) * kv_heads, keys, kManyKeys,

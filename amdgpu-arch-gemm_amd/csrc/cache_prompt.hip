@@ -84,9 +84,10 @@ __device__ __forceinline__ uint32_t larger(uint32_t x, uint32_t y) {
 __device__ __forceinline__ bool too_large(uint32_t m) { return ((m + 0x08000800u | m) & 0x80008000u) != 0; }
 
 // A wave has 64 rows, A and B of 32, so that keys and values are read from LDS once for both.  (8192 tokens of 32 heads of 128, BF16:
-// 623 us, 0.88 PFLOP/s, with the images' 14; eight waves of 32 rows on the same images 680; many_kernel 719; a large library product
-// 1.2 PFLOP/s.  Bound by issue: a wave alone on its SIMD issues some 117 instructions a turn, of which the 16 matrix instructions are busy 41%
-// of the cycles, without bank conflicts.)  For each 32 keys h there are two turns of 16 matrix instructions (heads of 128), between each two of which
+// 633 us, 0.87 PFLOP/s, with the images' 14; eight waves of 32 rows on the same images 680; many_kernel 719; a large library product
+// 1.2 PFLOP/s.  A turn of 16 matrix and some 100 vector instructions takes about 1200 cycles, without bank conflicts.  Matrix instructions
+// are busy 41% of the cycles and vector instructions 43%: the two hardly overlap.  A wave is alone on its SIMD, for its registers, and a turn's
+// scores are one chain of products through one accumulator; which of the two keeps the units apart was not measured.)  For each 32 keys h there are two turns of 16 matrix instructions (heads of 128), between each two of which
 // are the vector instructions of one or two weights of the other rows:
 //     scores of B(h), results of B(h - 1)   with the weights of A(h)
 //     scores of A(h + 1), results of A(h)   with the weights of B(h)

@@ -129,8 +129,8 @@ __device__ __forceinline__ void find_places(const Paged& c, uint32_t first, uint
     __syncthreads();
 }
 
-// Keys and values: G threads a head of eight values each, `step` tokens a work-group.  (16384 tokens of 8 heads of 128, BF16: writing 27.7 us,
-// 3.6 TB/s, as a row's largest value lies between its loads and its stores; reading 18.9, 5.3 TB/s; a large copy 5.1.)
+// Keys and values: G threads a head of eight values each, `step` tokens a work-group.  (16384 tokens of 8 heads of 128, BF16: writing 27.6 us,
+// 3.6 TB/s: a thread has one load of 16 bytes on its way, in 16 passes that wait for one another; reading 19.0, 5.3 TB/s; a large copy 5.1.)
 constexpr uint32_t kMostStep = 16;
 struct CachePlan {
     CacheRows p;

@@ -73,10 +73,12 @@ enum {
 
 typedef struct q8_handle q8_handle;
 
-/* A handle on the current device, with a stream of its own. */
+/* A handle on the current device, with a stream of its own.  Streams may be
+ * capturing meanwhile. */
 int q8_open(q8_handle** out);
 
-/* Waits for the handle's work and releases its stream and workspace. */
+/* Waits for the handle's work and releases its stream and workspace.  (Both end
+ * a capture that is under way.) */
 void q8_close(q8_handle* h);
 
 /* As sgemm_set_stream: later calls run on `stream` (of the handle's device; the
