@@ -195,3 +195,34 @@ def test_one_score_a_little_above_large_ones(ops, dtype, way):
         case.k[page, :, slot, 1] = 64
     q[:, 1::64] = 2.0 ** -12         # 2^18 2^-12 64 / 8 = 2^9
     check(ops, rng, case, dtype, q=q)
+
+
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("way", list(WAYS))
+@pytest.mark.parametrize("dim", [80, 128, 256])
+def test_the_same_with_wider_heads(ops, dtype, way, dim):
+    """Scores of up to 2^37 that rise along the keys, value scales of 0, and exponentials that FP32 holds two of, on the kernels for more than 64
+    values a head."""
+    rng = np.random.default_rng(dim)
+    scores = Scores(rng, WAYS[way], 4, 2, dim, 16)
+    q = np.zeros((scores.tokens, 4 * dim))
+    q[:, ::dim] = 8
+    scores.sk[:] = 2.0 ** 30
+    for b, (_, length) in enumerate(scores.sequences):
+        for p in range(length):
+            page, slot = scores.place(b, p)
+            scores.k[page, :, slot, 0] = 200 * p // length - 100
+    check(ops, rng, scores, dtype, q=q, scale=0.125)
+    case = Numbers(rng, WAYS[way], 4, 2, dim, 16)
+    case.sv[rng.random(case.sv.shape) < 0.5] = 0
+    check(ops, rng, case, dtype)
+    case.sv[:], case.v[:], case.sk[:] = 2.0 ** -126, 0, 0.001
+    case.k[..., 0] = 0
+    for b, (_, length) in enumerate(case.sequences):
+        for p in range(length):
+            if p % 16 in (0, 4) and p % 64 >= 32:
+                page, slot = case.place(b, p)
+                case.k[page, :, slot, 0] = 47
+    q = stored(rng.normal(0, 0.3, (case.tokens, 4 * dim)), dtype)
+    q[:, ::dim] = 2400
+    check(ops, rng, case, dtype, q=q, scale=0.125)
